@@ -8,6 +8,7 @@ models/experts.py, models/multiway_transformer.py:44-55):
 All computation happens in hand-written HIP kernels (eve_amd/csrc, gfx950) reached through
 the C ABI of libeve_moe.so (include/eve_moe.h).
 """
+from .attn import attention, self_attention
 from .encoder import (Attention, MultiwayTransformerEncoder, MultiwayTransformerEncoderLayer,
                       MultiwayTransformerEnocderLayer, eve_base_encoder)
 from .experts import ACT2FN, Experts, MultiwayTransformerMLP, QuickGELU
@@ -19,4 +20,4 @@ from .sharded_moe import DeviceNoise, MOELayer, TopKGate, gumbel_rsample, top2ga
 
 __all__ = ["Attention", "DeviceNoise", "MultiwayTransformerEncoder", "MultiwayTransformerEncoderLayer", "MultiwayTransformerEnocderLayer",
            "eve_base_encoder", "MoE", "GraphedTrainStep", "ModalitySplitFFN", "MOELayer", "TopKGate", "Experts", "MultiwayTransformerMLP", "QuickGELU", "ACT2FN",
-           "gumbel_rsample", "top2gating", "retrieval"]
+           "attention", "gumbel_rsample", "self_attention", "top2gating", "retrieval"]

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_double, c_float, c_int, c_size_t, c_void_p, c_long
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p, c_long
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libeve_moe.so")
@@ -17,7 +17,7 @@ LIB_PATH = os.environ.get("EVE_MOE_LIB", LIB_PATH)  # A/B experiments: an altern
 F32, BF16 = 0, 1
 MODE_NONE, MODE_VL, MODE_VISION, MODE_TEXT = 0, 1, 2, 3
 ACT_QUICK_GELU, ACT_GELU, ACT_RELU, ACT_IDENTITY = 0, 1, 2, 3
-ABI_VERSION = 11
+ABI_VERSION = 12
 FFN_SHARED_GPU = 1
 
 _P, _I, _Z = c_void_p, c_int, c_size_t
@@ -62,6 +62,10 @@ SIGNATURES = {
     "eve_moe_finish_fwd": (c_int, [_P, _P, _P, _Z, _P, _P]),
     "eve_moe_finish_bwd": (c_int, [_P, _P, _P, _P, _Z, _P, _P, _P]),
     "eve_moe_route_bwd": (c_int, [_P] * 9 + [_Z] + [_P] * 5 + [_Z, _P]),
+    "eve_attn_fwd_workspace_bytes": (c_size_t, [_P]),
+    "eve_attn_fwd": (c_int, [_P] * 9 + [_Z, _P]),
+    "eve_attn_bwd_workspace_bytes": (c_size_t, [_P]),
+    "eve_attn_bwd": (c_int, [_P] * 14 + [_Z, _P]),
 }
 MOE_PASS_INFERENCE, MOE_PASS_FORWARD, MOE_PASS_BACKWARD = 0, 1, 2
 MOE_PASS_ROUTE_FWD, MOE_PASS_ROUTE_BWD = 3, 4
@@ -72,6 +76,17 @@ MOE_SAVED_FIELDS = ("gates", "idx", "loc", "slot", "weight", "slot_token", "slot
 class MoEShape(ctypes.Structure):
     """`eve_moe_shape` of include/eve_moe.h."""
     _fields_ = [(n, c_int) for n in ("S", "T", "n_vis", "mode", "M", "I", "E", "C", "act", "dtype", "embed_dtype")]
+
+
+class AttnShape(ctypes.Structure):
+    """`eve_attn_shape` of include/eve_moe.h."""
+    _fields_ = [(n, c_int) for n in ("B", "Nq", "Nk", "H", "Hkv", "D", "dtype")] + [("scale", c_float)]
+
+
+class AttnLayout(ctypes.Structure):
+    """`eve_attn_layout` of include/eve_moe.h."""
+    _fields_ = [(n, c_int64) for n in ("q_b", "q_n", "q_h", "k_b", "k_n", "k_h", "v_b", "v_n", "v_h")]
+
 
 _lib = None
 

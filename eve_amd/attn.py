@@ -1,0 +1,112 @@
+"""Attention of the encoder layer on the library's kernels (eve_attn_fwd / eve_attn_bwd; the reference's explicit
+`softmax(q.float() @ k.float().T) @ v`, models/multiway_transformer.py:112-128): one pass over the keys forward, the
+probabilities recomputed backward, a key mask, heads that share keys and values.  No CPU fallback.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+def _check_mask(key_mask: Optional[Tensor], B: int, Nk: int, device) -> Optional[Tensor]:
+    if key_mask is None:
+        return None
+    if tuple(key_mask.shape) != (B, Nk):
+        raise ValueError(f"eve_amd.attention: `key_mask` has shape {tuple(key_mask.shape)}, the keys need {(B, Nk)}")
+    if key_mask.device != device:
+        raise RuntimeError(f"eve_amd.attention: `key_mask` is on {key_mask.device}, the queries on {device}")
+    return key_mask.bool().contiguous()
+
+
+def _check(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor], scale: Optional[float]):
+    """-> (key_mask, scale) as the kernels take them; shapes and types first, then the device."""
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 4:
+            raise ValueError(f"eve_amd.attention: `{n}` must be [B, N, heads, width], got {tuple(t.shape)}")
+    ops._dt(q)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"eve_amd.attention: q, k and v have types {q.dtype}, {k.dtype}, {v.dtype}: one is needed")
+    B, _, H, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"eve_amd.attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not belong together")
+    Nk, Hkv = k.shape[1], k.shape[2]
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise ValueError(f"eve_amd.attention: {H} query heads cannot share {Hkv} key/value heads")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"eve_amd.attention: head width {D} (a multiple of 8 up to 128 is supported)")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"eve_amd.attention: scale {scale} (must be positive and finite)")
+    key_mask = _check_mask(key_mask, B, Nk, q.device)
+    if not q.is_cuda or k.device != q.device or v.device != q.device:
+        raise RuntimeError(f"eve_amd.attention runs on one MI355X (inputs on {q.device}, {k.device}, {v.device}); no CPU fallback")
+    return key_mask, scale
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, key_mask, scale):  # type: ignore[override]
+        q, k, v = ops.attn_readable(q), ops.attn_readable(k), ops.attn_readable(v)
+        need = any(ctx.needs_input_grad[:3])
+        out, lse = ops.attn_fwd(q, k, v, key_mask, scale, want_lse=need)
+        if need:
+            ctx.save_for_backward(q, k, v, key_mask, out, lse)
+            ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):  # type: ignore[override]
+        q, k, v, key_mask, out, lse = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        ops.attn_bwd(dout.contiguous(), q, k, v, key_mask, out, lse, ctx.scale, dq, dk, dv)
+        return dq, dk, dv, None, None
+
+
+class _SelfAttentionFn(torch.autograd.Function):
+    """The three parts of one [B, N, 3, H, D] product, read where they lie; their gradient in one tensor of that shape."""
+
+    @staticmethod
+    def forward(ctx, qkv, key_mask, scale):  # type: ignore[override]
+        if qkv.numel() and (qkv.stride(4) != 1 or any(ops.attn_readable(t) is not t for t in qkv.unbind(2))):
+            qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
+        q, k, v = qkv.unbind(2)
+        need = ctx.needs_input_grad[0]
+        out, lse = ops.attn_fwd(q, k, v, key_mask, scale, want_lse=need)
+        if need:
+            ctx.save_for_backward(qkv, key_mask, out, lse)
+            ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):  # type: ignore[override]
+        qkv, key_mask, out, lse = ctx.saved_tensors
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        ops.attn_bwd(dout.contiguous(), *qkv.unbind(2), key_mask, out, lse, ctx.scale, *dqkv.unbind(2))
+        return dqkv, None, None
+
+
+def attention(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor] = None, scale: Optional[float] = None) -> Tensor:
+    """softmax(scale q k^T) v over the keys that `key_mask` leaves, differentiable in q, k and v.
+
+    q [B, Nq, H, D]; k, v [B, Nk, Hkv, D], float32 or bfloat16, at any strides (read in place where the last dimension is
+    contiguous and rows start on 16-byte boundaries, else copied); H a multiple of Hkv: head h reads key head h // (H // Hkv).
+    D is a multiple of 8 up to 128.  key_mask [B, Nk]: nonzero = visible.  scale: D ** -0.5 unless given, positive.
+    -> [B, Nq, H, D].  A sample without a visible key gives zeros and passes no gradient; masked keys and values may hold
+    anything, NaN included.  Scores and sums are float32; results do not depend on the order of execution."""
+    key_mask, scale = _check(q, k, v, key_mask, scale)
+    return _AttentionFn.apply(q, k, v, key_mask, scale)
+
+
+def self_attention(qkv: Tensor, key_mask: Optional[Tensor] = None, scale: Optional[float] = None) -> Tensor:
+    """`attention` over the three parts of one product qkv [B, N, 3, H, D] -> [B, N, H, D]; the gradient comes in qkv's shape."""
+    if qkv.dim() != 5 or qkv.shape[2] != 3:
+        raise ValueError(f"eve_amd.self_attention: `qkv` must be [B, N, 3, heads, width], got {tuple(qkv.shape)}")
+    key_mask, scale = _check(*qkv.unbind(2), key_mask, scale)
+    return _SelfAttentionFn.apply(qkv, key_mask, scale)

@@ -1,0 +1,775 @@
+// Attention of the encoder layer (reference models/multiway_transformer.py:99-132) and its gradient, gfx950.
+//
+//   s_ij = scale q_i . k_j,   p_ij = keep_j exp(s_ij - m_i) / sum_j,   o_i = sum_j p_ij v_j
+// in one pass over the keys with a running maximum and sum; the forward keeps L_i = m_i + log2 sum (base 2), from which the
+// backward recomputes p_ij = 2^(s_ij c - L_i), c = scale log2 e:
+//   delta_i = do_i . o_i,   ds_ij = p_ij (do_i . v_j - delta_i),
+//   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i.
+//
+// Rows.  The query heads that share a key/value head are rows of ONE problem: row i of (sample, kv head) is query i / G of head
+// kvhead * G + i % G, G = H / Hkv.  A key tile is then read once for all of them, and one query of G heads fills G columns of a
+// matrix instruction instead of one.
+//
+// Operand layout.  v_mfma_f32_32x32x16_bf16 (and, per 4 of them, v_mfma_f32_32x32x2_f32) leave in lane l column l & 31 and rows
+// (r & 3) + 8 (r >> 2) + 4 (l >> 5).  Every product is oriented so that the softmax index is the COLUMN (query in the forward and
+// dq kernels, key in the dk/dv kernel): maxima and sums are then register reductions plus one exchange between the wave's halves,
+// and the probabilities are, as they lie, the B operand of the next product: its contraction index may be taken in any order as
+// long as the A operand follows, so chunk c of a 32-row accumulator supplies rows 16c + 4h + {0..3} and 16c + 8 + 4h + {0..3} (bf16)
+// and the A operand is read from LDS in that order (ds_read_b64_tr_b16: four rows of one column each).
+//
+// LDS rows are padded by 16 bytes, which serves both the 16-byte row reads and the transposed reads.
+// No atomics: dq and dk/dv have a kernel each (7 products instead of 5), so results do not depend on the order of execution.
+#include <math.h>
+
+#include "common.h"
+
+namespace eve {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 at_bf16x8;
+typedef __attribute__((ext_vector_type(4))) short at_s16x4;
+typedef __attribute__((ext_vector_type(8))) short at_s16x8;
+typedef __attribute__((ext_vector_type(16))) float at_f32x16;
+typedef __attribute__((ext_vector_type(4))) float at_f32x4;
+typedef __attribute__((ext_vector_type(2))) float at_f32x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 at_bf16x2;
+
+struct AttnArgs {
+  const void *q, *k, *v, *o, *dout;
+  const uint8_t* mask;  // [B, Nk], nonzero = visible; may be null
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta;         // [B * Hkv, rows]
+  float *part_o, *part_ml;    // splits: [B * Hkv, nsplit, rows, D] and [..., 2]
+  eve_attn_layout in, grad;   // element strides of q, k, v and of their gradients
+  int Nq, Nk, Hkv, G, D, rows;
+  int heads;                  // B * Hkv
+  int nblk, nsplit;           // row (or key) blocks of a head, splits of its key tiles
+  int tiles_per_split;
+  int by_xcd;                 // blocks of a head on one XCD (block_coord)
+  float scale, c;             // c = scale log2 e
+};
+
+// ---- operand traits: a fragment is 16 bytes a lane for either type
+template <typename T> struct AT;
+template <> struct AT<bf16_t> { static constexpr int E = 8; };
+template <> struct AT<float> { static constexpr int E = 4; };
+
+template <typename T, int DP> struct AttnCfg {
+  static constexpr int E = AT<T>::E;
+  static constexpr int NKS = DP / (2 * E);              // contraction steps over the head width
+  static constexpr int CPR = DP / E;                    // 16-byte chunks of a row
+  static constexpr int PITCH = DP * (int)sizeof(T) + 16;
+  static constexpr int KT = sizeof(T) == 2 ? 64 : 32;   // rows of a staged tile
+  static constexpr int TILE = KT * PITCH;
+  static constexpr int PC = 32 / (2 * E);               // fragments of a 32-row accumulator
+  static constexpr int ND = DP / 32;
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+__device__ __forceinline__ at_f32x16 mma(const uint4& a, const uint4& b, at_f32x16 acc, bf16_t) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(at_bf16x8, a), __builtin_bit_cast(at_bf16x8, b), acc, 0, 0, 0);
+}
+__device__ __forceinline__ at_f32x16 mma(const uint4& a, const uint4& b, at_f32x16 acc, float) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), acc, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), acc, 0, 0, 0);
+}
+
+// row fragment: row r0 + (lane & 31), contraction step ks along the row
+template <int PITCH> __device__ __forceinline__ uint4 row_frag(const char* tile, int r0, int ks, int lane) {
+  return *reinterpret_cast<const uint4*>(tile + (r0 + (lane & 31)) * PITCH + (2 * ks + (lane >> 5)) * 16);
+}
+// column fragment: column d0 + (lane & 31), rows of chunk c of the 32 rows from r0, in the order of an accumulator's registers
+template <int PITCH> __device__ __forceinline__ uint4 col_frag(const char* tile, int r0, int c, int d0, int lane, bf16_t) {
+  const int i = lane & 15, q = i >> 2, p = i & 3, h = lane >> 5;
+  const char* a = tile + (r0 + 16 * c + 4 * h + q) * PITCH + (d0 + 16 * ((lane >> 4) & 1) + 4 * p) * 2;
+  const at_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) at_s16x4*)(__attribute__((address_space(3))) char*)(const_cast<char*>(a)));
+  const at_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) at_s16x4*)(__attribute__((address_space(3))) char*)(const_cast<char*>(a) + 8 * PITCH));
+  const at_s16x8 w = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(uint4, w);
+}
+template <int PITCH> __device__ __forceinline__ uint4 col_frag(const char* tile, int r0, int c, int d0, int lane, float) {
+  const char* a = tile + (r0 + 8 * c + 4 * (lane >> 5)) * PITCH + (d0 + (lane & 31)) * 4;
+  uint4 w;
+  w.x = *reinterpret_cast<const uint32_t*>(a);
+  w.y = *reinterpret_cast<const uint32_t*>(a + PITCH);
+  w.z = *reinterpret_cast<const uint32_t*>(a + 2 * PITCH);
+  w.w = *reinterpret_cast<const uint32_t*>(a + 3 * PITCH);
+  return w;
+}
+__device__ __forceinline__ uint32_t at_pack(float lo, float hi) {
+  const at_f32x2 t = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(t, at_bf16x2));
+}
+// chunk c of an accumulator as the B operand.  bf16: the probabilities (or ds) are rounded to the operands' type for the matrix
+// unit, by at most half a step each (2^-8 relative); the sums over them stay in fp32.
+__device__ __forceinline__ uint4 acc_frag(const at_f32x16& s, int c, bf16_t) {
+  return make_uint4(at_pack(s[8 * c], s[8 * c + 1]), at_pack(s[8 * c + 2], s[8 * c + 3]), at_pack(s[8 * c + 4], s[8 * c + 5]),
+                    at_pack(s[8 * c + 6], s[8 * c + 7]));
+}
+__device__ __forceinline__ uint4 acc_frag(const at_f32x16& s, int c, float) {
+  return make_uint4(__float_as_uint(s[4 * c]), __float_as_uint(s[4 * c + 1]), __float_as_uint(s[4 * c + 2]), __float_as_uint(s[4 * c + 3]));
+}
+__device__ __forceinline__ at_f32x16 acc_zero() {
+  at_f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+// the two halves of a wave hold the same columns: combine lane l with lane l ^ 32
+__device__ __forceinline__ void halves(float x, float& a, float& b) {
+  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  a = __uint_as_float(w[0]);
+  b = __uint_as_float(w[1]);
+}
+__device__ __forceinline__ float halves_max(float x) { float a, b; halves(x, a, b); return fmaxf(a, b); }
+__device__ __forceinline__ float halves_sum(float x) { float a, b; halves(x, a, b); return a + b; }
+
+template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
+template <> __device__ __forceinline__ void store4<float>(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+template <> __device__ __forceinline__ void store4<bf16_t>(bf16_t* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(at_pack(a, b), at_pack(c, d));
+}
+template <typename T> __device__ __forceinline__ float dot16(const uint4& a, const uint4& b) {
+  Vec16<T> x, y;
+  x.raw = __builtin_bit_cast(decltype(x.raw), a);
+  y.raw = __builtin_bit_cast(decltype(y.raw), b);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < Vec16<T>::N; ++i) s = fmaf(x.get(i), y.get(i), s);
+  return s;
+}
+
+// Workgroups are dealt round-robin over the 8 XCDs, each with an L2 of its own: with by_xcd all blocks of a head (which read the
+// same keys) run on one of them.  Only where every XCD gets work (the host decides); otherwise heads follow each other.
+__device__ __forceinline__ bool block_coord(const AttnArgs& a, int& head, int& blk, int& split) {
+  const int per = a.nblk * a.nsplit;
+  int r;
+  if (a.by_xcd) {
+    const int local = blockIdx.x >> 3;
+    head = (local / per) * 8 + (blockIdx.x & 7);
+    r = local % per;
+  } else {
+    head = blockIdx.x / per;
+    r = blockIdx.x % per;
+  }
+  blk = r / a.nsplit;
+  split = r % a.nsplit;
+  return head < a.heads;
+}
+
+// which of the KT keys from key0 on are visible, bit by bit (the same in every lane)
+template <int KT> __device__ __forceinline__ uint64_t key_bits(const AttnArgs& a, const uint8_t* mask, int key0, int lane) {
+  const int key = key0 + lane;
+  bool see = lane < KT && key < a.Nk;
+  if (see && mask) see = mask[key] != 0;
+  return __ballot(see);
+}
+
+// A tile of KT rows x DP columns on its way to LDS through registers (a masked row is not read and arrives as zeros: whatever it
+// holds, it takes no part).
+template <typename T, int DP, int NT> struct TileRegs {
+  using C = AttnCfg<T, DP>;
+  static constexpr int N = C::KT * C::CPR / NT;
+  uint4 w[N];
+  template <typename RowPtr> __device__ __forceinline__ void load(RowPtr row, uint64_t bits, int D, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = tid + i * NT, r = idx / C::CPR, c = idx % C::CPR;
+      w[i] = make_uint4(0, 0, 0, 0);
+      if (((bits >> r) & 1) && c * C::E < D) w[i] = *reinterpret_cast<const uint4*>(row(r) + c * C::E);
+    }
+  }
+  __device__ __forceinline__ void store(char* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = tid + i * NT;
+      *reinterpret_cast<uint4*>(tile + (idx / C::CPR) * C::PITCH + (idx % C::CPR) * 16) = w[i];
+    }
+  }
+};
+#endif  // __HIP_DEVICE_COMPILE__
+
+// ---------------------------------------------------------------------------------------------------------- forward
+// Block: NW waves of 32 rows each; the key tiles are staged for all of them, two stages deep.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using C = AttnCfg<T, DP>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  int head, blk, split;
+  if (!block_coord(a, head, blk, split)) return;
+  const int b = head / a.Hkv, hk = head % a.Hkv;
+  const T* kb = static_cast<const T*>(a.k) + b * a.in.k_b + hk * a.in.k_h;
+  const T* vb = static_cast<const T*>(a.v) + b * a.in.v_b + hk * a.in.v_h;
+  const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.Nk : nullptr;
+  const int row = blk * (NW * 32) + wave * 32 + (lane & 31);
+  const bool row_ok = row < a.rows;
+  const int qi = row / a.G, qh = hk * a.G + row % a.G;
+
+  uint4 qf[C::NKS];
+  {
+    const T* qp = static_cast<const T*>(a.q) + b * a.in.q_b + (int64_t)qi * a.in.q_n + qh * a.in.q_h;
+#pragma unroll
+    for (int ks = 0; ks < C::NKS; ++ks) {
+      const int d = (2 * ks + half) * C::E;
+      qf[ks] = make_uint4(0, 0, 0, 0);
+      if (row_ok && d < a.D) qf[ks] = *reinterpret_cast<const uint4*>(qp + d);
+    }
+  }
+  at_f32x16 o[C::ND];
+#pragma unroll
+  for (int i = 0; i < C::ND; ++i) o[i] = acc_zero();
+  float m = -INFINITY, l = 0.f;
+
+  const int ntiles = (a.Nk + C::KT - 1) / C::KT;
+  const int t0 = split * a.tiles_per_split, t1 = min(ntiles, t0 + a.tiles_per_split);
+  TileRegs<T, DP, NW * 64> kr, vr;
+  auto fetch = [&](int t, uint64_t bits) {
+    const int key0 = t * C::KT;
+    kr.load([&](int r) { return kb + (int64_t)(key0 + r) * a.in.k_n; }, bits, a.D, tid);
+    vr.load([&](int r) { return vb + (int64_t)(key0 + r) * a.in.v_n; }, bits, a.D, tid);
+  };
+  uint64_t bits = 0, bits_next = 0;
+  if (t0 < t1) {
+    bits = key_bits<C::KT>(a, mask, t0 * C::KT, lane);
+    fetch(t0, bits);
+    if (t0 + 1 < t1) bits_next = key_bits<C::KT>(a, mask, (t0 + 1) * C::KT, lane);
+  }
+  constexpr uint64_t kFull = C::KT == 64 ? ~0ull : 0xffffffffull;
+  for (int t = t0; t < t1; ++t) {
+    char* ks_ = smem + ((t - t0) & 1) * (2 * C::TILE);
+    char* vs_ = ks_ + C::TILE;
+    kr.store(ks_, tid);
+    vr.store(vs_, tid);
+    __syncthreads();
+    uint64_t bits_after = 0;
+    if (t + 1 < t1) {
+      fetch(t + 1, bits_next);
+      if (t + 2 < t1) bits_after = key_bits<C::KT>(a, mask, (t + 2) * C::KT, lane);
+    }
+    if (bits) {
+      at_f32x16 s[C::KT / 32];
+#pragma unroll
+      for (int j = 0; j < C::KT / 32; ++j) {
+        s[j] = acc_zero();
+#pragma unroll
+        for (int ks = 0; ks < C::NKS; ++ks) s[j] = mma(row_frag<C::PITCH>(ks_, 32 * j, ks, lane), qf[ks], s[j], T());
+      }
+      if (bits != kFull) {
+        const uint64_t mine = bits >> (4 * half);
+#pragma unroll
+        for (int j = 0; j < C::KT / 32; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!((mine >> (32 * j + (r & 3) + 8 * (r >> 2))) & 1)) s[j][r] = -INFINITY;
+      }
+      float mt = s[0][0];
+#pragma unroll
+      for (int j = 0; j < C::KT / 32; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[j][r]);
+      const float m_new = fmaxf(m, halves_max(mt) * a.c);
+      const float ms = m_new == -INFINITY ? 0.f : m_new;  // nothing visible so far: 2^(-inf - 0) = 0
+      const float alpha = __builtin_amdgcn_exp2f(m - ms);
+      m = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < C::KT / 32; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[j][r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], a.c, -ms));
+          sum += s[j][r];
+        }
+      l = fmaf(l, alpha, sum);
+      if (__any(alpha != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < C::ND; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+      }
+#pragma unroll
+      for (int j = 0; j < C::KT / 32; ++j)
+#pragma unroll
+        for (int cc = 0; cc < C::PC; ++cc) {
+          const uint4 p = acc_frag(s[j], cc, T());
+#pragma unroll
+          for (int i = 0; i < C::ND; ++i) o[i] = mma(col_frag<C::PITCH>(vs_, 32 * j, cc, 32 * i, lane, T()), p, o[i], T());
+        }
+    }
+    bits = bits_next;
+    bits_next = bits_after;
+  }
+  l = halves_sum(l);
+  if (!row_ok) return;
+  if (a.nsplit == 1) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // no visible key: zeros
+    T* op = static_cast<T*>(a.out) + (((int64_t)b * a.Nq + qi) * (a.Hkv * a.G) + qh) * a.D;
+#pragma unroll
+    for (int i = 0; i < C::ND; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * i + 8 * g + 4 * half;
+        if (d < a.D) store4<T>(op + d, o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv);
+      }
+    if (a.lse && half == 0) a.lse[(int64_t)head * a.rows + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  } else {
+    const int64_t at = ((int64_t)head * a.nsplit + split) * a.rows + row;
+    float* op = a.part_o + at * a.D;
+#pragma unroll
+    for (int i = 0; i < C::ND; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * i + 8 * g + 4 * half;
+        if (d < a.D) store4<float>(op + d, o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+      }
+    if (half == 0) {
+      a.part_ml[2 * at] = m;
+      a.part_ml[2 * at + 1] = l;
+    }
+  }
+#endif
+}
+
+// Joins the splits of a row, in their order: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  One wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int lane = lane_id();
+  const int64_t wid = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (wid >= (int64_t)a.heads * a.rows) return;
+  const int head = (int)(wid / a.rows), row = (int)(wid % a.rows);
+  const int64_t at0 = (int64_t)head * a.nsplit * a.rows + row;
+  float m = -INFINITY;
+  for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, a.part_ml[2 * (at0 + (int64_t)s * a.rows)]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const float ms = m == -INFINITY ? 0.f : m;
+  float l = 0.f, x0 = 0.f, x1 = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) {
+    const int64_t at = at0 + (int64_t)s * a.rows;
+    const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ms);
+    l = fmaf(w, a.part_ml[2 * at + 1], l);
+    if (lane < a.D) x0 = fmaf(w, a.part_o[at * a.D + lane], x0);
+    if (lane + 64 < a.D) x1 = fmaf(w, a.part_o[at * a.D + lane + 64], x1);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int b = head / a.Hkv, hk = head % a.Hkv;
+  T* op = static_cast<T*>(a.out) + (((int64_t)b * a.Nq + row / a.G) * (a.Hkv * a.G) + hk * a.G + row % a.G) * a.D;
+  if (lane < a.D) op[lane] = from_f32<T>(x0 * inv);
+  if (lane + 64 < a.D) op[lane + 64] = from_f32<T>(x1 * inv);
+  if (a.lse && lane == 0) a.lse[wid] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+#endif
+}
+
+// ---------------------------------------------------------------------------------------------------------- dq
+// The forward's shape: columns are query rows, the key tiles pass by.  Also forms delta_i for the dk/dv kernel.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using C = AttnCfg<T, DP>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  int head, blk, split;
+  if (!block_coord(a, head, blk, split)) return;
+  const int b = head / a.Hkv, hk = head % a.Hkv;
+  const T* kb = static_cast<const T*>(a.k) + b * a.in.k_b + hk * a.in.k_h;
+  const T* vb = static_cast<const T*>(a.v) + b * a.in.v_b + hk * a.in.v_h;
+  const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.Nk : nullptr;
+  const int row = blk * (NW * 32) + wave * 32 + (lane & 31);
+  const bool row_ok = row < a.rows;
+  const int qi = row / a.G, qh = hk * a.G + row % a.G;
+  const int64_t lrow = (int64_t)head * a.rows + row;
+
+  uint4 qf[C::NKS], gf[C::NKS];  // q and do
+  float L = INFINITY, delta = 0.f;
+  {
+    const T* qp = static_cast<const T*>(a.q) + b * a.in.q_b + (int64_t)qi * a.in.q_n + qh * a.in.q_h;
+    const int64_t oo = (((int64_t)b * a.Nq + qi) * (a.Hkv * a.G) + qh) * a.D;
+    const T *gp = static_cast<const T*>(a.dout) + oo, *op = static_cast<const T*>(a.o) + oo;
+#pragma unroll
+    for (int ks = 0; ks < C::NKS; ++ks) {
+      const int d = (2 * ks + half) * C::E;
+      qf[ks] = gf[ks] = make_uint4(0, 0, 0, 0);
+      if (row_ok && d < a.D) {
+        qf[ks] = *reinterpret_cast<const uint4*>(qp + d);
+        gf[ks] = *reinterpret_cast<const uint4*>(gp + d);
+        delta += dot16<T>(gf[ks], *reinterpret_cast<const uint4*>(op + d));
+      }
+    }
+    delta = halves_sum(delta);
+    if (row_ok) {
+      L = a.lse[lrow];
+      if (half == 0) a.delta[lrow] = delta;
+    }
+  }
+  at_f32x16 dq[C::ND];
+#pragma unroll
+  for (int i = 0; i < C::ND; ++i) dq[i] = acc_zero();
+
+  const int ntiles = (a.Nk + C::KT - 1) / C::KT;
+  TileRegs<T, DP, NW * 64> kr, vr;
+  auto fetch = [&](int t, uint64_t bits) {
+    const int key0 = t * C::KT;
+    kr.load([&](int r) { return kb + (int64_t)(key0 + r) * a.in.k_n; }, bits, a.D, tid);
+    vr.load([&](int r) { return vb + (int64_t)(key0 + r) * a.in.v_n; }, bits, a.D, tid);
+  };
+  uint64_t bits = 0, bits_next = 0;
+  if (ntiles) {
+    bits = key_bits<C::KT>(a, mask, 0, lane);
+    fetch(0, bits);
+    if (ntiles > 1) bits_next = key_bits<C::KT>(a, mask, C::KT, lane);
+  }
+  constexpr uint64_t kFull = C::KT == 64 ? ~0ull : 0xffffffffull;
+  for (int t = 0; t < ntiles; ++t) {
+    char* ks_ = smem + (t & 1) * (2 * C::TILE);
+    char* vs_ = ks_ + C::TILE;
+    kr.store(ks_, tid);
+    vr.store(vs_, tid);
+    __syncthreads();
+    uint64_t bits_after = 0;
+    if (t + 1 < ntiles) {
+      fetch(t + 1, bits_next);
+      if (t + 2 < ntiles) bits_after = key_bits<C::KT>(a, mask, (t + 2) * C::KT, lane);
+    }
+    if (bits) {
+      const uint64_t mine = bits >> (4 * half);
+#pragma unroll
+      for (int j = 0; j < C::KT / 32; ++j) {
+        at_f32x16 s = acc_zero(), dp = acc_zero();
+#pragma unroll
+        for (int ks = 0; ks < C::NKS; ++ks) {
+          s = mma(row_frag<C::PITCH>(ks_, 32 * j, ks, lane), qf[ks], s, T());
+          dp = mma(row_frag<C::PITCH>(vs_, 32 * j, ks, lane), gf[ks], dp, T());
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -L)) * (dp[r] - delta);
+        if (bits != kFull) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!((mine >> (32 * j + (r & 3) + 8 * (r >> 2))) & 1)) s[r] = 0.f;
+        }
+#pragma unroll
+        for (int cc = 0; cc < C::PC; ++cc) {
+          const uint4 p = acc_frag(s, cc, T());
+#pragma unroll
+          for (int i = 0; i < C::ND; ++i) dq[i] = mma(col_frag<C::PITCH>(ks_, 32 * j, cc, 32 * i, lane, T()), p, dq[i], T());
+        }
+      }
+    }
+    bits = bits_next;
+    bits_next = bits_after;
+  }
+  if (!row_ok) return;
+  T* dqp = static_cast<T*>(a.dq) + b * a.grad.q_b + (int64_t)qi * a.grad.q_n + qh * a.grad.q_h;
+#pragma unroll
+  for (int i = 0; i < C::ND; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * i + 8 * g + 4 * half;
+      if (d < a.D)
+        store4<T>(dqp + d, dq[i][4 * g] * a.scale, dq[i][4 * g + 1] * a.scale, dq[i][4 * g + 2] * a.scale, dq[i][4 * g + 3] * a.scale);
+    }
+#endif
+}
+
+// ---------------------------------------------------------------------------------------------------------- dk, dv
+// Columns are keys, held in registers; tiles of query rows (of all heads that share the keys) pass by.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using C = AttnCfg<T, DP>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* stats = reinterpret_cast<float*>(smem + 4 * C::TILE);  // [2 stages][L | delta][KT]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  int head, blk, split;
+  if (!block_coord(a, head, blk, split)) return;
+  const int b = head / a.Hkv, hk = head % a.Hkv;
+  const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.Nk : nullptr;
+  const int key = blk * (NW * 32) + wave * 32 + (lane & 31);
+  const bool key_ok = key < a.Nk, see = key_ok && (!mask || mask[key] != 0);
+  const T* qb = static_cast<const T*>(a.q) + b * a.in.q_b;
+  const int64_t o_b = (int64_t)b * a.Nq * (a.Hkv * a.G) * a.D;
+  const T* gb = static_cast<const T*>(a.dout) + o_b;
+
+  uint4 kf[C::NKS], vf[C::NKS];
+  {
+    const T* kp = static_cast<const T*>(a.k) + b * a.in.k_b + hk * a.in.k_h + (int64_t)key * a.in.k_n;
+    const T* vp = static_cast<const T*>(a.v) + b * a.in.v_b + hk * a.in.v_h + (int64_t)key * a.in.v_n;
+#pragma unroll
+    for (int ks = 0; ks < C::NKS; ++ks) {
+      const int d = (2 * ks + half) * C::E;
+      kf[ks] = vf[ks] = make_uint4(0, 0, 0, 0);
+      if (see && d < a.D) {
+        kf[ks] = *reinterpret_cast<const uint4*>(kp + d);
+        vf[ks] = *reinterpret_cast<const uint4*>(vp + d);
+      }
+    }
+  }
+  at_f32x16 dk[C::ND], dv[C::ND];
+#pragma unroll
+  for (int i = 0; i < C::ND; ++i) dk[i] = dv[i] = acc_zero();
+
+  const bool wave_sees = __any(see);
+  // a block without a visible key has nothing to add up (the same decision in all its waves)
+  const int ntiles = __syncthreads_or(see) ? (a.rows + C::KT - 1) / C::KT : 0;
+  TileRegs<T, DP, NW * 64> qr, gr;
+  float st = 0.f;
+  auto fetch = [&](int t) {
+    const int r0 = t * C::KT, n = a.rows - r0;
+    const uint64_t bits = n >= 64 ? ~0ull : (1ull << n) - 1;
+    qr.load([&](int r) { return qb + (int64_t)((r0 + r) / a.G) * a.in.q_n + (hk * a.G + (r0 + r) % a.G) * a.in.q_h; }, bits, a.D, tid);
+    gr.load([&](int r) { return gb + ((int64_t)((r0 + r) / a.G) * (a.Hkv * a.G) + hk * a.G + (r0 + r) % a.G) * a.D; }, bits, a.D, tid);
+    const int r = tid % C::KT;
+    if (tid < C::KT) st = r < n ? a.lse[(int64_t)head * a.rows + r0 + r] : INFINITY;  // rows past the end: p = 0
+    else if (tid < 2 * C::KT) st = r < n ? a.delta[(int64_t)head * a.rows + r0 + r] : 0.f;
+  };
+  if (ntiles) fetch(0);
+  for (int t = 0; t < ntiles; ++t) {
+    char* qs_ = smem + (t & 1) * (2 * C::TILE);
+    char* gs_ = qs_ + C::TILE;
+    float* st_ = stats + (t & 1) * (2 * C::KT);
+    qr.store(qs_, tid);
+    gr.store(gs_, tid);
+    if (tid < 2 * C::KT) st_[tid] = st;
+    __syncthreads();
+    if (t + 1 < ntiles) fetch(t + 1);
+    if (wave_sees) {
+#pragma unroll
+      for (int j = 0; j < C::KT / 32; ++j) {
+        at_f32x16 s = acc_zero(), dp = acc_zero();
+#pragma unroll
+        for (int ks = 0; ks < C::NKS; ++ks) {
+          s = mma(row_frag<C::PITCH>(qs_, 32 * j, ks, lane), kf[ks], s, T());
+          dp = mma(row_frag<C::PITCH>(gs_, 32 * j, ks, lane), vf[ks], dp, T());
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const at_f32x4 L = *reinterpret_cast<const at_f32x4*>(st_ + 32 * j + 8 * g + 4 * half);
+          const at_f32x4 de = *reinterpret_cast<const at_f32x4*>(st_ + C::KT + 32 * j + 8 * g + 4 * half);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + r], a.c, -L[r]));
+            s[4 * g + r] = p;
+            dp[4 * g + r] = p * (dp[4 * g + r] - de[r]);
+          }
+        }
+#pragma unroll
+        for (int cc = 0; cc < C::PC; ++cc) {
+          const uint4 p = acc_frag(s, cc, T()), ds = acc_frag(dp, cc, T());
+#pragma unroll
+          for (int i = 0; i < C::ND; ++i) {
+            dv[i] = mma(col_frag<C::PITCH>(gs_, 32 * j, cc, 32 * i, lane, T()), p, dv[i], T());
+            dk[i] = mma(col_frag<C::PITCH>(qs_, 32 * j, cc, 32 * i, lane, T()), ds, dk[i], T());
+          }
+        }
+      }
+    }
+  }
+  if (!key_ok) return;
+  T* dkp = static_cast<T*>(a.dk) + b * a.grad.k_b + hk * a.grad.k_h + (int64_t)key * a.grad.k_n;
+  T* dvp = static_cast<T*>(a.dv) + b * a.grad.v_b + hk * a.grad.v_h + (int64_t)key * a.grad.v_n;
+#pragma unroll
+  for (int i = 0; i < C::ND; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * i + 8 * g + 4 * half;
+      float x[4], y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {  // a column's sums are its own: a masked key's are dropped here
+        x[r] = see ? dk[i][4 * g + r] * a.scale : 0.f;
+        y[r] = see ? dv[i][4 * g + r] : 0.f;
+      }
+      if (d < a.D) {
+        store4<T>(dkp + d, x[0], x[1], x[2], x[3]);
+        store4<T>(dvp + d, y[0], y[1], y[2], y[3]);
+      }
+    }
+#endif
+}
+
+// ---------------------------------------------------------------------------------------------------------- host
+namespace {
+
+int attn_cus() {
+  static thread_local int cached_dev = -1, cached = 0;
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  if (dev != cached_dev) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cached = n;
+    cached_dev = dev;
+  }
+  return cached;
+}
+
+struct FwdPlan { int nw, nblk, ntiles, tiles_per_split, nsplit; };
+
+// Few rows against many keys: the key tiles are split until the launch has about eight waves a CU, and the parts are joined.
+FwdPlan fwd_plan(const eve_attn_shape& s, int cus) {
+  FwdPlan p;
+  const int64_t rows = (int64_t)s.Nq * (s.H / s.Hkv);
+  p.nw = rows <= 64 ? 1 : 4;
+  p.nblk = (int)((rows + p.nw * 32 - 1) / (p.nw * 32));
+  const int kt = s.dtype == EVE_BF16 ? 64 : 32;
+  p.ntiles = (int)(((int64_t)s.Nk + kt - 1) / kt);
+  const int64_t blocks = (int64_t)s.B * s.Hkv * p.nblk, want = (int64_t)cus * (p.nw == 1 ? 8 : 2);
+  int64_t split = blocks > 0 ? want / blocks : 1;
+  if (split > p.ntiles / 2) split = p.ntiles / 2;  // at least two tiles each
+  if (split > 256) split = 256;
+  if (split < 1) split = 1;
+  p.tiles_per_split = (int)((p.ntiles + split - 1) / split);
+  if (p.tiles_per_split < 1) p.tiles_per_split = 1;
+  p.nsplit = p.ntiles ? (p.ntiles + p.tiles_per_split - 1) / p.tiles_per_split : 1;
+  return p;
+}
+
+size_t fwd_ws(const eve_attn_shape& s, const FwdPlan& p) {
+  if (p.nsplit == 1) return 0;
+  const size_t rows = (size_t)s.B * s.Hkv * p.nsplit * s.Nq * (s.H / s.Hkv);
+  return align_up(rows * s.D * 4, 256) + align_up(rows * 8, 256);
+}
+
+int check_shape(const eve_attn_shape* s) {
+  EVE_REQUIRE(s, EVE_ERR_ARG, "eve_attn: null shape");
+  EVE_REQUIRE(s->dtype == EVE_F32 || s->dtype == EVE_BF16, EVE_ERR_ARG, "eve_attn: dtype %d", s->dtype);
+  EVE_REQUIRE(s->B >= 0 && s->Nq >= 0 && s->Nk >= 0, EVE_ERR_ARG, "eve_attn: negative size");
+  EVE_REQUIRE(s->H >= 1 && s->Hkv >= 1 && s->H % s->Hkv == 0, EVE_ERR_ARG, "eve_attn: %d query heads do not share %d key heads", s->H, s->Hkv);
+  EVE_REQUIRE(s->D >= 8 && s->D <= 128 && s->D % 8 == 0, EVE_ERR_UNSUPPORTED, "eve_attn: head width %d (a multiple of 8 up to 128)", s->D);
+  EVE_REQUIRE(s->scale > 0.f && s->scale <= 3.4e38f, EVE_ERR_ARG, "eve_attn: scale must be positive and finite");
+  EVE_REQUIRE((int64_t)s->Nq * (s->H / s->Hkv) <= 0x7fff0000LL && s->Nk <= 0x7fff0000, EVE_ERR_UNSUPPORTED, "eve_attn: too many rows");
+  EVE_REQUIRE((int64_t)s->B * s->Hkv <= 0x7fff0000LL && (int64_t)s->B * s->Nq <= 0x7fff0000LL, EVE_ERR_UNSUPPORTED, "eve_attn: batch too large");
+  return EVE_OK;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int check_layout(const eve_attn_layout* l, int dtype, const char* what) {
+  EVE_REQUIRE(l, EVE_ERR_ARG, "eve_attn: null %s layout", what);
+  const int64_t e = dtype == EVE_BF16 ? 8 : 4;
+  const int64_t st[9] = {l->q_b, l->q_n, l->q_h, l->k_b, l->k_n, l->k_h, l->v_b, l->v_n, l->v_h};
+  for (int64_t x : st) EVE_REQUIRE(x >= 0 && x % e == 0, EVE_ERR_ARG, "eve_attn: %s strides must be multiples of 16 bytes", what);
+  return EVE_OK;
+}
+
+AttnArgs base_args(const eve_attn_shape& s) {
+  AttnArgs a = {};
+  a.Nq = s.Nq; a.Nk = s.Nk; a.Hkv = s.Hkv; a.G = s.H / s.Hkv; a.D = s.D;
+  a.rows = s.Nq * a.G;
+  a.heads = s.B * s.Hkv;
+  a.nsplit = 1;
+  a.scale = s.scale;
+  a.c = (float)((double)s.scale * 1.4426950408889634);
+  return a;
+}
+
+template <typename T, int DP> constexpr int attn_lds(bool stats) {
+  return 4 * AttnCfg<T, DP>::TILE + (stats ? 4 * AttnCfg<T, DP>::KT * 4 : 0);
+}
+
+int launch_attn(void (*kern)(AttnArgs), AttnArgs& a, int nw, int lds, hipStream_t st, const char* name) {
+  const int64_t per = (int64_t)a.nblk * a.nsplit;
+  a.by_xcd = a.heads % 8 == 0 || a.heads >= 64;
+  const int64_t grid = (a.by_xcd ? ((int64_t)a.heads + 7) / 8 * 8 : a.heads) * per;
+  EVE_REQUIRE(grid <= 0x7fffffffLL && per <= 0x7fffffffLL, EVE_ERR_UNSUPPORTED, "%s: too many workgroups", name);
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    EVE_REQUIRE(e == hipSuccess, EVE_ERR_LAUNCH, "%s: %d bytes of LDS: %s", name, lds, hipGetErrorString(e));
+  }
+  kern<<<dim3((unsigned)grid), dim3(nw * 64), lds, st>>>(a);
+  EVE_CHECK_LAUNCH(name);
+  return EVE_OK;
+}
+
+template <typename T, int DP>
+int fwd_typed(AttnArgs& a, const FwdPlan& p, hipStream_t st) {
+  int rc = launch_attn(p.nw == 1 ? attn_fwd_kernel<T, DP, 1> : attn_fwd_kernel<T, DP, 4>, a, p.nw, attn_lds<T, DP>(false), st, "eve_attn_fwd");
+  if (rc != EVE_OK || a.nsplit == 1) return rc;
+  attn_join_kernel<T><<<dim3((unsigned)(((int64_t)a.heads * a.rows + 3) / 4)), dim3(256), 0, st>>>(a);
+  EVE_CHECK_LAUNCH("eve_attn_fwd (join)");
+  return EVE_OK;
+}
+
+template <typename T, int DP>
+int bwd_typed(AttnArgs& a, hipStream_t st) {
+  const int nw_q = a.rows <= 64 ? 1 : 4, nw_k = 4;
+  if (a.rows > 0) {
+    a.nblk = (a.rows + nw_q * 32 - 1) / (nw_q * 32);
+    const int rc = launch_attn(nw_q == 1 ? attn_dq_kernel<T, DP, 1> : attn_dq_kernel<T, DP, 4>, a, nw_q, attn_lds<T, DP>(false), st, "eve_attn_bwd (dq)");
+    if (rc != EVE_OK) return rc;
+  }
+  if (a.Nk == 0) return EVE_OK;
+  a.nblk = (a.Nk + nw_k * 32 - 1) / (nw_k * 32);
+  return launch_attn(attn_dkv_kernel<T, DP, 4>, a, nw_k, attn_lds<T, DP>(true), st, "eve_attn_bwd (dk, dv)");
+}
+
+}  // namespace
+}  // namespace eve
+
+using namespace eve;
+
+extern "C" size_t eve_attn_fwd_workspace_bytes(const eve_attn_shape* s) {
+  if (check_shape(s) != EVE_OK) return 0;
+  return fwd_ws(*s, fwd_plan(*s, attn_cus()));
+}
+
+extern "C" int eve_attn_fwd(const eve_attn_shape* s, const eve_attn_layout* in, const void* q, const void* k, const void* v,
+                            const uint8_t* key_mask, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_shape(s);
+  if (rc != EVE_OK) return rc;
+  rc = check_layout(in, s->dtype, "input");
+  if (rc != EVE_OK) return rc;
+  if (s->B == 0 || s->Nq == 0) return EVE_OK;
+  EVE_REQUIRE(q && out && (s->Nk == 0 || (k && v)), EVE_ERR_ARG, "eve_attn_fwd: null pointer");
+  EVE_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), EVE_ERR_ARG, "eve_attn_fwd: pointers must be 16-byte aligned");
+  const FwdPlan p = fwd_plan(*s, attn_cus());
+  AttnArgs a = base_args(*s);
+  a.q = q; a.k = k; a.v = v; a.mask = key_mask; a.out = out; a.lse = lse; a.in = *in;
+  a.nblk = p.nblk; a.nsplit = p.nsplit; a.tiles_per_split = p.tiles_per_split;
+  if (p.nsplit > 1) {
+    EVE_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= fwd_ws(*s, p), EVE_ERR_WORKSPACE, "eve_attn_fwd: workspace of %zu bytes, %zu needed",
+                workspace_bytes, fwd_ws(*s, p));
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                         align_up((size_t)a.heads * p.nsplit * a.rows * a.D * 4, 256));
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (s->dtype == EVE_BF16) return s->D <= 64 ? fwd_typed<bf16_t, 64>(a, p, st) : fwd_typed<bf16_t, 128>(a, p, st);
+  return s->D <= 64 ? fwd_typed<float, 64>(a, p, st) : fwd_typed<float, 128>(a, p, st);
+}
+
+extern "C" size_t eve_attn_bwd_workspace_bytes(const eve_attn_shape* s) {
+  if (check_shape(s) != EVE_OK) return 0;
+  return align_up((size_t)s->B * s->H * s->Nq * 4, 256);
+}
+
+extern "C" int eve_attn_bwd(const eve_attn_shape* s, const eve_attn_layout* in, const eve_attn_layout* grad, const void* q,
+                            const void* k, const void* v, const uint8_t* key_mask, const void* out, const float* lse,
+                            const void* dout, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_shape(s);
+  if (rc != EVE_OK) return rc;
+  rc = check_layout(in, s->dtype, "input");
+  if (rc != EVE_OK) return rc;
+  rc = check_layout(grad, s->dtype, "gradient");
+  if (rc != EVE_OK) return rc;
+  if (s->B == 0 || (s->Nq == 0 && s->Nk == 0)) return EVE_OK;
+  EVE_REQUIRE(s->Nq == 0 || (q && out && lse && dout && dq), EVE_ERR_ARG, "eve_attn_bwd: null pointer");
+  EVE_REQUIRE(s->Nk == 0 || (k && v && dk && dv), EVE_ERR_ARG, "eve_attn_bwd: null pointer");
+  const void* ptrs[8] = {q, k, v, out, dout, dq, dk, dv};
+  for (const void* x : ptrs) EVE_REQUIRE(aligned16(x), EVE_ERR_ARG, "eve_attn_bwd: pointers must be 16-byte aligned");
+  const size_t need = eve_attn_bwd_workspace_bytes(s);
+  EVE_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), EVE_ERR_WORKSPACE,
+              "eve_attn_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  AttnArgs a = base_args(*s);
+  a.q = q; a.k = k; a.v = v; a.mask = key_mask; a.o = out; a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv;
+  a.lse = const_cast<float*>(lse); a.delta = static_cast<float*>(workspace); a.in = *in; a.grad = *grad;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (s->dtype == EVE_BF16) return s->D <= 64 ? bwd_typed<bf16_t, 64>(a, st) : bwd_typed<bf16_t, 128>(a, st);
+  return s->D <= 64 ? bwd_typed<float, 64>(a, st) : bwd_typed<float, 128>(a, st);
+}

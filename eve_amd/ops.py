@@ -6,6 +6,7 @@ kernels on the current stream.  No function here has a CPU implementation.
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
@@ -407,3 +408,60 @@ def scale_residual_bwd(dout, x, gamma, row_scale, T: int):
     PROFILE.call("eve_scale_residual_bwd", _p(dout), _p(x), _p(gamma), _p(row_scale), _p(dx), _p(dgamma), S, T, M, _dt(dout),
                  _p(ws), nbytes, _stream())
     return dx, dgamma
+
+
+# ----------------------------------------------------------------------------------- attention of the encoder layer
+def _on(device):
+    """Calls are enqueued on the current stream of the tensors' device, whichever device is current."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _attn_strides(t: torch.Tensor):
+    """Element strides of the first three dimensions of [B,N,H,D]; a dimension of one element has none to speak of."""
+    return tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3]))
+
+
+def attn_readable(t: torch.Tensor) -> torch.Tensor:
+    """`t` [B,N,H,D] as the kernels can read it: the last dimension contiguous, rows on 16-byte boundaries; else a copy."""
+    unit = 16 // t.element_size()
+    if t.numel() and (t.stride(3) != 1 or t.data_ptr() % 16 or any(s % unit for s in _attn_strides(t))):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _attn_args(q, k, v, scale: float):
+    B, Nq, H, D = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    return (_lib.AttnShape(B, Nq, Nk, H, Hkv, D, _dt(q), scale),
+            _lib.AttnLayout(*_attn_strides(q), *_attn_strides(k), *_attn_strides(v)))
+
+
+def attn_fwd(q, k, v, key_mask, scale: float, want_lse: bool = True):
+    """q [B,Nq,H,D]; k, v [B,Nk,Hkv,D] (attn_readable); key_mask [B,Nk] bool | None -> (out [B,Nq,H,D], lse [B,H,Nq] | None).
+    The order inside lse is the kernels' own."""
+    _chk(key_mask, "key_mask", torch.bool)
+    B, Nq, H, D = q.shape
+    with _on(q.device):
+        shape, layout = _attn_args(q, k, v, scale)
+        out = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device)
+        lse = torch.empty(B, H, Nq, dtype=torch.float32, device=q.device) if want_lse else None
+        ref = _lib.ctypes.addressof(shape)
+        nbytes = _lib.load().eve_attn_fwd_workspace_bytes(ref)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        PROFILE.call("eve_attn_fwd", ref, _lib.ctypes.addressof(layout), _p(q), _p(k), _p(v), _p(key_mask), _p(out), _p(lse),
+                     _p(ws), nbytes, _stream(), tag=f"N={Nq}x{k.shape[1]}")
+    return out, lse
+
+
+def attn_bwd(dout, q, k, v, key_mask, out, lse, scale: float, dq, dk, dv) -> None:
+    """Writes the gradients into dq, dk, dv, which have q's, k's, v's shapes and lie as attn_readable says."""
+    _chk(dout, "dout", q.dtype), _chk(out, "out", q.dtype), _chk(lse, "lse", torch.float32)
+    with _on(q.device):
+        shape, layout = _attn_args(q, k, v, scale)
+        grads = _lib.AttnLayout(*_attn_strides(dq), *_attn_strides(dk), *_attn_strides(dv))
+        ref = _lib.ctypes.addressof(shape)
+        nbytes = _lib.load().eve_attn_bwd_workspace_bytes(ref)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        PROFILE.call("eve_attn_bwd", ref, _lib.ctypes.addressof(layout), _lib.ctypes.addressof(grads), _p(q), _p(k), _p(v),
+                     _p(key_mask), _p(out), _p(lse), _p(dout), _p(dq), _p(dk), _p(dv), _p(ws), nbytes, _stream(),
+                     tag=f"N={q.shape[1]}x{k.shape[1]}")

@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define EVE_MOE_ABI_VERSION 11
+#define EVE_MOE_ABI_VERSION 12
 
 enum { EVE_F32 = 0, EVE_BF16 = 1 };
 
@@ -395,6 +395,34 @@ size_t eve_scale_residual_workspace_bytes(int S, int M);
 int eve_scale_residual_bwd(const void* dout, const void* x, const void* gamma, const void* row_scale, void* dx,
                            float* dgamma, int S, int T, int M, int dtype, void* workspace, size_t workspace_bytes,
                            void* stream);
+
+/* ------------------------------------------------ attention of the encoder layer, models/multiway_transformer.py:99-132
+ * out[b,i,h] = sum_j p_ij v[b,j,h'], p = softmax_j(scale q[b,i,h] . k[b,j,h']) over the keys whose key_mask[b,j] is nonzero
+ * (NULL: all); h' = h / (H / Hkv): query heads may share a key/value head.  A sample without a visible key gives zeros, and what
+ * a masked key or value row holds (NaN included) takes no part.  q [B,Nq,H,D], k and v [B,Nk,Hkv,D] lie anywhere with the last
+ * dimension contiguous (strides below, in elements, multiples of 16 bytes; every pointer 16-byte aligned), so the three parts of
+ * one qkv product are read where they are.  D is a multiple of 8 up to 128; scale > 0.  out, dout: contiguous [B,Nq,H,D].
+ * lse [B, H, Nq] fp32 (opaque order; may be NULL without a backward) is what the backward recomputes the probabilities from.
+ * Scores, maxima, sums and accumulators are fp32; with EVE_BF16 the probabilities and ds enter the second products as bf16.
+ * No atomics: results do not depend on the order of execution. */
+typedef struct eve_attn_shape {
+  int B, Nq, Nk, H, Hkv, D, dtype;
+  float scale;
+} eve_attn_shape;
+typedef struct eve_attn_layout {
+  int64_t q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;
+} eve_attn_layout;
+
+/* The workspace holds the parts that few query rows against many keys are split into (0 bytes otherwise). */
+size_t eve_attn_fwd_workspace_bytes(const eve_attn_shape* shape);
+int eve_attn_fwd(const eve_attn_shape* shape, const eve_attn_layout* in, const void* q, const void* k, const void* v,
+                 const uint8_t* key_mask, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dq, dk, dv at the strides of `grad` (every element of the three is written; masked keys get zeros). */
+size_t eve_attn_bwd_workspace_bytes(const eve_attn_shape* shape);
+int eve_attn_bwd(const eve_attn_shape* shape, const eve_attn_layout* in, const eve_attn_layout* grad, const void* q,
+                 const void* k, const void* v, const uint8_t* key_mask, const void* out, const float* lse, const void* dout,
+                 void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
