@@ -14,10 +14,11 @@ from .encoder import (Attention, MultiwayTransformerEncoder, MultiwayTransformer
 from .experts import ACT2FN, Experts, MultiwayTransformerMLP, QuickGELU
 from .graph import GraphedTrainStep
 from .layer import MoE
+from .linear import fused_linear
 from .multiway import ModalitySplitFFN
 from . import retrieval
 from .sharded_moe import DeviceNoise, MOELayer, TopKGate, gumbel_rsample, top2gating
 
 __all__ = ["Attention", "DeviceNoise", "MultiwayTransformerEncoder", "MultiwayTransformerEncoderLayer", "MultiwayTransformerEnocderLayer",
            "eve_base_encoder", "MoE", "GraphedTrainStep", "ModalitySplitFFN", "MOELayer", "TopKGate", "Experts", "MultiwayTransformerMLP", "QuickGELU", "ACT2FN",
-           "attention", "gumbel_rsample", "self_attention", "top2gating", "retrieval"]
+           "attention", "fused_linear", "gumbel_rsample", "self_attention", "top2gating", "retrieval"]

@@ -66,6 +66,9 @@ SIGNATURES = {
     "eve_attn_fwd": (c_int, [_P] * 9 + [_Z, _P]),
     "eve_attn_bwd_workspace_bytes": (c_size_t, [_P]),
     "eve_attn_bwd": (c_int, [_P] * 14 + [_Z, _P]),
+    "eve_linear_fwd": (c_int, [_P] * 8 + [_I] * 6 + [_P]),
+    "eve_linear_bwd_workspace_bytes": (c_size_t, [_I] * 4),
+    "eve_linear_bwd": (c_int, [_P] * 10 + [_I] * 6 + [_P, _Z, _P]),
 }
 MOE_PASS_INFERENCE, MOE_PASS_FORWARD, MOE_PASS_BACKWARD = 0, 1, 2
 MOE_PASS_ROUTE_FWD, MOE_PASS_ROUTE_BWD = 3, 4

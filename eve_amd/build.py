@@ -21,7 +21,7 @@ CSRC = os.path.join(HERE, "csrc")
 HEADER = os.path.join(HERE, "..", "include", "eve_moe.h")
 OUT = os.path.join(HERE, "libeve_moe.so")
 OUT_DBG = os.path.join(HERE, "libeve_moe_dbg.so")
-SOURCES = ["capi.hip", "gate.hip", "permute.hip", "ffn.hip", "ffn_mfma.hip", "multiway.hip", "fused.hip", "attn.hip"]
+SOURCES = ["capi.hip", "gate.hip", "permute.hip", "ffn.hip", "ffn_mfma.hip", "multiway.hip", "fused.hip", "attn.hip", "linear.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",
          "-Wno-unused-const-variable",
          # no packed fp32 instructions: some of their forms have given wrong results on this hardware now and then

@@ -1,0 +1,79 @@
+"""A linear layer with its epilogue fused (eve_linear_fwd / eve_linear_bwd): the products around the encoder's attention and
+the residual branch that follows the second one (reference models/multiway_transformer.py:104-106, :129-130, :341), one pass
+each instead of the product, the layer scale, the DropPath product and the sum.  No CPU fallback.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, gamma, row_scale, residual, act):  # type: ignore[override]
+        N, K = weight.shape
+        rows = math.prod(x.shape[:-1])
+        x2 = x.contiguous().view(rows, K)
+        weight = weight.contiguous()
+        bias, gamma, row_scale = (None if t is None else t.contiguous() for t in (bias, gamma, row_scale))
+        res2 = None if residual is None else residual.contiguous().view(rows, N)
+        per = max(1, rows // max(1, x.shape[0])) if row_scale is not None else 1
+        need = ctx.needs_input_grad
+        save_z = need[3] or (act != ops.ACTS["identity"] and any(need[:3]))
+        y, z = ops.linear_fwd(x2, weight, bias, gamma, row_scale, res2, per, act, save_z=save_z)
+        if any(need[:4]):
+            ctx.save_for_backward(x2, weight, z, gamma, row_scale)
+        ctx.how = (x.shape, per, act, need)
+        return y.view(x.shape[:-1] + (N,))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):  # type: ignore[override]
+        shape, per, act, need = ctx.how
+        dx = dw = db = dg = None
+        if any(need[:4]):
+            x2, weight, z, gamma, row_scale = ctx.saved_tensors
+            dx, dw, db, dg = ops.linear_bwd(dy.contiguous().view(x2.shape[0], weight.shape[0]), x2, weight, z, gamma, row_scale, per, act,
+                                            need[:4])
+        return None if dx is None else dx.view(shape), dw, db, dg, None, dy if need[5] else None, None
+
+
+def fused_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: str = "identity",
+                 gamma: Optional[Tensor] = None, row_scale: Optional[Tensor] = None,
+                 residual: Optional[Tensor] = None) -> Tensor:
+    """residual + row_scale * gamma * act(x @ weight.T + bias), differentiable in all but row_scale.
+
+    x [..., K]; weight [N, K]; bias, gamma [N]; row_scale [x.shape[0]], one factor per sample (DropPath's mask / keep
+    probability); residual [..., N]; all of one type, float32 or bfloat16.  activation: "identity", "quick_gelu", "gelu" or
+    "relu".  Everything after the product works on its float32 accumulator and is rounded once; gradients are summed in a
+    fixed order."""
+    if activation not in ops.ACTS:
+        raise ValueError(f"eve_amd.fused_linear: activation {activation!r} (one of {', '.join(ops.ACTS)})")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"eve_amd.fused_linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not belong together")
+    ops._dt(x)
+    N = weight.shape[0]
+    want = {"bias": (N,), "gamma": (N,), "row_scale": tuple(x.shape[:1]), "residual": tuple(x.shape[:-1]) + (N,)}
+    parts = {"weight": weight, "bias": bias, "gamma": gamma, "row_scale": row_scale, "residual": residual}
+    for name, t in parts.items():
+        if t is None:
+            continue
+        if t.dtype != x.dtype:
+            raise TypeError(f"eve_amd.fused_linear: `{name}` is {t.dtype}, x {x.dtype}")
+        if name in want and tuple(t.shape) != want[name]:
+            raise ValueError(f"eve_amd.fused_linear: `{name}` has shape {tuple(t.shape)}, {want[name]} is needed")
+    if row_scale is not None and x.dim() < 2:
+        raise ValueError("eve_amd.fused_linear: row_scale needs samples: x with two dimensions or more")
+    if row_scale is not None and row_scale.requires_grad:
+        raise ValueError("eve_amd.fused_linear: row_scale is a mask and has no gradient")
+    for name, t in parts.items():
+        if not x.is_cuda or (t is not None and t.device != x.device):
+            raise RuntimeError(f"eve_amd.fused_linear runs on one MI355X (x on {x.device}"
+                               + (f", `{name}` on {t.device}" if t is not None else "") + "); no CPU fallback")
+    return _LinearFn.apply(x, weight, bias, gamma, row_scale, residual, ops.ACTS[activation])

@@ -465,3 +465,35 @@ def attn_bwd(dout, q, k, v, key_mask, out, lse, scale: float, dq, dk, dv) -> Non
         PROFILE.call("eve_attn_bwd", ref, _lib.ctypes.addressof(layout), _lib.ctypes.addressof(grads), _p(q), _p(k), _p(v),
                      _p(key_mask), _p(out), _p(lse), _p(dout), _p(dq), _p(dk), _p(dv), _p(ws), nbytes, _stream(),
                      tag=f"N={q.shape[1]}x{k.shape[1]}")
+
+
+# ----------------------------------------------------------------------------- linear layer with its epilogue fused
+def linear_fwd(x, w, bias, gamma, row_scale, residual, rows_per_scale: int, act: int, save_z: bool = False):
+    """x [S,K]; w [N,K]; bias, gamma [N] | None; row_scale [S / rows_per_scale] | None; residual [S,N] | None
+    -> (residual + row_scale * gamma * act(x w^T + bias) [S,N], z = x w^T + bias [S,N] | None)."""
+    for t, n in ((x, "x"), (w, "weight"), (bias, "bias"), (gamma, "gamma"), (row_scale, "row_scale"), (residual, "residual")):
+        _chk(t, n, x.dtype)
+    S, K = x.shape
+    N = w.shape[0]
+    with _on(x.device):
+        y = torch.empty(S, N, dtype=x.dtype, device=x.device)
+        z = torch.empty_like(y) if save_z else None
+        PROFILE.call("eve_linear_fwd", _p(x), _p(w), _p(bias), _p(gamma), _p(row_scale), _p(residual), _p(y), _p(z), S,
+                     rows_per_scale, K, N, act, _dt(x), _stream(), tag=f"{S}x{K}x{N}")
+    return y, z
+
+
+def linear_bwd(dy, x, w, z, gamma, row_scale, rows_per_scale: int, act: int, want):
+    """-> (dx, dw, dbias, dgamma), None where `want` (four truth values) does not ask for one."""
+    for t, n in ((dy, "dy"), (w, "weight"), (z, "z"), (gamma, "gamma"), (row_scale, "row_scale")):
+        _chk(t, n, x.dtype)
+    S, K = x.shape
+    N = w.shape[0]
+    with _on(x.device):
+        shapes = ((S, K), (N, K), (N,), (N,))
+        outs = [torch.empty(s, dtype=x.dtype, device=x.device) if yes else None for s, yes in zip(shapes, want)]
+        nbytes = _lib.load().eve_linear_bwd_workspace_bytes(S, K, N, _dt(x))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        PROFILE.call("eve_linear_bwd", _p(dy), _p(x), _p(w), _p(z), _p(gamma), _p(row_scale), *(_p(o) for o in outs), S,
+                     rows_per_scale, K, N, act, _dt(x), _p(ws), nbytes, _stream(), tag=f"{S}x{K}x{N}")
+    return outs

@@ -424,6 +424,24 @@ int eve_attn_bwd(const eve_attn_shape* shape, const eve_attn_layout* in, const e
                  const void* k, const void* v, const uint8_t* key_mask, const void* out, const float* lse, const void* dout,
                  void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------ the products around the attention, models/multiway_transformer.py:104-106, :129-130, :341
+ * y = residual + row_scale[row / rows_per_scale] * gamma * act(x w^T + bias): a linear layer with its bias and activation, the
+ * layer scale, DropPath's per-sample factor and the residual sum in ONE pass.  x [rows,K], w [N,K], y and residual [rows,N],
+ * bias and gamma [N], row_scale [ceil(rows / rows_per_scale)], all of `dtype` and contiguous; bias, gamma, row_scale and residual
+ * may be NULL.  z (may be NULL) receives x w^T + bias rounded to dtype, for the backward.  The epilogue works on the fp32
+ * accumulator and rounds once.  Any sizes, alignment of the element type. */
+int eve_linear_fwd(const void* x, const void* w, const void* bias, const void* gamma, const void* row_scale,
+                   const void* residual, void* y, void* z, int rows, int rows_per_scale, int K, int N, int act, int dtype,
+                   void* stream);
+
+/* dx [rows,K], dw [N,K], dbias [N], dgamma [N] of `dtype`, each skipped where NULL (the residual's gradient is dy itself).
+ * z: eve_linear_fwd's, needed for an activation other than identity and for dgamma.  dz = dy row_scale gamma act'(z) is rounded to
+ * dtype once, sums are fp32 in a fixed order (no atomics). */
+size_t eve_linear_bwd_workspace_bytes(int rows, int K, int N, int dtype);
+int eve_linear_bwd(const void* dy, const void* x, const void* w, const void* z, const void* gamma, const void* row_scale,
+                   void* dx, void* dw, void* dbias, void* dgamma, int rows, int rows_per_scale, int K, int N, int act, int dtype,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
