@@ -10,8 +10,10 @@ what runs:
   (fused split LayerNorm + two-group grouped GEMM);
 * single MLPs (`mlp_vl`, `single_ffn['type'] == 'single'`) are `eve_amd.MultiwayTransformerMLP`;
 * attention is PyTorch-ROCm's fused scaled-dot-product attention (fp32 softmax and accumulation inside the
-  kernel, as the reference's explicit `q.float() @ k.float().T` asks for) -- a stock op: attention is not on
-  the hot path this package rebuilds.
+  kernel, as the reference's explicit `q.float() @ k.float().T` asks for) between stock products, or -- after
+  `set_attention("fused")` on the encoder, a layer or an `Attention` -- this library's: the qkv product with its
+  bias, `eve_amd.self_attention` on it where it lies, and the output product whose epilogue applies the layer
+  scale and DropPath and adds the residual (`eve_amd.fused_linear`).
 
 `MultiwayTransformerEncoder.gate_loss()` is the aggregation that the reference's task models do by hand
 (model_vqa_beit.py:75-83).  The relative-position-bias TABLE (:462-531, off in EVE's configs) is not built
@@ -26,8 +28,10 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
 
+from .attn import self_attention
 from .experts import MultiwayTransformerMLP
 from .layer import MoE
+from .linear import fused_linear
 from .multiway import ModalitySplitFFN
 
 
@@ -132,12 +136,44 @@ class Attention(nn.Module):
         self.proj = nn.Linear(dim, dim)
         self.proj_drop = nn.Dropout(proj_drop)
 
-    def forward(self, x: Tensor, mask: Optional[Tensor] = None, relative_position_bias: Optional[Tensor] = None) -> Tensor:
+    impl = "stock"  # set_attention
+
+    def set_attention(self, impl: str = "stock") -> None:
+        """"stock": PyTorch's products and scaled-dot-product attention.  "fused": this library's kernels, where they take the
+        call (`takes_fused`), else the stock operations."""
+        if impl not in ("stock", "fused"):
+            raise ValueError(f"eve_amd: attention {impl!r} ('stock' or 'fused')")
+        self.impl = impl
+
+    def takes_fused(self, x: Tensor, mask: Optional[Tensor], relative_position_bias: Optional[Tensor]) -> bool:
+        """Whether the library's kernels compute this call: one type on the GPU, no bias on the scores, no dropout inside."""
+        if self.impl != "fused" or relative_position_bias is not None or not x.is_cuda or x.dim() != 3 or torch.is_autocast_enabled():
+            return False
+        dropout = self.training and (self.attn_drop.p > 0.0 or self.proj_drop.p > 0.0)
+        params = (self.qkv.weight, self.q_bias, self.v_bias, self.proj.weight, self.proj.bias)
+        width = x.shape[2] // self.num_heads
+        return (not dropout and x.dtype in (torch.float32, torch.bfloat16) and width % 8 == 0 and 8 <= width <= 128 and self.scale > 0
+                and self.qkv.weight.shape[0] == 3 * self.num_heads * width  # heads that do not divide the width: the stock path's error
+                and all(p is None or p.dtype == x.dtype for p in params) and (mask is None or tuple(mask.shape) == tuple(x.shape[:2])))
+
+    def _qkv_bias(self) -> Optional[Tensor]:
+        if self.q_bias is None:
+            return None
+        return torch.cat((self.q_bias, torch.zeros_like(self.v_bias, requires_grad=False), self.v_bias))
+
+    def fused(self, x: Tensor, mask: Optional[Tensor], gamma: Optional[Tensor] = None, row_scale: Optional[Tensor] = None,
+              residual: Optional[Tensor] = None) -> Tensor:
+        """`forward`, or with the rest of the layer's branch: residual + row_scale * gamma * forward(x, mask)."""
         B, N, C = x.shape
-        qkv_bias = None
-        if self.q_bias is not None:
-            qkv_bias = torch.cat((self.q_bias, torch.zeros_like(self.v_bias, requires_grad=False), self.v_bias))
-        qkv = F.linear(x, self.qkv.weight, qkv_bias)
+        qkv = fused_linear(x, self.qkv.weight, self._qkv_bias())
+        out = self_attention(qkv.view(B, N, 3, self.num_heads, -1), mask, self.scale)
+        return fused_linear(out.view(B, N, C), self.proj.weight, self.proj.bias, gamma=gamma, row_scale=row_scale, residual=residual)
+
+    def forward(self, x: Tensor, mask: Optional[Tensor] = None, relative_position_bias: Optional[Tensor] = None) -> Tensor:
+        if self.takes_fused(x, mask, relative_position_bias):
+            return self.fused(x, mask)
+        B, N, C = x.shape
+        qkv = F.linear(x, self.qkv.weight, self._qkv_bias())
         q, k, v = qkv.reshape(B, N, 3, self.num_heads, -1).permute(2, 0, 3, 1, 4).unbind(0)
         attn_mask = None
         if relative_position_bias is not None:
@@ -241,20 +277,34 @@ class MultiwayTransformerEnocderLayer(nn.Module):
         if not (x.is_cuda and x.dim() == 3 and x.dtype in (torch.float32, torch.bfloat16) and x.dtype == residual.dtype
                 and x.shape == residual.shape and x.shape[-1] % 8 == 0 and x.shape[-1] <= 16384 and gamma_ok):
             return residual + self.drop_path(x * gamma)
-        row_scale = None
+        return _ScaleResidualFn.apply(x, gamma if isinstance(gamma, Tensor) else None, self._drop_path_scale(x), residual)
+
+    def _drop_path_scale(self, x: Tensor) -> Optional[Tensor]:
+        """DropPath's own draw (same generator consumption) as one factor per sample, applied inside the kernels."""
         p = getattr(self.drop_path, "drop_prob", 0.0)
-        if p > 0.0 and self.training:  # DropPath's own draw (same generator consumption), applied inside the kernel
-            keep = 1.0 - p
-            row_scale = x.new_empty(x.shape[0]).bernoulli_(keep)
-            if keep > 0.0:
-                row_scale.div_(keep)
-        return _ScaleResidualFn.apply(x, gamma if isinstance(gamma, Tensor) else None, row_scale, residual)
+        if p == 0.0 or not self.training:
+            return None
+        keep = 1.0 - p
+        row_scale = x.new_empty(x.shape[0]).bernoulli_(keep)
+        if keep > 0.0:
+            row_scale.div_(keep)
+        return row_scale
+
+    def set_attention(self, impl: str = "stock") -> None:
+        self.attn.set_attention(impl)
+
+    def _attention_branch(self, residual: Tensor, attention_mask, relative_position_bias) -> Tensor:
+        """residual + drop_path(gamma_1 * attn(norm1(residual))) (reference :338-341)."""
+        x = layer_norm(self.norm1, residual)
+        gamma = self.gamma_1 if isinstance(self.gamma_1, Tensor) else None
+        if (self.attn.takes_fused(x, attention_mask, relative_position_bias) and x.dtype == residual.dtype
+                and (gamma is None or (gamma.dtype == x.dtype and tuple(gamma.shape) == (x.shape[-1],)))):
+            return self.attn.fused(x, attention_mask, gamma, self._drop_path_scale(x), residual)
+        x = self.attn(x, mask=attention_mask, relative_position_bias=relative_position_bias)
+        return self._branch(residual, x, self.gamma_1)
 
     def forward(self, hidden_states: Tensor, attention_mask=None, relative_position_bias=None, mode='vl') -> Tensor:
-        residual = hidden_states
-        hidden_states = self.attn(layer_norm(self.norm1, hidden_states), mask=attention_mask,
-                                  relative_position_bias=relative_position_bias)
-        hidden_states = self._branch(residual, hidden_states, self.gamma_1)
+        hidden_states = self._attention_branch(hidden_states, attention_mask, relative_position_bias)
         residual = hidden_states
         hidden_states = self._ffn(hidden_states, mode)
         return self._branch(residual, hidden_states, self.gamma_2)
@@ -322,6 +372,11 @@ class MultiwayTransformerEncoder(nn.Module):
                 hidden_states = layer(hidden_states=hidden_states, attention_mask=attention_mask,
                                       relative_position_bias=None, mode=mode)
         return hidden_states
+
+    def set_attention(self, impl: str = "stock") -> None:
+        """Whose attention all layers run (`Attention.set_attention`)."""
+        for layer in self.layers:
+            layer.set_attention(impl)
 
     def gate_loss(self, moe_lossweight: float = 1.0):
         """moe_lossweight * mean over MoE layers of (sum of the layer's l_aux / its number of calls), then the
