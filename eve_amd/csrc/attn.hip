@@ -17,7 +17,8 @@
 // long as the A operand follows, so chunk c of a 32-row accumulator supplies rows 16c + 4h + {0..3} and 16c + 8 + 4h + {0..3} (bf16)
 // and the A operand is read from LDS in that order (ds_read_b64_tr_b16: four rows of one column each).
 //
-// LDS rows are padded by 16 bytes, which serves both the 16-byte row reads and the transposed reads.
+// LDS rows are padded by 16 bytes, which serves both the 16-byte row reads and the transposed reads.  Tiles come through buffer
+// descriptors: a masked row is an offset outside the descriptor, for which the hardware delivers zeros without a branch.
 // No atomics: dq and dk/dv have a kernel each (7 products instead of 5), so results do not depend on the order of execution.
 #include <math.h>
 
@@ -38,14 +39,15 @@ struct AttnArgs {
   const uint8_t* mask;  // [B, Nk], nonzero = visible; may be null
   void *out, *dq, *dk, *dv;
   float *lse, *delta;         // [B * Hkv, rows]
-  float *part_o, *part_ml;    // splits: [B * Hkv, nsplit, rows, D] and [..., 2]
+  float *part_o, *part_ml;    // forward splits: [B * Hkv, nsplit, rows, D] and [..., 2]
+  float *part_a, *part_b;     // backward splits: dq | dk, and dv: [B * Hkv, nsplit, rows or keys, D]
   eve_attn_layout in, grad;   // element strides of q, k, v and of their gradients
   int Nq, Nk, Hkv, G, D, rows;
   int heads;                  // B * Hkv
   int nblk, nsplit;           // row (or key) blocks of a head, splits of its key tiles
   int tiles_per_split;
   int by_xcd;                 // blocks of a head on one XCD (block_coord)
-  float scale, c;             // c = scale log2 e
+  float scale, c, inv_c;      // c = scale log2 e
 };
 
 // ---- operand traits: a fragment is 16 bytes a lane for either type
@@ -53,12 +55,13 @@ template <typename T> struct AT;
 template <> struct AT<bf16_t> { static constexpr int E = 8; };
 template <> struct AT<float> { static constexpr int E = 4; };
 
-template <typename T, int DP> struct AttnCfg {
+template <typename T, int DP, int KT_ = (sizeof(T) == 2 ? 64 : 32)> struct AttnCfg {
   static constexpr int E = AT<T>::E;
   static constexpr int NKS = DP / (2 * E);              // contraction steps over the head width
   static constexpr int CPR = DP / E;                    // 16-byte chunks of a row
   static constexpr int PITCH = DP * (int)sizeof(T) + 16;
-  static constexpr int KT = sizeof(T) == 2 ? 64 : 32;   // rows of a staged tile
+  static constexpr int KT = KT_;                        // rows of a staged tile
+  static constexpr uint64_t kFull = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
   static constexpr int TILE = KT * PITCH;
   static constexpr int PC = 32 / (2 * E);               // fragments of a 32-row accumulator
   static constexpr int ND = DP / 32;
@@ -170,34 +173,60 @@ template <int KT> __device__ __forceinline__ uint64_t key_bits(const AttnArgs& a
   return __ballot(see);
 }
 
-// A tile of KT rows x DP columns on its way to LDS through registers (a masked row is not read and arrives as zeros: whatever it
-// holds, it takes no part).
-template <typename T, int DP, int NT> struct TileRegs {
-  using C = AttnCfg<T, DP>;
-  static constexpr int N = C::KT * C::CPR / NT;
-  uint4 w[N];
-  template <typename RowPtr> __device__ __forceinline__ void load(RowPtr row, uint64_t bits, int D, int tid) {
+// Two tiles of KT rows x DP columns (keys and values, or queries and gradients) on their way to LDS through registers.  A row
+// without its bit is not read and arrives as zeros: whatever it holds, it takes no part.
+constexpr uint32_t kNowhere = 0xfffffff0u, kReach = 0x80000000u;  // an offset outside every descriptor, and their extent
+typedef uint32_t at_u32x4 __attribute__((ext_vector_type(4)));
+template <typename C, int NT> struct TilePair {
+  static constexpr int N = C::KT * C::CPR / NT, STEP = NT / C::CPR;  // chunks of a thread, rows between them
+  at_u32x4 x[N], y[N];
+  uint32_t x_off, y_off, x_row, y_row;  // first chunk, bytes of a row
+  int row0;
+  __device__ __forceinline__ TilePair(int64_t x_n, int64_t y_n, int D, int tid) {
+    row0 = tid / C::CPR;
+    const int c = tid % C::CPR;
+    x_row = (uint32_t)x_n * (16 / C::E);
+    y_row = (uint32_t)y_n * (16 / C::E);
+    const bool in = c * C::E < D;
+    x_off = in ? row0 * x_row + c * 16 : kNowhere;
+    y_off = in ? row0 * y_row + c * 16 : kNowhere;
+  }
+  __device__ __forceinline__ void load(const void* xp, const void* yp, uint64_t bits) {
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(xp), 0, kReach, 0x00020000);
+    const __amdgpu_buffer_rsrc_t yr = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(yp), 0, kReach, 0x00020000);
+    if (bits == C::kFull) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * NT, r = idx / C::CPR, c = idx % C::CPR;
-      w[i] = make_uint4(0, 0, 0, 0);
-      if (((bits >> r) & 1) && c * C::E < D) w[i] = *reinterpret_cast<const uint4*>(row(r) + c * C::E);
+      for (int i = 0; i < N; ++i) {
+        x[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, x_off, i * STEP * x_row, 0);
+        y[i] = __builtin_amdgcn_raw_buffer_load_b128(yr, y_off, i * STEP * y_row, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool see = (bits >> (row0 + i * STEP)) & 1;
+        x[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, see ? x_off : kNowhere, i * STEP * x_row, 0);
+        y[i] = __builtin_amdgcn_raw_buffer_load_b128(yr, see ? y_off : kNowhere, i * STEP * y_row, 0);
+      }
     }
   }
-  __device__ __forceinline__ void store(char* tile, int tid) const {
+  __device__ __forceinline__ void store(char* xs, char* ys, int tid) const {
+    const int at = row0 * C::PITCH + (tid % C::CPR) * 16;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * NT;
-      *reinterpret_cast<uint4*>(tile + (idx / C::CPR) * C::PITCH + (idx % C::CPR) * 16) = w[i];
+      *reinterpret_cast<at_u32x4*>(xs + at + i * STEP * C::PITCH) = x[i];
+      *reinterpret_cast<at_u32x4*>(ys + at + i * STEP * C::PITCH) = y[i];
     }
   }
 };
 #endif  // __HIP_DEVICE_COMPILE__
 
 // ---------------------------------------------------------------------------------------------------------- forward
-// Block: NW waves of 32 rows each; the key tiles are staged for all of them, two stages deep.
+// Block: NW waves of 32 rows each; the key tiles are staged for all of them, two stages deep.  A block of one wave (few rows,
+// bound by the keys' bytes) has one stage, so that more of them fit a CU.
+// The bounds on waves keep the register budget at 256, where the compiler holds accumulators in plain registers: in the larger
+// budget it moves them to and from accumulation registers, a third of the instructions of the loop.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 64 ? 3 : 2) void attn_fwd_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using C = AttnCfg<T, DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -229,11 +258,9 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
 
   const int ntiles = (a.Nk + C::KT - 1) / C::KT;
   const int t0 = split * a.tiles_per_split, t1 = min(ntiles, t0 + a.tiles_per_split);
-  TileRegs<T, DP, NW * 64> kr, vr;
+  TilePair<C, NW * 64> kv(a.in.k_n, a.in.v_n, a.D, tid);
   auto fetch = [&](int t, uint64_t bits) {
-    const int key0 = t * C::KT;
-    kr.load([&](int r) { return kb + (int64_t)(key0 + r) * a.in.k_n; }, bits, a.D, tid);
-    vr.load([&](int r) { return vb + (int64_t)(key0 + r) * a.in.v_n; }, bits, a.D, tid);
+    kv.load(kb + (int64_t)t * C::KT * a.in.k_n, vb + (int64_t)t * C::KT * a.in.v_n, bits);
   };
   uint64_t bits = 0, bits_next = 0;
   if (t0 < t1) {
@@ -241,12 +268,11 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
     fetch(t0, bits);
     if (t0 + 1 < t1) bits_next = key_bits<C::KT>(a, mask, (t0 + 1) * C::KT, lane);
   }
-  constexpr uint64_t kFull = C::KT == 64 ? ~0ull : 0xffffffffull;
   for (int t = t0; t < t1; ++t) {
-    char* ks_ = smem + ((t - t0) & 1) * (2 * C::TILE);
+    char* ks_ = smem + (NW == 1 ? 0 : ((t - t0) & 1) * (2 * C::TILE));
     char* vs_ = ks_ + C::TILE;
-    kr.store(ks_, tid);
-    vr.store(vs_, tid);
+    if (NW == 1) __syncthreads();
+    kv.store(ks_, vs_, tid);
     __syncthreads();
     uint64_t bits_after = 0;
     if (t + 1 < t1) {
@@ -261,7 +287,7 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
 #pragma unroll
         for (int ks = 0; ks < C::NKS; ++ks) s[j] = mma(row_frag<C::PITCH>(ks_, 32 * j, ks, lane), qf[ks], s[j], T());
       }
-      if (bits != kFull) {
+      if (bits != C::kFull) {
         const uint64_t mine = bits >> (4 * half);
 #pragma unroll
         for (int j = 0; j < C::KT / 32; ++j)
@@ -336,41 +362,97 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(AttnArgs a) {
 #endif
 }
 
-// Joins the splits of a row, in their order: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  One wave a row.
+// Joins the splits of a row, in a fixed order: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  A block a row: 8 splits of 32
+// chunks of 4 columns at a time, then the 8 are added.
+constexpr int kMaxSplit = 256;
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  const int lane = lane_id();
-  const int64_t wid = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (wid >= (int64_t)a.heads * a.rows) return;
-  const int head = (int)(wid / a.rows), row = (int)(wid % a.rows);
+  __shared__ float weight[kMaxSplit], red[8];
+  __shared__ float4 sums[8][32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int head = blockIdx.x / a.rows, row = blockIdx.x % a.rows;
   const int64_t at0 = (int64_t)head * a.nsplit * a.rows + row;
-  float m = -INFINITY;
-  for (int s = lane; s < a.nsplit; s += 64) m = fmaxf(m, a.part_ml[2 * (at0 + (int64_t)s * a.rows)]);
+  float m = -INFINITY, l = 0.f;
+  if (tid < a.nsplit) {
+    m = a.part_ml[2 * (at0 + (int64_t)tid * a.rows)];
+    l = a.part_ml[2 * (at0 + (int64_t)tid * a.rows) + 1];
+  }
+  float top = m;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  const float ms = m == -INFINITY ? 0.f : m;
-  float l = 0.f, x0 = 0.f, x1 = 0.f;
-  for (int s = 0; s < a.nsplit; ++s) {
-    const int64_t at = at0 + (int64_t)s * a.rows;
-    const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ms);
-    l = fmaf(w, a.part_ml[2 * at + 1], l);
-    if (lane < a.D) x0 = fmaf(w, a.part_o[at * a.D + lane], x0);
-    if (lane + 64 < a.D) x1 = fmaf(w, a.part_o[at * a.D + lane + 64], x1);
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  if (lane == 0) red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float w = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+  weight[tid] = w;
+  l = wave_sum(w * l);
+  if (lane == 0) red[4 + wave] = l;
+  __syncthreads();
+  l = (red[4] + red[5]) + (red[6] + red[7]);
+  const int d = (tid & 31) * 4;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (d < a.D) {
+#pragma unroll 4
+    for (int s = tid >> 5; s < a.nsplit; s += 8) {
+      const float4 y = *reinterpret_cast<const float4*>(a.part_o + (at0 + (int64_t)s * a.rows) * a.D + d);
+      const float ws = weight[s];
+      x.x = fmaf(ws, y.x, x.x);
+      x.y = fmaf(ws, y.y, x.y);
+      x.z = fmaf(ws, y.z, x.z);
+      x.w = fmaf(ws, y.w, x.w);
+    }
+  }
+  sums[tid >> 5][tid & 31] = x;
+  __syncthreads();
+  if (tid >= 32 || d >= a.D) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    const float4 y = sums[i][tid];
+    x.x += y.x;
+    x.y += y.y;
+    x.z += y.z;
+    x.w += y.w;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int b = head / a.Hkv, hk = head % a.Hkv;
   T* op = static_cast<T*>(a.out) + (((int64_t)b * a.Nq + row / a.G) * (a.Hkv * a.G) + hk * a.G + row % a.G) * a.D;
-  if (lane < a.D) op[lane] = from_f32<T>(x0 * inv);
-  if (lane + 64 < a.D) op[lane + 64] = from_f32<T>(x1 * inv);
-  if (a.lse && lane == 0) a.lse[wid] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  store4<T>(op + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  if (a.lse && tid == 0) a.lse[(int64_t)head * a.rows + row] = l == 0.f ? INFINITY : top + __builtin_amdgcn_logf(l);
+#endif
+}
+
+// Adds the splits of a gradient in their order: g = factor * sum_s part[head, s, row].  Four columns a thread; for dq a row is
+// query row / G of query head (key head) G + row % G, for dk and dv (G = 1) a key.
+struct AttnSum { const float* part; void* g; int64_t g_b, g_n, g_h; int64_t total; int Hkv, G, D, rows, nsplit; float factor; };
+template <typename T>
+__global__ __launch_bounds__(256) void attn_sum_kernel(AttnSum a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.total) return;
+  const int cols = a.D / 4, d = (int)(i % cols) * 4;
+  const int64_t hr = i / cols;
+  const int row = (int)(hr % a.rows), head = (int)(hr / a.rows);
+  const float* p = a.part + ((int64_t)head * a.nsplit * a.rows + row) * a.D + d;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float4 y = *reinterpret_cast<const float4*>(p + (int64_t)s * a.rows * a.D);
+    x.x += y.x;
+    x.y += y.y;
+    x.z += y.z;
+    x.w += y.w;
+  }
+  T* g = static_cast<T*>(a.g) + (head / a.Hkv) * a.g_b + (int64_t)(row / a.G) * a.g_n + ((head % a.Hkv) * a.G + row % a.G) * a.g_h + d;
+  store4<T>(g, x.x * a.factor, x.y * a.factor, x.z * a.factor, x.w * a.factor);
 #endif
 }
 
 // ---------------------------------------------------------------------------------------------------------- dq
-// The forward's shape: columns are query rows, the key tiles pass by.  Also forms delta_i for the dk/dv kernel.
+// The forward's shape: columns are query rows, the key tiles pass by (or a split of them).  Also forms delta_i for the dk/dv
+// kernel.  -delta is the accumulator that the product do v^T starts from.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using C = AttnCfg<T, DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -405,51 +487,52 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
     delta = halves_sum(delta);
     if (row_ok) {
       L = a.lse[lrow];
-      if (half == 0) a.delta[lrow] = delta;
+      if (half == 0 && split == 0) a.delta[lrow] = delta;
     }
   }
+  at_f32x16 minus_delta;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) minus_delta[r] = -delta;
   at_f32x16 dq[C::ND];
 #pragma unroll
   for (int i = 0; i < C::ND; ++i) dq[i] = acc_zero();
 
   const int ntiles = (a.Nk + C::KT - 1) / C::KT;
-  TileRegs<T, DP, NW * 64> kr, vr;
+  const int t0 = split * a.tiles_per_split, t1 = min(ntiles, t0 + a.tiles_per_split);
+  TilePair<C, NW * 64> kv(a.in.k_n, a.in.v_n, a.D, tid);
   auto fetch = [&](int t, uint64_t bits) {
-    const int key0 = t * C::KT;
-    kr.load([&](int r) { return kb + (int64_t)(key0 + r) * a.in.k_n; }, bits, a.D, tid);
-    vr.load([&](int r) { return vb + (int64_t)(key0 + r) * a.in.v_n; }, bits, a.D, tid);
+    kv.load(kb + (int64_t)t * C::KT * a.in.k_n, vb + (int64_t)t * C::KT * a.in.v_n, bits);
   };
   uint64_t bits = 0, bits_next = 0;
-  if (ntiles) {
-    bits = key_bits<C::KT>(a, mask, 0, lane);
-    fetch(0, bits);
-    if (ntiles > 1) bits_next = key_bits<C::KT>(a, mask, C::KT, lane);
+  if (t0 < t1) {
+    bits = key_bits<C::KT>(a, mask, t0 * C::KT, lane);
+    fetch(t0, bits);
+    if (t0 + 1 < t1) bits_next = key_bits<C::KT>(a, mask, (t0 + 1) * C::KT, lane);
   }
-  constexpr uint64_t kFull = C::KT == 64 ? ~0ull : 0xffffffffull;
-  for (int t = 0; t < ntiles; ++t) {
-    char* ks_ = smem + (t & 1) * (2 * C::TILE);
+  for (int t = t0; t < t1; ++t) {
+    char* ks_ = smem + (NW == 1 ? 0 : ((t - t0) & 1) * (2 * C::TILE));
     char* vs_ = ks_ + C::TILE;
-    kr.store(ks_, tid);
-    vr.store(vs_, tid);
+    if (NW == 1) __syncthreads();
+    kv.store(ks_, vs_, tid);
     __syncthreads();
     uint64_t bits_after = 0;
-    if (t + 1 < ntiles) {
+    if (t + 1 < t1) {
       fetch(t + 1, bits_next);
-      if (t + 2 < ntiles) bits_after = key_bits<C::KT>(a, mask, (t + 2) * C::KT, lane);
+      if (t + 2 < t1) bits_after = key_bits<C::KT>(a, mask, (t + 2) * C::KT, lane);
     }
     if (bits) {
       const uint64_t mine = bits >> (4 * half);
 #pragma unroll
       for (int j = 0; j < C::KT / 32; ++j) {
-        at_f32x16 s = acc_zero(), dp = acc_zero();
+        at_f32x16 s = acc_zero(), dp = minus_delta;
 #pragma unroll
         for (int ks = 0; ks < C::NKS; ++ks) {
           s = mma(row_frag<C::PITCH>(ks_, 32 * j, ks, lane), qf[ks], s, T());
           dp = mma(row_frag<C::PITCH>(vs_, 32 * j, ks, lane), gf[ks], dp, T());
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -L)) * (dp[r] - delta);
-        if (bits != kFull) {
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -L)) * dp[r];
+        if (bits != C::kFull) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (!((mine >> (32 * j + (r & 3) + 8 * (r >> 2))) & 1)) s[r] = 0.f;
@@ -466,6 +549,17 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
     bits_next = bits_after;
   }
   if (!row_ok) return;
+  if (a.nsplit > 1) {
+    float* p = a.part_a + (((int64_t)head * a.nsplit + split) * a.rows + row) * a.D;
+#pragma unroll
+    for (int i = 0; i < C::ND; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * i + 8 * g + 4 * half;
+        if (d < a.D) store4<float>(p + d, dq[i][4 * g], dq[i][4 * g + 1], dq[i][4 * g + 2], dq[i][4 * g + 3]);
+      }
+    return;
+  }
   T* dqp = static_cast<T*>(a.dq) + b * a.grad.q_b + (int64_t)qi * a.grad.q_n + qh * a.grad.q_h;
 #pragma unroll
   for (int i = 0; i < C::ND; ++i)
@@ -479,13 +573,26 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------- dk, dv
-// Columns are keys, held in registers; tiles of query rows (of all heads that share the keys) pass by.
+// x = hi + mid + lo exactly, eight bits of the significand each
+__device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffff0000u;
+  const float r = x - __uint_as_float(hi);
+  mid = __float_as_uint(r) & 0xffff0000u;
+  lo = __float_as_uint(r - __uint_as_float(mid)) & 0xffff0000u;
+}
+
+// Columns are keys, held in registers; tiles of query rows (head after head of those that share the keys) pass by.
+//
+// Here L_i and delta_i belong to a row, that is, to a register, the same in 32 lanes.  The products start from -L_i / c and -delta_i:
+// p = 2^(c acc), ds = p acc'.  For bf16 these starts are themselves a matrix product: a row's 16 bytes hold both values as three
+// bf16 each, which multiply ones; read as values, four at a time, they would be a third of the LDS traffic that bounds this loop.
+template <typename T, int DP> constexpr int dkv_rows() { return sizeof(T) == 2 && DP == 64 ? 64 : 32; }
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using C = AttnCfg<T, DP>;
+  using C = AttnCfg<T, DP, dkv_rows<T, DP>()>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* stats = reinterpret_cast<float*>(smem + 4 * C::TILE);  // [2 stages][L | delta][KT]
+  char* stats = smem + 4 * C::TILE;  // [2 stages][KT] of 16 bytes
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   int head, blk, split;
   if (!block_coord(a, head, blk, split)) return;
@@ -493,9 +600,9 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
   const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.Nk : nullptr;
   const int key = blk * (NW * 32) + wave * 32 + (lane & 31);
   const bool key_ok = key < a.Nk, see = key_ok && (!mask || mask[key] != 0);
-  const T* qb = static_cast<const T*>(a.q) + b * a.in.q_b;
-  const int64_t o_b = (int64_t)b * a.Nq * (a.Hkv * a.G) * a.D;
-  const T* gb = static_cast<const T*>(a.dout) + o_b;
+  const int64_t o_n = (int64_t)a.Hkv * a.G * a.D;
+  const T* qb = static_cast<const T*>(a.q) + b * a.in.q_b + (int64_t)hk * a.G * a.in.q_h;
+  const T* gb = static_cast<const T*>(a.dout) + (int64_t)b * a.Nq * o_n + (int64_t)hk * a.G * a.D;
 
   uint4 kf[C::NKS], vf[C::NKS];
   {
@@ -514,50 +621,75 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
   at_f32x16 dk[C::ND], dv[C::ND];
 #pragma unroll
   for (int i = 0; i < C::ND; ++i) dk[i] = dv[i] = acc_zero();
+  // ones (bf16 0x3f80) against the three parts of -L / c, and of -delta
+  const uint4 one_L = half ? make_uint4(0, 0, 0, 0) : make_uint4(0x3f803f80u, 0x00003f80u, 0, 0);
+  const uint4 one_d = half ? make_uint4(0, 0, 0, 0) : make_uint4(0, 0x3f800000u, 0x3f803f80u, 0);
 
   const bool wave_sees = __any(see);
+  const int tq = (a.Nq + C::KT - 1) / C::KT;
   // a block without a visible key has nothing to add up (the same decision in all its waves)
-  const int ntiles = __syncthreads_or(see) ? (a.rows + C::KT - 1) / C::KT : 0;
-  TileRegs<T, DP, NW * 64> qr, gr;
-  float st = 0.f;
-  auto fetch = [&](int t) {
-    const int r0 = t * C::KT, n = a.rows - r0;
-    const uint64_t bits = n >= 64 ? ~0ull : (1ull << n) - 1;
-    qr.load([&](int r) { return qb + (int64_t)((r0 + r) / a.G) * a.in.q_n + (hk * a.G + (r0 + r) % a.G) * a.in.q_h; }, bits, a.D, tid);
-    gr.load([&](int r) { return gb + ((int64_t)((r0 + r) / a.G) * (a.Hkv * a.G) + hk * a.G + (r0 + r) % a.G) * a.D; }, bits, a.D, tid);
-    const int r = tid % C::KT;
-    if (tid < C::KT) st = r < n ? a.lse[(int64_t)head * a.rows + r0 + r] : INFINITY;  // rows past the end: p = 0
-    else if (tid < 2 * C::KT) st = r < n ? a.delta[(int64_t)head * a.rows + r0 + r] : 0.f;
+  const int t0 = split * a.tiles_per_split, t1 = __syncthreads_or(see) ? min(tq * a.G, t0 + a.tiles_per_split) : t0;
+  TilePair<C, NW * 64> qg(a.in.q_n, o_n, a.D, tid);
+  float st_L = 0.f, st_d = 0.f;
+  int g = tq ? t0 / tq : 0, tr = tq ? t0 % tq : 0;  // head of the group, tile of its rows
+  auto fetch = [&]() {
+    const int r0 = tr * C::KT, n = a.Nq - r0;
+    qg.load(qb + g * a.in.q_h + r0 * a.in.q_n, gb + (int64_t)g * a.D + r0 * o_n, n >= C::KT ? C::kFull : (1ull << n) - 1);
+    if (tid < C::KT) {  // rows past the end: p = 2^(-1e30) = 0
+      const int64_t i = (int64_t)head * a.rows + (int64_t)(r0 + tid) * a.G + g;
+      st_L = tid < n ? fminf(a.lse[i], 1e30f) : 1e30f;
+      st_d = tid < n ? a.delta[i] : 0.f;
+    }
+    if (++tr == tq) { tr = 0; ++g; }
   };
-  if (ntiles) fetch(0);
-  for (int t = 0; t < ntiles; ++t) {
-    char* qs_ = smem + (t & 1) * (2 * C::TILE);
+  if (t0 < t1) fetch();
+  for (int t = t0; t < t1; ++t) {
+    char* qs_ = smem + ((t - t0) & 1) * (2 * C::TILE);
     char* gs_ = qs_ + C::TILE;
-    float* st_ = stats + (t & 1) * (2 * C::KT);
-    qr.store(qs_, tid);
-    gr.store(gs_, tid);
-    if (tid < 2 * C::KT) st_[tid] = st;
+    char* st_ = stats + ((t - t0) & 1) * (C::KT * 16);
+    qg.store(qs_, gs_, tid);
+    if (tid < C::KT) {
+      if constexpr (sizeof(T) == 2) {
+        uint32_t l0, l1, l2, d0, d1, d2;
+        split3(st_L * -a.inv_c, l0, l1, l2);
+        split3(-st_d, d0, d1, d2);
+        *reinterpret_cast<uint4*>(st_ + tid * 16) = make_uint4((l0 >> 16) | l1, (l2 >> 16) | d0, (d1 >> 16) | d2, 0);
+      } else {
+        reinterpret_cast<float*>(st_)[tid] = st_L * -a.inv_c;
+        reinterpret_cast<float*>(st_)[C::KT + tid] = -st_d;
+      }
+    }
     __syncthreads();
-    if (t + 1 < ntiles) fetch(t + 1);
+    if (t + 1 < t1) fetch();
     if (wave_sees) {
 #pragma unroll
       for (int j = 0; j < C::KT / 32; ++j) {
         at_f32x16 s = acc_zero(), dp = acc_zero();
+        if constexpr (sizeof(T) == 2) {
+          const uint4 both = *reinterpret_cast<const uint4*>(st_ + (32 * j + (lane & 31)) * 16);
+          s = mma(both, one_L, s, T());
+          dp = mma(both, one_d, dp, T());
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const at_f32x4 L = *reinterpret_cast<const at_f32x4*>(st_ + (32 * j + 8 * i + 4 * half) * 4);
+            const at_f32x4 de = *reinterpret_cast<const at_f32x4*>(st_ + (C::KT + 32 * j + 8 * i + 4 * half) * 4);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              s[4 * i + r] = L[r];
+              dp[4 * i + r] = de[r];
+            }
+          }
+        }
 #pragma unroll
         for (int ks = 0; ks < C::NKS; ++ks) {
           s = mma(row_frag<C::PITCH>(qs_, 32 * j, ks, lane), kf[ks], s, T());
           dp = mma(row_frag<C::PITCH>(gs_, 32 * j, ks, lane), vf[ks], dp, T());
         }
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const at_f32x4 L = *reinterpret_cast<const at_f32x4*>(st_ + 32 * j + 8 * g + 4 * half);
-          const at_f32x4 de = *reinterpret_cast<const at_f32x4*>(st_ + C::KT + 32 * j + 8 * g + 4 * half);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + r], a.c, -L[r]));
-            s[4 * g + r] = p;
-            dp[4 * g + r] = p * (dp[4 * g + r] - de[r]);
-          }
+        for (int r = 0; r < 16; ++r) {
+          s[r] = __builtin_amdgcn_exp2f(s[r] * a.c);
+          dp[r] *= s[r];
         }
 #pragma unroll
         for (int cc = 0; cc < C::PC; ++cc) {
@@ -572,18 +704,39 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(AttnArgs a) {
     }
   }
   if (!key_ok) return;
+  // a column's sums are its own: a masked key's are dropped here
+  if (a.nsplit > 1) {
+    const int64_t at = (((int64_t)head * a.nsplit + split) * a.Nk + key) * a.D;
+#pragma unroll
+    for (int i = 0; i < C::ND; ++i)
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        const int d = 32 * i + 8 * gq + 4 * half;
+        float x[4], y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[r] = see ? dk[i][4 * gq + r] : 0.f;
+          y[r] = see ? dv[i][4 * gq + r] : 0.f;
+        }
+        if (d < a.D) {
+          store4<float>(a.part_a + at + d, x[0], x[1], x[2], x[3]);
+          store4<float>(a.part_b + at + d, y[0], y[1], y[2], y[3]);
+        }
+      }
+    return;
+  }
   T* dkp = static_cast<T*>(a.dk) + b * a.grad.k_b + hk * a.grad.k_h + (int64_t)key * a.grad.k_n;
   T* dvp = static_cast<T*>(a.dv) + b * a.grad.v_b + hk * a.grad.v_h + (int64_t)key * a.grad.v_n;
 #pragma unroll
   for (int i = 0; i < C::ND; ++i)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * i + 8 * g + 4 * half;
+    for (int gq = 0; gq < 4; ++gq) {
+      const int d = 32 * i + 8 * gq + 4 * half;
       float x[4], y[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {  // a column's sums are its own: a masked key's are dropped here
-        x[r] = see ? dk[i][4 * g + r] * a.scale : 0.f;
-        y[r] = see ? dv[i][4 * g + r] : 0.f;
+      for (int r = 0; r < 4; ++r) {
+        x[r] = see ? dk[i][4 * gq + r] * a.scale : 0.f;
+        y[r] = see ? dv[i][4 * gq + r] : 0.f;
       }
       if (d < a.D) {
         store4<T>(dkp + d, x[0], x[1], x[2], x[3]);
@@ -609,31 +762,63 @@ int attn_cus() {
   return cached;
 }
 
-struct FwdPlan { int nw, nblk, ntiles, tiles_per_split, nsplit; };
+// How a kernel's rows (or keys) are cut into blocks, and the tiles that pass by them into splits.
+struct AttnPlan { int nw, nblk, tiles_per_split, nsplit; };
 
-// Few rows against many keys: the key tiles are split until the launch has about eight waves a CU, and the parts are joined.
-FwdPlan fwd_plan(const eve_attn_shape& s, int cus) {
-  FwdPlan p;
-  const int64_t rows = (int64_t)s.Nq * (s.H / s.Hkv);
-  p.nw = rows <= 64 ? 1 : 4;
-  p.nblk = (int)((rows + p.nw * 32 - 1) / (p.nw * 32));
-  const int kt = s.dtype == EVE_BF16 ? 64 : 32;
-  p.ntiles = (int)(((int64_t)s.Nk + kt - 1) / kt);
-  const int64_t blocks = (int64_t)s.B * s.Hkv * p.nblk, want = (int64_t)cus * (p.nw == 1 ? 8 : 2);
-  int64_t split = blocks > 0 ? want / blocks : 1;
-  if (split > p.ntiles / 2) split = p.ntiles / 2;  // at least two tiles each
-  if (split > 256) split = 256;
+AttnPlan plan_of(int64_t rows, int nw, int64_t heads, int64_t tiles, int64_t want_blocks, int64_t least_tiles) {
+  AttnPlan p;
+  p.nw = nw;
+  p.nblk = (int)((rows + nw * 32 - 1) / (nw * 32));
+  const int64_t blocks = heads * p.nblk;
+  int64_t split = blocks > 0 ? want_blocks / blocks : 1;
+  if (split > tiles / least_tiles) split = tiles / least_tiles;
+  if (split > kMaxSplit) split = kMaxSplit;
   if (split < 1) split = 1;
-  p.tiles_per_split = (int)((p.ntiles + split - 1) / split);
+  p.tiles_per_split = (int)((tiles + split - 1) / split);
   if (p.tiles_per_split < 1) p.tiles_per_split = 1;
-  p.nsplit = p.ntiles ? (p.ntiles + p.tiles_per_split - 1) / p.tiles_per_split : 1;
+  p.nsplit = tiles > 0 ? (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
   return p;
 }
 
-size_t fwd_ws(const eve_attn_shape& s, const FwdPlan& p) {
+int64_t q_rows(const eve_attn_shape& s) { return (int64_t)s.Nq * (s.H / s.Hkv); }
+int64_t key_tiles(const eve_attn_shape& s) {
+  const int kt = s.dtype == EVE_BF16 ? 64 : 32;
+  return ((int64_t)s.Nk + kt - 1) / kt;
+}
+
+// Few rows against many keys: the key tiles are split until the launch fills the CUs, and the parts are joined.  Up to 64 rows a
+// head go to blocks of one wave, of which 8 (head width up to 64) or 4 fit a CU.
+AttnPlan fwd_plan(const eve_attn_shape& s, int cus) {
+  const int nw = q_rows(s) <= 64 ? 1 : 4;
+  return plan_of(q_rows(s), nw, (int64_t)s.B * s.Hkv, key_tiles(s), (int64_t)cus * (nw == 4 ? 2 : s.D <= 64 ? 8 : 4), 2);
+}
+AttnPlan dq_plan(const eve_attn_shape& s, int cus) {
+  const int nw = q_rows(s) <= 64 ? 1 : 4;
+  return plan_of(q_rows(s), nw, (int64_t)s.B * s.Hkv, key_tiles(s), (int64_t)cus * (nw == 4 ? 2 : 4), 4);
+}
+// The row tiles are counted head by head of a group, as the kernel walks them.
+AttnPlan dkv_plan(const eve_attn_shape& s, int cus) {
+  const int kt = s.dtype == EVE_BF16 && s.D <= 64 ? 64 : 32;
+  return plan_of(s.Nk, 4, (int64_t)s.B * s.Hkv, ((int64_t)s.Nq + kt - 1) / kt * (s.H / s.Hkv), (int64_t)cus * 2, 4);
+}
+
+size_t fwd_ws(const eve_attn_shape& s, const AttnPlan& p) {
   if (p.nsplit == 1) return 0;
-  const size_t rows = (size_t)s.B * s.Hkv * p.nsplit * s.Nq * (s.H / s.Hkv);
+  const size_t rows = (size_t)s.B * s.Hkv * p.nsplit * q_rows(s);
   return align_up(rows * s.D * 4, 256) + align_up(rows * 8, 256);
+}
+// delta, then the parts of dq, and in their place afterwards those of dk and dv
+struct BwdWs { size_t delta, part, dv, bytes; };
+BwdWs bwd_ws(const eve_attn_shape& s, const AttnPlan& pq, const AttnPlan& pk) {
+  BwdWs w;
+  const size_t heads = (size_t)s.B * s.Hkv;
+  w.delta = 0;
+  w.part = align_up(heads * q_rows(s) * 4, 256);
+  const size_t dq = pq.nsplit > 1 ? align_up(heads * pq.nsplit * q_rows(s) * s.D * 4, 256) : 0;
+  const size_t dk = pk.nsplit > 1 ? align_up(heads * pk.nsplit * s.Nk * s.D * 4, 256) : 0;
+  w.dv = w.part + dk;
+  w.bytes = w.part + (dq > 2 * dk ? dq : 2 * dk);
+  return w;
 }
 
 int check_shape(const eve_attn_shape* s) {
@@ -641,6 +826,7 @@ int check_shape(const eve_attn_shape* s) {
   EVE_REQUIRE(s->dtype == EVE_F32 || s->dtype == EVE_BF16, EVE_ERR_ARG, "eve_attn: dtype %d", s->dtype);
   EVE_REQUIRE(s->B >= 0 && s->Nq >= 0 && s->Nk >= 0, EVE_ERR_ARG, "eve_attn: negative size");
   EVE_REQUIRE(s->H >= 1 && s->Hkv >= 1 && s->H % s->Hkv == 0, EVE_ERR_ARG, "eve_attn: %d query heads do not share %d key heads", s->H, s->Hkv);
+  EVE_REQUIRE((int64_t)s->H * s->D <= (1 << 22), EVE_ERR_UNSUPPORTED, "eve_attn: %d heads of %d", s->H, s->D);
   EVE_REQUIRE(s->D >= 8 && s->D <= 128 && s->D % 8 == 0, EVE_ERR_UNSUPPORTED, "eve_attn: head width %d (a multiple of 8 up to 128)", s->D);
   EVE_REQUIRE(s->scale > 0.f && s->scale <= 3.4e38f, EVE_ERR_ARG, "eve_attn: scale must be positive and finite");
   EVE_REQUIRE((int64_t)s->Nq * (s->H / s->Hkv) <= 0x7fff0000LL && s->Nk <= 0x7fff0000, EVE_ERR_UNSUPPORTED, "eve_attn: too many rows");
@@ -655,6 +841,9 @@ int check_layout(const eve_attn_layout* l, int dtype, const char* what) {
   const int64_t e = dtype == EVE_BF16 ? 8 : 4;
   const int64_t st[9] = {l->q_b, l->q_n, l->q_h, l->k_b, l->k_n, l->k_h, l->v_b, l->v_n, l->v_h};
   for (int64_t x : st) EVE_REQUIRE(x >= 0 && x % e == 0, EVE_ERR_ARG, "eve_attn: %s strides must be multiples of 16 bytes", what);
+  // a tile of 64 rows is reached by 32-bit offsets from its first row (64-bit from tile to tile)
+  for (int i = 1; i < 9; i += 3)
+    EVE_REQUIRE(st[i] <= (1 << 22), EVE_ERR_UNSUPPORTED, "eve_attn: %s rows more than 2^22 elements apart", what);
   return EVE_OK;
 }
 
@@ -666,11 +855,14 @@ AttnArgs base_args(const eve_attn_shape& s) {
   a.nsplit = 1;
   a.scale = s.scale;
   a.c = (float)((double)s.scale * 1.4426950408889634);
+  a.inv_c = (float)(1.0 / ((double)s.scale * 1.4426950408889634));
   return a;
 }
 
-template <typename T, int DP> constexpr int attn_lds(bool stats) {
-  return 4 * AttnCfg<T, DP>::TILE + (stats ? 4 * AttnCfg<T, DP>::KT * 4 : 0);
+template <typename T, int DP> constexpr int attn_lds(int nw) { return (nw == 1 ? 2 : 4) * AttnCfg<T, DP>::TILE; }
+template <typename T, int DP> constexpr int dkv_lds() {
+  using C = AttnCfg<T, DP, dkv_rows<T, DP>()>;
+  return 4 * C::TILE + 2 * C::KT * 16;
 }
 
 int launch_attn(void (*kern)(AttnArgs), AttnArgs& a, int nw, int lds, hipStream_t st, const char* name) {
@@ -687,26 +879,50 @@ int launch_attn(void (*kern)(AttnArgs), AttnArgs& a, int nw, int lds, hipStream_
   return EVE_OK;
 }
 
+void use_plan(AttnArgs& a, const AttnPlan& p) {
+  a.nblk = p.nblk;
+  a.nsplit = p.nsplit;
+  a.tiles_per_split = p.tiles_per_split;
+}
+
 template <typename T, int DP>
-int fwd_typed(AttnArgs& a, const FwdPlan& p, hipStream_t st) {
-  int rc = launch_attn(p.nw == 1 ? attn_fwd_kernel<T, DP, 1> : attn_fwd_kernel<T, DP, 4>, a, p.nw, attn_lds<T, DP>(false), st, "eve_attn_fwd");
+int fwd_typed(AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+  use_plan(a, p);
+  const int rc = launch_attn(p.nw == 1 ? attn_fwd_kernel<T, DP, 1> : attn_fwd_kernel<T, DP, 4>, a, p.nw, attn_lds<T, DP>(p.nw), st, "eve_attn_fwd");
   if (rc != EVE_OK || a.nsplit == 1) return rc;
-  attn_join_kernel<T><<<dim3((unsigned)(((int64_t)a.heads * a.rows + 3) / 4)), dim3(256), 0, st>>>(a);
+  EVE_REQUIRE((int64_t)a.heads * a.rows <= 0x7fffffffLL, EVE_ERR_UNSUPPORTED, "eve_attn_fwd: too many rows");
+  attn_join_kernel<T><<<dim3((unsigned)(a.heads * a.rows)), dim3(256), 0, st>>>(a);
   EVE_CHECK_LAUNCH("eve_attn_fwd (join)");
   return EVE_OK;
 }
 
+template <typename T>
+int sum_parts(const AttnArgs& a, const float* part, void* g, int64_t g_b, int64_t g_n, int64_t g_h, int G, int rows, float factor, hipStream_t st) {
+  AttnSum s = {part, g, g_b, g_n, g_h, (int64_t)a.heads * rows * (a.D / 4), a.Hkv, G, a.D, rows, a.nsplit, factor};
+  const int64_t grid = (s.total + 255) / 256;
+  EVE_REQUIRE(grid <= 0x7fffffffLL, EVE_ERR_UNSUPPORTED, "eve_attn_bwd: too many rows");
+  attn_sum_kernel<T><<<dim3((unsigned)grid), dim3(256), 0, st>>>(s);
+  EVE_CHECK_LAUNCH("eve_attn_bwd (sum of the splits)");
+  return EVE_OK;
+}
+
 template <typename T, int DP>
-int bwd_typed(AttnArgs& a, hipStream_t st) {
-  const int nw_q = a.rows <= 64 ? 1 : 4, nw_k = 4;
+int bwd_typed(AttnArgs& a, const AttnPlan& pq, const AttnPlan& pk, hipStream_t st) {
   if (a.rows > 0) {
-    a.nblk = (a.rows + nw_q * 32 - 1) / (nw_q * 32);
-    const int rc = launch_attn(nw_q == 1 ? attn_dq_kernel<T, DP, 1> : attn_dq_kernel<T, DP, 4>, a, nw_q, attn_lds<T, DP>(false), st, "eve_attn_bwd (dq)");
+    use_plan(a, pq);
+    int rc = launch_attn(pq.nw == 1 ? attn_dq_kernel<T, DP, 1> : attn_dq_kernel<T, DP, 4>, a, pq.nw, attn_lds<T, DP>(pq.nw), st, "eve_attn_bwd (dq)");
+    if (rc == EVE_OK && a.nsplit > 1)
+      rc = sum_parts<T>(a, a.part_a, a.dq, a.grad.q_b, a.grad.q_n, a.grad.q_h, a.G, a.rows, a.scale, st);
     if (rc != EVE_OK) return rc;
   }
   if (a.Nk == 0) return EVE_OK;
-  a.nblk = (a.Nk + nw_k * 32 - 1) / (nw_k * 32);
-  return launch_attn(attn_dkv_kernel<T, DP, 4>, a, nw_k, attn_lds<T, DP>(true), st, "eve_attn_bwd (dk, dv)");
+  use_plan(a, pk);
+  int rc = launch_attn(attn_dkv_kernel<T, DP, 4>, a, pk.nw, dkv_lds<T, DP>(), st, "eve_attn_bwd (dk, dv)");
+  if (rc == EVE_OK && a.nsplit > 1)
+    rc = sum_parts<T>(a, a.part_a, a.dk, a.grad.k_b, a.grad.k_n, a.grad.k_h, 1, a.Nk, a.scale, st);
+  if (rc == EVE_OK && a.nsplit > 1)
+    rc = sum_parts<T>(a, a.part_b, a.dv, a.grad.v_b, a.grad.v_n, a.grad.v_h, 1, a.Nk, 1.f, st);
+  return rc;
 }
 
 }  // namespace
@@ -728,10 +944,9 @@ extern "C" int eve_attn_fwd(const eve_attn_shape* s, const eve_attn_layout* in, 
   if (s->B == 0 || s->Nq == 0) return EVE_OK;
   EVE_REQUIRE(q && out && (s->Nk == 0 || (k && v)), EVE_ERR_ARG, "eve_attn_fwd: null pointer");
   EVE_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), EVE_ERR_ARG, "eve_attn_fwd: pointers must be 16-byte aligned");
-  const FwdPlan p = fwd_plan(*s, attn_cus());
+  const AttnPlan p = fwd_plan(*s, attn_cus());
   AttnArgs a = base_args(*s);
   a.q = q; a.k = k; a.v = v; a.mask = key_mask; a.out = out; a.lse = lse; a.in = *in;
-  a.nblk = p.nblk; a.nsplit = p.nsplit; a.tiles_per_split = p.tiles_per_split;
   if (p.nsplit > 1) {
     EVE_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= fwd_ws(*s, p), EVE_ERR_WORKSPACE, "eve_attn_fwd: workspace of %zu bytes, %zu needed",
                 workspace_bytes, fwd_ws(*s, p));
@@ -746,7 +961,7 @@ extern "C" int eve_attn_fwd(const eve_attn_shape* s, const eve_attn_layout* in, 
 
 extern "C" size_t eve_attn_bwd_workspace_bytes(const eve_attn_shape* s) {
   if (check_shape(s) != EVE_OK) return 0;
-  return align_up((size_t)s->B * s->H * s->Nq * 4, 256);
+  return bwd_ws(*s, dq_plan(*s, attn_cus()), dkv_plan(*s, attn_cus())).bytes;
 }
 
 extern "C" int eve_attn_bwd(const eve_attn_shape* s, const eve_attn_layout* in, const eve_attn_layout* grad, const void* q,
@@ -763,13 +978,18 @@ extern "C" int eve_attn_bwd(const eve_attn_shape* s, const eve_attn_layout* in, 
   EVE_REQUIRE(s->Nk == 0 || (k && v && dk && dv), EVE_ERR_ARG, "eve_attn_bwd: null pointer");
   const void* ptrs[8] = {q, k, v, out, dout, dq, dk, dv};
   for (const void* x : ptrs) EVE_REQUIRE(aligned16(x), EVE_ERR_ARG, "eve_attn_bwd: pointers must be 16-byte aligned");
-  const size_t need = eve_attn_bwd_workspace_bytes(s);
-  EVE_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), EVE_ERR_WORKSPACE,
-              "eve_attn_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  const AttnPlan pq = dq_plan(*s, attn_cus()), pk = dkv_plan(*s, attn_cus());
+  const BwdWs ws = bwd_ws(*s, pq, pk);
+  EVE_REQUIRE(ws.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= ws.bytes), EVE_ERR_WORKSPACE,
+              "eve_attn_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, ws.bytes);
   AttnArgs a = base_args(*s);
   a.q = q; a.k = k; a.v = v; a.mask = key_mask; a.o = out; a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv;
-  a.lse = const_cast<float*>(lse); a.delta = static_cast<float*>(workspace); a.in = *in; a.grad = *grad;
+  a.lse = const_cast<float*>(lse); a.in = *in; a.grad = *grad;
+  char* base = static_cast<char*>(workspace);
+  a.delta = reinterpret_cast<float*>(base + ws.delta);
+  a.part_a = reinterpret_cast<float*>(base + ws.part);
+  a.part_b = reinterpret_cast<float*>(base + ws.dv);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (s->dtype == EVE_BF16) return s->D <= 64 ? bwd_typed<bf16_t, 64>(a, st) : bwd_typed<bf16_t, 128>(a, st);
-  return s->D <= 64 ? bwd_typed<float, 64>(a, st) : bwd_typed<float, 128>(a, st);
+  if (s->dtype == EVE_BF16) return s->D <= 64 ? bwd_typed<bf16_t, 64>(a, pq, pk, st) : bwd_typed<bf16_t, 128>(a, pq, pk, st);
+  return s->D <= 64 ? bwd_typed<float, 64>(a, pq, pk, st) : bwd_typed<float, 128>(a, pq, pk, st);
 }

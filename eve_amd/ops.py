@@ -422,9 +422,11 @@ def _attn_strides(t: torch.Tensor):
 
 
 def attn_readable(t: torch.Tensor) -> torch.Tensor:
-    """`t` [B,N,H,D] as the kernels can read it: the last dimension contiguous, rows on 16-byte boundaries; else a copy."""
+    """`t` [B,N,H,D] as the kernels can read it: the last dimension contiguous, rows on 16-byte boundaries and at most 2^22
+    elements apart; else a copy."""
     unit = 16 // t.element_size()
-    if t.numel() and (t.stride(3) != 1 or t.data_ptr() % 16 or any(s % unit for s in _attn_strides(t))):
+    strides = _attn_strides(t)
+    if t.numel() and (t.stride(3) != 1 or t.data_ptr() % 16 or strides[1] > 1 << 22 or any(s % unit for s in strides)):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
