@@ -17,8 +17,11 @@
 // long as the A operand follows, so chunk c of a 32-row accumulator supplies rows 16c + 4h + {0..3} and 16c + 8 + 4h + {0..3} (bf16)
 // and the A operand is read from LDS in that order (ds_read_b64_tr_b16: four rows of one column each).
 //
-// LDS rows are padded by 16 bytes, which serves both the 16-byte row reads and the transposed reads.  Tiles come through buffer
-// descriptors: a masked row is an offset outside the descriptor, for which the hardware delivers zeros without a branch.
+// LDS.  Tiles go from memory to LDS directly (buffer_load ... lds, 1 KiB a wave instruction) into a ring of stages, one tile
+// ahead of the one that is worked on.  A masked row is an offset outside the descriptor, for which the hardware delivers zeros.
+// The 16-byte chunks of a row are permuted by ((row & 3) << 1 | row >> 2 & 1) -- on the source side, since the transfer writes LDS
+// in lane order -- so that both ways of reading spread over all banks: the same chunk of eight consecutive rows (row fragments),
+// and a pair of chunks of four consecutive rows (transposed fragments).
 // No atomics: dq and dk/dv have a kernel each (7 products instead of 5), so results do not depend on the order of execution.
 #include <math.h>
 
@@ -38,7 +41,8 @@ struct AttnArgs {
   const void *q, *k, *v, *o, *dout;
   const uint8_t* mask;  // [B, Nk], nonzero = visible; may be null
   void *out, *dq, *dk, *dv;
-  float *lse, *delta;         // [B * Hkv, rows]
+  float* lse;                 // [B * Hkv, rows]
+  uint4* stats;               // [B * Hkv, rows]: -L / c and -delta, as the dk/dv kernel wants them
   float *part_o, *part_ml;    // forward splits: [B * Hkv, nsplit, rows, D] and [..., 2]
   float *part_a, *part_b;     // backward splits: dq | dk, and dv: [B * Hkv, nsplit, rows or keys, D]
   eve_attn_layout in, grad;   // element strides of q, k, v and of their gradients
@@ -55,17 +59,22 @@ template <typename T> struct AT;
 template <> struct AT<bf16_t> { static constexpr int E = 8; };
 template <> struct AT<float> { static constexpr int E = 4; };
 
-template <typename T, int DP, int KT_ = (sizeof(T) == 2 ? 64 : 32)> struct AttnCfg {
+template <typename T, int DP> struct AttnCfg {
   static constexpr int E = AT<T>::E;
   static constexpr int NKS = DP / (2 * E);              // contraction steps over the head width
   static constexpr int CPR = DP / E;                    // 16-byte chunks of a row
-  static constexpr int PITCH = DP * (int)sizeof(T) + 16;
-  static constexpr int KT = KT_;                        // rows of a staged tile
+  static constexpr int RB = DP * (int)sizeof(T);        // bytes of a row: 128, 256 or 512
+  static constexpr int KT = RB == 128 ? 64 : 32;        // rows of a staged tile
   static constexpr uint64_t kFull = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
-  static constexpr int TILE = KT * PITCH;
+  static constexpr int TILE = KT * RB;
+  static constexpr int STAGE = 2 * TILE;                // keys and values, or queries and gradients
+  static constexpr int NST = 2;                         // stages of the ring: NST - 1 tiles ahead
   static constexpr int PC = 32 / (2 * E);               // fragments of a 32-row accumulator
   static constexpr int ND = DP / 32;
+  static constexpr int NJ = KT / 32;
 };
+
+constexpr int kBitTiles = 64;  // tiles whose mask words a workgroup holds
 
 #if defined(__HIP_DEVICE_COMPILE__)
 __device__ __forceinline__ at_f32x16 mma(const uint4& a, const uint4& b, at_f32x16 acc, bf16_t) {
@@ -78,30 +87,93 @@ __device__ __forceinline__ at_f32x16 mma(const uint4& a, const uint4& b, at_f32x
   return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), acc, 0, 0, 0);
 }
 
-// row fragment: row r0 + (lane & 31), contraction step ks along the row
-template <int PITCH> __device__ __forceinline__ uint4 row_frag(const char* tile, int r0, int ks, int lane) {
-  return *reinterpret_cast<const uint4*>(tile + (r0 + (lane & 31)) * PITCH + (2 * ks + (lane >> 5)) * 16);
+// 16 bytes from LDS.  (A load of a vector type keeps its type information; without it the compiler takes the load for one that
+// may read what a transfer in flight writes, and waits for all of them.)
+typedef uint32_t at_u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 lds16(const char* p) {
+  const at_u32x4 w = *reinterpret_cast<const at_u32x4*>(p);
+  return make_uint4(w.x, w.y, w.z, w.w);
 }
-// column fragment: column d0 + (lane & 31), rows of chunk c of the 32 rows from r0, in the order of an accumulator's registers
-template <int PITCH> __device__ __forceinline__ uint4 col_frag(const char* tile, int r0, int c, int d0, int lane, bf16_t) {
-  const int i = lane & 15, q = i >> 2, p = i & 3, h = lane >> 5;
-  const char* a = tile + (r0 + 16 * c + 4 * h + q) * PITCH + (d0 + 16 * ((lane >> 4) & 1) + 4 * p) * 2;
-  const at_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (__attribute__((address_space(3))) at_s16x4*)(__attribute__((address_space(3))) char*)(const_cast<char*>(a)));
-  const at_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (__attribute__((address_space(3))) at_s16x4*)(__attribute__((address_space(3))) char*)(const_cast<char*>(a) + 8 * PITCH));
-  const at_s16x8 w = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  return __builtin_bit_cast(uint4, w);
+__device__ __forceinline__ int chunk_swizzle(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+__device__ __forceinline__ uint32_t lds_offset(const char* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
+
+// A lane's place in the row fragments of a tile (at smem + tile, a multiple of 128 bytes): row lane & 31 of 32-row block j, step ks.
+template <typename C> struct RowReader {
+  uint32_t base;
+  __device__ __forceinline__ explicit RowReader(int lane) {
+    const int row = lane & 31;
+    base = row * C::RB + (((lane >> 5) ^ chunk_swizzle(row)) << 4);
+  }
+  __device__ __forceinline__ uint4 get(const char* smem, uint32_t tile, int j, int ks) const {
+    return lds16(smem + (((tile + base) ^ ((ks & 3) << 5)) + (ks >> 2) * 128 + j * 32 * C::RB));
+  }
+};
+
+// Transposed fragments, bf16: column d0 + (lane & 31), rows of 16-row chunk rc in the order of an accumulator's registers (rows
+// 4 h + {0..3}, then 8 + 4 h + {0..3}).  Fragments -- of the two 16-row chunks of 32 rows, two column blocks -- are read and
+// waited for in one block: through the builtin the compiler would also wait for the tiles in flight, which it cannot tell apart
+// from what is read.
+template <int RB> __device__ __forceinline__ void tr_frags4(uint32_t a0, uint32_t a1, uint4 (&f)[4]) {  // f[2 chunk + column block]
+  at_s16x4 v[8];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%10\n\t"
+      "ds_read_b64_tr_b16 %4, %8 offset:%11\n\tds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %9 offset:%11\n\tds_read_b64_tr_b16 %7, %9 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(a0), "v"(a1), "n"(8 * RB), "n"(16 * RB), "n"(24 * RB)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const at_s16x8 w = __builtin_shufflevector(v[2 * i], v[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+    f[i] = __builtin_bit_cast(uint4, w);
+  }
 }
-template <int PITCH> __device__ __forceinline__ uint4 col_frag(const char* tile, int r0, int c, int d0, int lane, float) {
-  const char* a = tile + (r0 + 8 * c + 4 * (lane >> 5)) * PITCH + (d0 + (lane & 31)) * 4;
-  uint4 w;
-  w.x = *reinterpret_cast<const uint32_t*>(a);
-  w.y = *reinterpret_cast<const uint32_t*>(a + PITCH);
-  w.z = *reinterpret_cast<const uint32_t*>(a + 2 * PITCH);
-  w.w = *reinterpret_cast<const uint32_t*>(a + 3 * PITCH);
-  return w;
+// A lane's place in them: column blocks 0 and 1 (block i: (i & 1), + 128 (i >> 1) bytes)
+template <typename C> struct ColReader {
+  uint32_t base[2];
+  __device__ __forceinline__ explicit ColReader(int lane) {
+    const int i = lane & 15, q = i >> 2, p = i & 3, h = lane >> 5;
+    const int c = 2 * ((lane >> 4) & 1) + (p >> 1);
+    base[0] = (4 * h + q) * C::RB + ((c ^ (q << 1 | h)) << 4) + (p & 1) * 8;
+    base[1] = base[0] ^ 64;
+  }
+};
+// fp32: chunk c (8 rows) of the 32 rows from r0, column d0 + (lane & 31)
+template <typename C> __device__ __forceinline__ uint4 col_frag_f32(const char* smem, uint32_t tile, int r0, int c, int d0, int lane) {
+  const int h = lane >> 5, col = d0 + (lane & 31);
+  uint32_t w[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int row = r0 + 8 * c + 4 * h + t;
+    w[t] = *reinterpret_cast<const uint32_t*>(smem + (tile + row * C::RB + (((col >> 2) ^ (t << 1 | h)) << 4) + (col & 3) * 4));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
+// The column fragments of 32-row block j of a tile: f[c ND + i]
+template <typename T, typename C> struct ColFrags {
+  uint4 f[C::PC * C::ND];
+  __device__ __forceinline__ void read(const char* smem, uint32_t at, int j, const ColReader<C>& r, int lane) {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t tile = lds_offset(smem) + at + j * 32 * C::RB;
+#pragma unroll
+      for (int pair = 0; pair < C::ND / 2; ++pair) {
+        uint4 g[4];
+        tr_frags4<C::RB>(tile + r.base[0] + pair * 128, tile + r.base[1] + pair * 128, g);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) f[c * C::ND + 2 * pair + i] = g[2 * c + i];
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < C::PC; ++c)
+#pragma unroll
+        for (int i = 0; i < C::ND; ++i) f[c * C::ND + i] = col_frag_f32<C>(smem, at, 32 * j, c, 32 * i, lane);
+    }
+  }
+};
 __device__ __forceinline__ uint32_t at_pack(float lo, float hi) {
   const at_f32x2 t = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(t, at_bf16x2));
@@ -165,72 +237,85 @@ __device__ __forceinline__ bool block_coord(const AttnArgs& a, int& head, int& b
   return head < a.heads;
 }
 
-// which of the KT keys from key0 on are visible, bit by bit (the same in every lane)
-template <int KT> __device__ __forceinline__ uint64_t key_bits(const AttnArgs& a, const uint8_t* mask, int key0, int lane) {
-  const int key = key0 + lane;
-  bool see = lane < KT && key < a.Nk;
-  if (see && mask) see = mask[key] != 0;
-  return __ballot(see);
-}
-
-// Two tiles of KT rows x DP columns (keys and values, or queries and gradients) on their way to LDS through registers.  A row
-// without its bit is not read and arrives as zeros: whatever it holds, it takes no part.
 constexpr uint32_t kNowhere = 0xfffffff0u, kReach = 0x80000000u;  // an offset outside every descriptor, and their extent
-typedef uint32_t at_u32x4 __attribute__((ext_vector_type(4)));
-template <typename C, int NT> struct TilePair {
-  static constexpr int N = C::KT * C::CPR / NT, STEP = NT / C::CPR;  // chunks of a thread, rows between them
-  at_u32x4 x[N], y[N];
-  uint32_t x_off, y_off, x_row, y_row;  // first chunk, bytes of a row
-  int row0;
-  __device__ __forceinline__ TilePair(int64_t x_n, int64_t y_n, int D, int tid) {
-    row0 = tid / C::CPR;
-    const int c = tid % C::CPR;
-    x_row = (uint32_t)x_n * (16 / C::E);
-    y_row = (uint32_t)y_n * (16 / C::E);
-    const bool in = c * C::E < D;
-    x_off = in ? row0 * x_row + c * 16 : kNowhere;
-    y_off = in ? row0 * y_row + c * 16 : kNowhere;
-  }
-  __device__ __forceinline__ void load(const void* xp, const void* yp, uint64_t bits) {
-    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(xp), 0, kReach, 0x00020000);
-    const __amdgpu_buffer_rsrc_t yr = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(yp), 0, kReach, 0x00020000);
-    if (bits == C::kFull) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        x[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, x_off, i * STEP * x_row, 0);
-        y[i] = __builtin_amdgcn_raw_buffer_load_b128(yr, y_off, i * STEP * y_row, 0);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const bool see = (bits >> (row0 + i * STEP)) & 1;
-        x[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, see ? x_off : kNowhere, i * STEP * x_row, 0);
-        y[i] = __builtin_amdgcn_raw_buffer_load_b128(yr, see ? y_off : kNowhere, i * STEP * y_row, 0);
-      }
+
+// Which of the KT keys of a tile are visible, bit by bit.  A mask is turned into words in LDS, kBitTiles tiles at a time: were its
+// bytes loaded tile by tile, their wait would also be one for the tiles in flight, which the same counter counts.
+template <int KT, int NW> struct KeyBits {
+  const uint8_t* mask;
+  uint64_t* words;
+  int Nk, t0, t1, wave, lane;
+  // called by all waves, with t0, t0 + 1, ... one after the other
+  __device__ __forceinline__ uint64_t of(int t) const {
+    if (t >= t1) return 0;
+    if (!mask) {
+      const int n = Nk - t * KT;
+      return n >= KT ? (KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1) : (1ull << n) - 1;
     }
+    const int at = (t - t0) % kBitTiles;
+    if (at == 0) {
+      __syncthreads();
+#pragma unroll 4
+      for (int j = wave; j < kBitTiles; j += NW) {
+        const int key = (t + j) * KT + lane;
+        const uint64_t w = __ballot(t + j < t1 && lane < KT && key < Nk && mask[key] != 0);
+        if (lane == 0) words[j] = w;
+      }
+      __syncthreads();
+    }
+    const uint64_t w = words[at];
+    return (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(w >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)w);
   }
-  __device__ __forceinline__ void store(char* xs, char* ys, int tid) const {
-    const int at = row0 * C::PITCH + (tid % C::CPR) * 16;
+};
+
+// Pieces of 1 KiB of a tile, dealt to the NW waves; lane l of piece p holds chunk l % CPR of row p (64 / CPR) + l / CPR.
+template <typename C, int NW> struct TileLoader {
+  static constexpr int N = C::TILE / 1024 / NW;  // a wave's transfers for a tile
+  uint32_t off[N];
+  int row[N];
+  __device__ __forceinline__ TileLoader(int64_t stride, int D, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      *reinterpret_cast<at_u32x4*>(xs + at + i * STEP * C::PITCH) = x[i];
-      *reinterpret_cast<at_u32x4*>(ys + at + i * STEP * C::PITCH) = y[i];
+      row[i] = (i * NW + wave) * (64 / C::CPR) + lane / C::CPR;
+      const int c = (lane % C::CPR) ^ chunk_swizzle(row[i]);
+      off[i] = c * C::E < D ? (uint32_t)row[i] * ((uint32_t)stride * (16 / C::E)) + c * 16 : kNowhere;
+    }
+  }
+  __device__ __forceinline__ void load(const void* p, char* tile, int wave, uint64_t bits) const {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, kReach, 0x00020000);
+    auto to_lds = [&](int i, uint32_t o) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(tile + (i * NW + wave) * 1024), 16, o, 0, 0, 0);
+    };
+    if (bits == C::kFull) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) to_lds(i, off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) to_lds(i, (bits >> row[i]) & 1 ? off[i] : kNowhere);
     }
   }
 };
+// Waits until this wave's transfers of a tile have landed while the NEWER ones of later tiles may be in flight (loads between them
+// only make the wait stricter), then for the other waves, which also have read what the next transfer overwrites.
+template <int NEWER> __device__ __forceinline__ void tile_ready() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NEWER) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// No transfer may be on its way into LDS when the workgroup ends.
+__device__ __forceinline__ void tiles_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 #endif  // __HIP_DEVICE_COMPILE__
 
 // ---------------------------------------------------------------------------------------------------------- forward
-// Block: NW waves of 32 rows each; the key tiles are staged for all of them, two stages deep.  A block of one wave (few rows,
-// bound by the keys' bytes) has one stage, so that more of them fit a CU.
+// Block: NW waves of 32 rows each; the key tiles are staged for all of them.
 // The bounds on waves keep the register budget at 256, where the compiler holds accumulators in plain registers: in the larger
 // budget it moves them to and from accumulation registers, a third of the instructions of the loop.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 64 ? 3 : 2) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) == 2 ? 4 : 3) void attn_fwd_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using C = AttnCfg<T, DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, wave_u = __builtin_amdgcn_readfirstlane(wave);
   int head, blk, split;
   if (!block_coord(a, head, blk, split)) return;
   const int b = head / a.Hkv, hk = head % a.Hkv;
@@ -258,46 +343,48 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 64 ? 3 : 2) void attn_
 
   const int ntiles = (a.Nk + C::KT - 1) / C::KT;
   const int t0 = split * a.tiles_per_split, t1 = min(ntiles, t0 + a.tiles_per_split);
-  TilePair<C, NW * 64> kv(a.in.k_n, a.in.v_n, a.D, tid);
-  auto fetch = [&](int t, uint64_t bits) {
-    kv.load(kb + (int64_t)t * C::KT * a.in.k_n, vb + (int64_t)t * C::KT * a.in.v_n, bits);
+  const TileLoader<C, NW> kl(a.in.k_n, a.D, wave, lane), vl(a.in.v_n, a.D, wave, lane);
+  const RowReader<C> rows(lane);
+  const ColReader<C> cols(lane);
+  const KeyBits<C::KT, NW> keys{mask, reinterpret_cast<uint64_t*>(smem + C::NST * C::STAGE), a.Nk, t0, t1, wave, lane};
+  // of tiles t .. t + NST - 1
+  uint64_t bits[C::NST];
+  auto fetch = [&](int t, uint64_t b) {  // past the last tile: nothing is read
+    char* stage = smem + (t - t0) % C::NST * C::STAGE;
+    kl.load(kb + (int64_t)t * C::KT * a.in.k_n, stage, wave_u, b);
+    vl.load(vb + (int64_t)t * C::KT * a.in.v_n, stage + C::TILE, wave_u, b);
   };
-  uint64_t bits = 0, bits_next = 0;
-  if (t0 < t1) {
-    bits = key_bits<C::KT>(a, mask, t0 * C::KT, lane);
-    fetch(t0, bits);
-    if (t0 + 1 < t1) bits_next = key_bits<C::KT>(a, mask, (t0 + 1) * C::KT, lane);
+#pragma unroll
+  for (int i = 0; i < C::NST - 1; ++i) {
+    bits[i] = keys.of(t0 + i);
+    fetch(t0 + i, bits[i]);
   }
   for (int t = t0; t < t1; ++t) {
-    char* ks_ = smem + (NW == 1 ? 0 : ((t - t0) & 1) * (2 * C::TILE));
-    char* vs_ = ks_ + C::TILE;
-    if (NW == 1) __syncthreads();
-    kv.store(ks_, vs_, tid);
-    __syncthreads();
-    uint64_t bits_after = 0;
-    if (t + 1 < t1) {
-      fetch(t + 1, bits_next);
-      if (t + 2 < t1) bits_after = key_bits<C::KT>(a, mask, (t + 2) * C::KT, lane);
-    }
-    if (bits) {
-      at_f32x16 s[C::KT / 32];
+    const uint32_t ks_ = (t - t0) % C::NST * C::STAGE, vs_ = ks_ + C::TILE;
+    tile_ready<2 * TileLoader<C, NW>::N * (C::NST - 2)>();
+    bits[C::NST - 1] = keys.of(t + C::NST - 1);
+    fetch(t + C::NST - 1, bits[C::NST - 1]);
+    if (bits[0]) {
+      at_f32x16 s[C::NJ];
 #pragma unroll
-      for (int j = 0; j < C::KT / 32; ++j) {
+      for (int j = 0; j < C::NJ; ++j) {
         s[j] = acc_zero();
 #pragma unroll
-        for (int ks = 0; ks < C::NKS; ++ks) s[j] = mma(row_frag<C::PITCH>(ks_, 32 * j, ks, lane), qf[ks], s[j], T());
+        for (int ks = 0; ks < C::NKS; ++ks) s[j] = mma(rows.get(smem, ks_, j, ks), qf[ks], s[j], T());
       }
-      if (bits != C::kFull) {
-        const uint64_t mine = bits >> (4 * half);
+      ColFrags<T, C> vf;  // read while the matrix unit works on the scores
+      vf.read(smem, vs_, 0, cols, lane);
+      if (bits[0] != C::kFull) {
+        const uint64_t mine = bits[0] >> (4 * half);
 #pragma unroll
-        for (int j = 0; j < C::KT / 32; ++j)
+        for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (!((mine >> (32 * j + (r & 3) + 8 * (r >> 2))) & 1)) s[j][r] = -INFINITY;
       }
       float mt = s[0][0];
 #pragma unroll
-      for (int j = 0; j < C::KT / 32; ++j)
+      for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[j][r]);
       const float m_new = fmaxf(m, halves_max(mt) * a.c);
@@ -306,7 +393,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 64 ? 3 : 2) void attn_
       m = m_new;
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < C::KT / 32; ++j)
+      for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[j][r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], a.c, -ms));
@@ -320,17 +407,20 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 64 ? 3 : 2) void attn_
           for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
       }
 #pragma unroll
-      for (int j = 0; j < C::KT / 32; ++j)
+      for (int j = 0; j < C::NJ; ++j) {
+        if (j > 0) vf.read(smem, vs_, j, cols, lane);
 #pragma unroll
         for (int cc = 0; cc < C::PC; ++cc) {
           const uint4 p = acc_frag(s[j], cc, T());
 #pragma unroll
-          for (int i = 0; i < C::ND; ++i) o[i] = mma(col_frag<C::PITCH>(vs_, 32 * j, cc, 32 * i, lane, T()), p, o[i], T());
+          for (int i = 0; i < C::ND; ++i) o[i] = mma(vf.f[cc * C::ND + i], p, o[i], T());
         }
+      }
     }
-    bits = bits_next;
-    bits_next = bits_after;
+#pragma unroll
+    for (int i = 0; i < C::NST - 1; ++i) bits[i] = bits[i + 1];
   }
+  tiles_landed();
   l = halves_sum(l);
   if (!row_ok) return;
   if (a.nsplit == 1) {
@@ -449,14 +539,31 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(AttnSum a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------- dq
+#if defined(__HIP_DEVICE_COMPILE__)
+// x = hi + mid + lo exactly, eight bits of the significand each
+__device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffff0000u;
+  const float r = x - __uint_as_float(hi);
+  mid = __float_as_uint(r) & 0xffff0000u;
+  lo = __float_as_uint(r - __uint_as_float(mid)) & 0xffff0000u;
+}
+// -L / c and -delta as three bf16 each (a row that sees nothing: p = 2^(-1e30) = 0)
+__device__ __forceinline__ uint4 row_stats(float L, float delta, float inv_c) {
+  uint32_t l0, l1, l2, d0, d1, d2;
+  split3(fminf(L, 1e30f) * -inv_c, l0, l1, l2);
+  split3(-delta, d0, d1, d2);
+  return make_uint4((l0 >> 16) | l1, (l2 >> 16) | d0, (d1 >> 16) | d2, 0);
+}
+#endif
+
 // The forward's shape: columns are query rows, the key tiles pass by (or a split of them).  Also forms delta_i for the dk/dv
 // kernel.  -delta is the accumulator that the product do v^T starts from.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ? 1 : sizeof(T) == 2 && DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using C = AttnCfg<T, DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, wave_u = __builtin_amdgcn_readfirstlane(wave);
   int head, blk, split;
   if (!block_coord(a, head, blk, split)) return;
   const int b = head / a.Hkv, hk = head % a.Hkv;
@@ -487,7 +594,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
     delta = halves_sum(delta);
     if (row_ok) {
       L = a.lse[lrow];
-      if (half == 0 && split == 0) a.delta[lrow] = delta;
+      if (half == 0 && split == 0) a.stats[lrow] = row_stats(L, delta, a.inv_c);
     }
   }
   at_f32x16 minus_delta;
@@ -499,40 +606,41 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
 
   const int ntiles = (a.Nk + C::KT - 1) / C::KT;
   const int t0 = split * a.tiles_per_split, t1 = min(ntiles, t0 + a.tiles_per_split);
-  TilePair<C, NW * 64> kv(a.in.k_n, a.in.v_n, a.D, tid);
-  auto fetch = [&](int t, uint64_t bits) {
-    kv.load(kb + (int64_t)t * C::KT * a.in.k_n, vb + (int64_t)t * C::KT * a.in.v_n, bits);
+  const TileLoader<C, NW> kl(a.in.k_n, a.D, wave, lane), vl(a.in.v_n, a.D, wave, lane);
+  const RowReader<C> rows(lane);
+  const ColReader<C> cols(lane);
+  const KeyBits<C::KT, NW> keys{mask, reinterpret_cast<uint64_t*>(smem + C::NST * C::STAGE), a.Nk, t0, t1, wave, lane};
+  uint64_t bits[C::NST];
+  auto fetch = [&](int t, uint64_t b) {  // past the last tile: nothing is read
+    char* stage = smem + (t - t0) % C::NST * C::STAGE;
+    kl.load(kb + (int64_t)t * C::KT * a.in.k_n, stage, wave_u, b);
+    vl.load(vb + (int64_t)t * C::KT * a.in.v_n, stage + C::TILE, wave_u, b);
   };
-  uint64_t bits = 0, bits_next = 0;
-  if (t0 < t1) {
-    bits = key_bits<C::KT>(a, mask, t0 * C::KT, lane);
-    fetch(t0, bits);
-    if (t0 + 1 < t1) bits_next = key_bits<C::KT>(a, mask, (t0 + 1) * C::KT, lane);
+#pragma unroll
+  for (int i = 0; i < C::NST - 1; ++i) {
+    bits[i] = keys.of(t0 + i);
+    fetch(t0 + i, bits[i]);
   }
   for (int t = t0; t < t1; ++t) {
-    char* ks_ = smem + (NW == 1 ? 0 : ((t - t0) & 1) * (2 * C::TILE));
-    char* vs_ = ks_ + C::TILE;
-    if (NW == 1) __syncthreads();
-    kv.store(ks_, vs_, tid);
-    __syncthreads();
-    uint64_t bits_after = 0;
-    if (t + 1 < t1) {
-      fetch(t + 1, bits_next);
-      if (t + 2 < t1) bits_after = key_bits<C::KT>(a, mask, (t + 2) * C::KT, lane);
-    }
-    if (bits) {
-      const uint64_t mine = bits >> (4 * half);
+    const uint32_t ks_ = (t - t0) % C::NST * C::STAGE, vs_ = ks_ + C::TILE;
+    tile_ready<2 * TileLoader<C, NW>::N * (C::NST - 2)>();
+    bits[C::NST - 1] = keys.of(t + C::NST - 1);
+    fetch(t + C::NST - 1, bits[C::NST - 1]);
+    if (bits[0]) {
 #pragma unroll
-      for (int j = 0; j < C::KT / 32; ++j) {
+      for (int j = 0; j < C::NJ; ++j) {
         at_f32x16 s = acc_zero(), dp = minus_delta;
 #pragma unroll
         for (int ks = 0; ks < C::NKS; ++ks) {
-          s = mma(row_frag<C::PITCH>(ks_, 32 * j, ks, lane), qf[ks], s, T());
-          dp = mma(row_frag<C::PITCH>(vs_, 32 * j, ks, lane), gf[ks], dp, T());
+          s = mma(rows.get(smem, ks_, j, ks), qf[ks], s, T());
+          dp = mma(rows.get(smem, vs_, j, ks), gf[ks], dp, T());
         }
+        ColFrags<T, C> kf;  // read while the matrix unit works
+        kf.read(smem, ks_, j, cols, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -L)) * dp[r];
-        if (bits != C::kFull) {
+        if (bits[0] != C::kFull) {
+          const uint64_t mine = bits[0] >> (4 * half);
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (!((mine >> (32 * j + (r & 3) + 8 * (r >> 2))) & 1)) s[r] = 0.f;
@@ -541,13 +649,14 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
         for (int cc = 0; cc < C::PC; ++cc) {
           const uint4 p = acc_frag(s, cc, T());
 #pragma unroll
-          for (int i = 0; i < C::ND; ++i) dq[i] = mma(col_frag<C::PITCH>(ks_, 32 * j, cc, 32 * i, lane, T()), p, dq[i], T());
+          for (int i = 0; i < C::ND; ++i) dq[i] = mma(kf.f[cc * C::ND + i], p, dq[i], T());
         }
       }
     }
-    bits = bits_next;
-    bits_next = bits_after;
+#pragma unroll
+    for (int i = 0; i < C::NST - 1; ++i) bits[i] = bits[i + 1];
   }
+  tiles_landed();
   if (!row_ok) return;
   if (a.nsplit > 1) {
     float* p = a.part_a + (((int64_t)head * a.nsplit + split) * a.rows + row) * a.D;
@@ -573,27 +682,19 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
 }
 
 // ---------------------------------------------------------------------------------------------------------- dk, dv
-// x = hi + mid + lo exactly, eight bits of the significand each
-__device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-  hi = __float_as_uint(x) & 0xffff0000u;
-  const float r = x - __uint_as_float(hi);
-  mid = __float_as_uint(r) & 0xffff0000u;
-  lo = __float_as_uint(r - __uint_as_float(mid)) & 0xffff0000u;
-}
-
 // Columns are keys, held in registers; tiles of query rows (head after head of those that share the keys) pass by.
 //
 // Here L_i and delta_i belong to a row, that is, to a register, the same in 32 lanes.  The products start from -L_i / c and -delta_i:
-// p = 2^(c acc), ds = p acc'.  For bf16 these starts are themselves a matrix product: a row's 16 bytes hold both values as three
-// bf16 each, which multiply ones; read as values, four at a time, they would be a third of the LDS traffic that bounds this loop.
-template <typename T, int DP> constexpr int dkv_rows() { return sizeof(T) == 2 && DP == 64 ? 64 : 32; }
+// p = 2^(c acc), ds = p acc'.  These starts are themselves a matrix product: a row's 16 bytes hold both values as three bf16 each
+// (exactly, 24 bits), which multiply ones; read as values, four at a time, they would be a third of the loop's LDS traffic.
+// A row past the end is all zeros: p = 1 there, and its q and do, which p and ds multiply, are zero.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using C = AttnCfg<T, DP, dkv_rows<T, DP>()>;
+  using C = AttnCfg<T, DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  char* stats = smem + 4 * C::TILE;  // [2 stages][KT] of 16 bytes
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  char* stats = smem + C::NST * C::STAGE;  // [NST][64] of 16 bytes
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, wave_u = __builtin_amdgcn_readfirstlane(wave);
   int head, blk, split;
   if (!block_coord(a, head, blk, split)) return;
   const int b = head / a.Hkv, hk = head % a.Hkv;
@@ -629,63 +730,42 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
   const int tq = (a.Nq + C::KT - 1) / C::KT;
   // a block without a visible key has nothing to add up (the same decision in all its waves)
   const int t0 = split * a.tiles_per_split, t1 = __syncthreads_or(see) ? min(tq * a.G, t0 + a.tiles_per_split) : t0;
-  TilePair<C, NW * 64> qg(a.in.q_n, o_n, a.D, tid);
-  float st_L = 0.f, st_d = 0.f;
-  int g = tq ? t0 / tq : 0, tr = tq ? t0 % tq : 0;  // head of the group, tile of its rows
-  auto fetch = [&]() {
-    const int r0 = tr * C::KT, n = a.Nq - r0;
-    qg.load(qb + g * a.in.q_h + r0 * a.in.q_n, gb + (int64_t)g * a.D + r0 * o_n, n >= C::KT ? C::kFull : (1ull << n) - 1);
-    if (tid < C::KT) {  // rows past the end: p = 2^(-1e30) = 0
-      const int64_t i = (int64_t)head * a.rows + (int64_t)(r0 + tid) * a.G + g;
-      st_L = tid < n ? fminf(a.lse[i], 1e30f) : 1e30f;
-      st_d = tid < n ? a.delta[i] : 0.f;
+  const TileLoader<C, NW> ql(a.in.q_n, a.D, wave, lane), gl(o_n, a.D, wave, lane);
+  const RowReader<C> rows(lane);
+  const ColReader<C> cols(lane);
+  // tile t: head t / tq of the group, rows from (t % tq) KT on; past the last one nothing is read
+  auto fetch = [&](int t) {
+    const int g = t < t1 ? t / tq : 0, r0 = t < t1 ? (t - g * tq) * C::KT : 0, n = t < t1 ? a.Nq - r0 : 0;
+    const uint64_t bits = n >= C::KT ? C::kFull : (1ull << n) - 1;
+    const int slot = (t - t0) % C::NST;
+    char* stage = smem + slot * C::STAGE;
+    if (wave_u == 0) {
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(a.stats + (int64_t)head * a.rows + (int64_t)r0 * a.G + g, 0, kReach, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(stats + slot * 1024), 16,
+                                               lane < n && lane < C::KT ? (uint32_t)lane * a.G * 16 : kNowhere, 0, 0, 0);
     }
-    if (++tr == tq) { tr = 0; ++g; }
+    ql.load(qb + g * a.in.q_h + r0 * a.in.q_n, stage, wave_u, bits);
+    gl.load(gb + (int64_t)g * a.D + r0 * o_n, stage + C::TILE, wave_u, bits);
   };
-  if (t0 < t1) fetch();
+#pragma unroll
+  for (int i = 0; i < C::NST - 1; ++i) fetch(t0 + i);
   for (int t = t0; t < t1; ++t) {
-    char* qs_ = smem + ((t - t0) & 1) * (2 * C::TILE);
-    char* gs_ = qs_ + C::TILE;
-    char* st_ = stats + ((t - t0) & 1) * (C::KT * 16);
-    qg.store(qs_, gs_, tid);
-    if (tid < C::KT) {
-      if constexpr (sizeof(T) == 2) {
-        uint32_t l0, l1, l2, d0, d1, d2;
-        split3(st_L * -a.inv_c, l0, l1, l2);
-        split3(-st_d, d0, d1, d2);
-        *reinterpret_cast<uint4*>(st_ + tid * 16) = make_uint4((l0 >> 16) | l1, (l2 >> 16) | d0, (d1 >> 16) | d2, 0);
-      } else {
-        reinterpret_cast<float*>(st_)[tid] = st_L * -a.inv_c;
-        reinterpret_cast<float*>(st_)[C::KT + tid] = -st_d;
-      }
-    }
-    __syncthreads();
-    if (t + 1 < t1) fetch();
+    const uint32_t qs_ = (t - t0) % C::NST * C::STAGE, gs_ = qs_ + C::TILE;
+    const char* st_ = stats + (t - t0) % C::NST * 1024;
+    tile_ready<2 * TileLoader<C, NW>::N * (C::NST - 2)>();  // (wave 0 has one transfer more a tile, ahead of the others)
+    fetch(t + C::NST - 1);
     if (wave_sees) {
 #pragma unroll
-      for (int j = 0; j < C::KT / 32; ++j) {
-        at_f32x16 s = acc_zero(), dp = acc_zero();
-        if constexpr (sizeof(T) == 2) {
-          const uint4 both = *reinterpret_cast<const uint4*>(st_ + (32 * j + (lane & 31)) * 16);
-          s = mma(both, one_L, s, T());
-          dp = mma(both, one_d, dp, T());
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const at_f32x4 L = *reinterpret_cast<const at_f32x4*>(st_ + (32 * j + 8 * i + 4 * half) * 4);
-            const at_f32x4 de = *reinterpret_cast<const at_f32x4*>(st_ + (C::KT + 32 * j + 8 * i + 4 * half) * 4);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              s[4 * i + r] = L[r];
-              dp[4 * i + r] = de[r];
-            }
-          }
-        }
+      for (int j = 0; j < C::NJ; ++j) {
+        const uint4 both = lds16(st_ + (32 * j + (lane & 31)) * 16);
+        at_f32x16 s = mma(both, one_L, acc_zero(), bf16_t()), dp = mma(both, one_d, acc_zero(), bf16_t());
 #pragma unroll
         for (int ks = 0; ks < C::NKS; ++ks) {
-          s = mma(row_frag<C::PITCH>(qs_, 32 * j, ks, lane), kf[ks], s, T());
-          dp = mma(row_frag<C::PITCH>(gs_, 32 * j, ks, lane), vf[ks], dp, T());
+          s = mma(rows.get(smem, qs_, j, ks), kf[ks], s, T());
+          dp = mma(rows.get(smem, gs_, j, ks), vf[ks], dp, T());
         }
+        ColFrags<T, C> f;  // of do, read while the matrix unit works
+        f.read(smem, gs_, j, cols, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[r] = __builtin_amdgcn_exp2f(s[r] * a.c);
@@ -693,16 +773,21 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
         }
 #pragma unroll
         for (int cc = 0; cc < C::PC; ++cc) {
-          const uint4 p = acc_frag(s, cc, T()), ds = acc_frag(dp, cc, T());
+          const uint4 p = acc_frag(s, cc, T());
 #pragma unroll
-          for (int i = 0; i < C::ND; ++i) {
-            dv[i] = mma(col_frag<C::PITCH>(gs_, 32 * j, cc, 32 * i, lane, T()), p, dv[i], T());
-            dk[i] = mma(col_frag<C::PITCH>(qs_, 32 * j, cc, 32 * i, lane, T()), ds, dk[i], T());
-          }
+          for (int i = 0; i < C::ND; ++i) dv[i] = mma(f.f[cc * C::ND + i], p, dv[i], T());
+        }
+        f.read(smem, qs_, j, cols, lane);
+#pragma unroll
+        for (int cc = 0; cc < C::PC; ++cc) {
+          const uint4 ds = acc_frag(dp, cc, T());
+#pragma unroll
+          for (int i = 0; i < C::ND; ++i) dk[i] = mma(f.f[cc * C::ND + i], ds, dk[i], T());
         }
       }
     }
   }
+  tiles_landed();
   if (!key_ok) return;
   // a column's sums are its own: a masked key's are dropped here
   if (a.nsplit > 1) {
@@ -781,24 +866,22 @@ AttnPlan plan_of(int64_t rows, int nw, int64_t heads, int64_t tiles, int64_t wan
 }
 
 int64_t q_rows(const eve_attn_shape& s) { return (int64_t)s.Nq * (s.H / s.Hkv); }
-int64_t key_tiles(const eve_attn_shape& s) {
-  const int kt = s.dtype == EVE_BF16 ? 64 : 32;
-  return ((int64_t)s.Nk + kt - 1) / kt;
-}
+int tile_rows(const eve_attn_shape& s) { return s.dtype == EVE_BF16 && s.D <= 64 ? 64 : 32; }
+int64_t key_tiles(const eve_attn_shape& s) { return ((int64_t)s.Nk + tile_rows(s) - 1) / tile_rows(s); }
 
 // Few rows against many keys: the key tiles are split until the launch fills the CUs, and the parts are joined.  Up to 64 rows a
-// head go to blocks of one wave, of which 8 (head width up to 64) or 4 fit a CU.
+// head go to blocks of one wave, of which three fit a CU.
 AttnPlan fwd_plan(const eve_attn_shape& s, int cus) {
   const int nw = q_rows(s) <= 64 ? 1 : 4;
-  return plan_of(q_rows(s), nw, (int64_t)s.B * s.Hkv, key_tiles(s), (int64_t)cus * (nw == 4 ? 2 : s.D <= 64 ? 8 : 4), 2);
+  return plan_of(q_rows(s), nw, (int64_t)s.B * s.Hkv, key_tiles(s), (int64_t)cus * (nw == 4 ? 2 : 3), 4);
 }
 AttnPlan dq_plan(const eve_attn_shape& s, int cus) {
   const int nw = q_rows(s) <= 64 ? 1 : 4;
-  return plan_of(q_rows(s), nw, (int64_t)s.B * s.Hkv, key_tiles(s), (int64_t)cus * (nw == 4 ? 2 : 4), 4);
+  return plan_of(q_rows(s), nw, (int64_t)s.B * s.Hkv, key_tiles(s), (int64_t)cus * (nw == 4 ? 2 : 3), 4);
 }
 // The row tiles are counted head by head of a group, as the kernel walks them.
 AttnPlan dkv_plan(const eve_attn_shape& s, int cus) {
-  const int kt = s.dtype == EVE_BF16 && s.D <= 64 ? 64 : 32;
+  const int kt = tile_rows(s);
   return plan_of(s.Nk, 4, (int64_t)s.B * s.Hkv, ((int64_t)s.Nq + kt - 1) / kt * (s.H / s.Hkv), (int64_t)cus * 2, 4);
 }
 
@@ -807,13 +890,13 @@ size_t fwd_ws(const eve_attn_shape& s, const AttnPlan& p) {
   const size_t rows = (size_t)s.B * s.Hkv * p.nsplit * q_rows(s);
   return align_up(rows * s.D * 4, 256) + align_up(rows * 8, 256);
 }
-// delta, then the parts of dq, and in their place afterwards those of dk and dv
-struct BwdWs { size_t delta, part, dv, bytes; };
+// the rows' statistics, then the parts of dq, and in their place afterwards those of dk and dv
+struct BwdWs { size_t stats, part, dv, bytes; };
 BwdWs bwd_ws(const eve_attn_shape& s, const AttnPlan& pq, const AttnPlan& pk) {
   BwdWs w;
   const size_t heads = (size_t)s.B * s.Hkv;
-  w.delta = 0;
-  w.part = align_up(heads * q_rows(s) * 4, 256);
+  w.stats = 0;
+  w.part = align_up(heads * q_rows(s) * 16, 256);
   const size_t dq = pq.nsplit > 1 ? align_up(heads * pq.nsplit * q_rows(s) * s.D * 4, 256) : 0;
   const size_t dk = pk.nsplit > 1 ? align_up(heads * pk.nsplit * s.Nk * s.D * 4, 256) : 0;
   w.dv = w.part + dk;
@@ -859,11 +942,9 @@ AttnArgs base_args(const eve_attn_shape& s) {
   return a;
 }
 
-template <typename T, int DP> constexpr int attn_lds(int nw) { return (nw == 1 ? 2 : 4) * AttnCfg<T, DP>::TILE; }
-template <typename T, int DP> constexpr int dkv_lds() {
-  using C = AttnCfg<T, DP, dkv_rows<T, DP>()>;
-  return 4 * C::TILE + 2 * C::KT * 16;
-}
+// the ring, and behind it the mask's words or the rows' statistics
+template <typename T, int DP> constexpr int attn_lds() { return AttnCfg<T, DP>::NST * AttnCfg<T, DP>::STAGE + kBitTiles * 8; }
+template <typename T, int DP> constexpr int dkv_lds() { return AttnCfg<T, DP>::NST * (AttnCfg<T, DP>::STAGE + 1024); }
 
 int launch_attn(void (*kern)(AttnArgs), AttnArgs& a, int nw, int lds, hipStream_t st, const char* name) {
   const int64_t per = (int64_t)a.nblk * a.nsplit;
@@ -888,7 +969,7 @@ void use_plan(AttnArgs& a, const AttnPlan& p) {
 template <typename T, int DP>
 int fwd_typed(AttnArgs& a, const AttnPlan& p, hipStream_t st) {
   use_plan(a, p);
-  const int rc = launch_attn(p.nw == 1 ? attn_fwd_kernel<T, DP, 1> : attn_fwd_kernel<T, DP, 4>, a, p.nw, attn_lds<T, DP>(p.nw), st, "eve_attn_fwd");
+  const int rc = launch_attn(p.nw == 1 ? attn_fwd_kernel<T, DP, 1> : attn_fwd_kernel<T, DP, 4>, a, p.nw, attn_lds<T, DP>(), st, "eve_attn_fwd");
   if (rc != EVE_OK || a.nsplit == 1) return rc;
   EVE_REQUIRE((int64_t)a.heads * a.rows <= 0x7fffffffLL, EVE_ERR_UNSUPPORTED, "eve_attn_fwd: too many rows");
   attn_join_kernel<T><<<dim3((unsigned)(a.heads * a.rows)), dim3(256), 0, st>>>(a);
@@ -910,7 +991,7 @@ template <typename T, int DP>
 int bwd_typed(AttnArgs& a, const AttnPlan& pq, const AttnPlan& pk, hipStream_t st) {
   if (a.rows > 0) {
     use_plan(a, pq);
-    int rc = launch_attn(pq.nw == 1 ? attn_dq_kernel<T, DP, 1> : attn_dq_kernel<T, DP, 4>, a, pq.nw, attn_lds<T, DP>(pq.nw), st, "eve_attn_bwd (dq)");
+    int rc = launch_attn(pq.nw == 1 ? attn_dq_kernel<T, DP, 1> : attn_dq_kernel<T, DP, 4>, a, pq.nw, attn_lds<T, DP>(), st, "eve_attn_bwd (dq)");
     if (rc == EVE_OK && a.nsplit > 1)
       rc = sum_parts<T>(a, a.part_a, a.dq, a.grad.q_b, a.grad.q_n, a.grad.q_h, a.G, a.rows, a.scale, st);
     if (rc != EVE_OK) return rc;
@@ -986,7 +1067,7 @@ extern "C" int eve_attn_bwd(const eve_attn_shape* s, const eve_attn_layout* in, 
   a.q = q; a.k = k; a.v = v; a.mask = key_mask; a.o = out; a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv;
   a.lse = const_cast<float*>(lse); a.in = *in; a.grad = *grad;
   char* base = static_cast<char*>(workspace);
-  a.delta = reinterpret_cast<float*>(base + ws.delta);
+  a.stats = reinterpret_cast<uint4*>(base + ws.stats);
   a.part_a = reinterpret_cast<float*>(base + ws.part);
   a.part_b = reinterpret_cast<float*>(base + ws.dv);
   hipStream_t st = static_cast<hipStream_t>(stream);
