@@ -87,9 +87,10 @@ __device__ __forceinline__ at_f32x16 mma(const uint4& a, const uint4& b, at_f32x
   return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), acc, 0, 0, 0);
 }
 
-// 16 bytes from LDS.  (A load of a vector type keeps its type information; without it the compiler takes the load for one that
-// may read what a transfer in flight writes, and waits for all of them.)
+// 16 bytes from LDS.  (An access of a vector type keeps its type information; without it the compiler takes it for one that may
+// meet what a transfer in flight writes, and waits for all of them.)
 typedef uint32_t at_u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t at_u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint4 lds16(const char* p) {
   const at_u32x4 w = *reinterpret_cast<const at_u32x4*>(p);
   return make_uint4(w.x, w.y, w.z, w.w);
@@ -347,24 +348,19 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
   const RowReader<C> rows(lane);
   const ColReader<C> cols(lane);
   const KeyBits<C::KT, NW> keys{mask, reinterpret_cast<uint64_t*>(smem + C::NST * C::STAGE), a.Nk, t0, t1, wave, lane};
-  // of tiles t .. t + NST - 1
-  uint64_t bits[C::NST];
   auto fetch = [&](int t, uint64_t b) {  // past the last tile: nothing is read
     char* stage = smem + (t - t0) % C::NST * C::STAGE;
     kl.load(kb + (int64_t)t * C::KT * a.in.k_n, stage, wave_u, b);
     vl.load(vb + (int64_t)t * C::KT * a.in.v_n, stage + C::TILE, wave_u, b);
   };
-#pragma unroll
-  for (int i = 0; i < C::NST - 1; ++i) {
-    bits[i] = keys.of(t0 + i);
-    fetch(t0 + i, bits[i]);
-  }
+  uint64_t bits = keys.of(t0);
+  fetch(t0, bits);
   for (int t = t0; t < t1; ++t) {
     const uint32_t ks_ = (t - t0) % C::NST * C::STAGE, vs_ = ks_ + C::TILE;
-    tile_ready<2 * TileLoader<C, NW>::N * (C::NST - 2)>();
-    bits[C::NST - 1] = keys.of(t + C::NST - 1);
-    fetch(t + C::NST - 1, bits[C::NST - 1]);
-    if (bits[0]) {
+    tile_ready<0>();
+    const uint64_t bits_next = keys.of(t + 1);
+    fetch(t + 1, bits_next);
+    if (bits) {
       at_f32x16 s[C::NJ];
 #pragma unroll
       for (int j = 0; j < C::NJ; ++j) {
@@ -374,8 +370,8 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
       }
       ColFrags<T, C> vf;  // read while the matrix unit works on the scores
       vf.read(smem, vs_, 0, cols, lane);
-      if (bits[0] != C::kFull) {
-        const uint64_t mine = bits[0] >> (4 * half);
+      if (bits != C::kFull) {
+        const uint64_t mine = bits >> (4 * half);
 #pragma unroll
         for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
@@ -417,8 +413,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
         }
       }
     }
-#pragma unroll
-    for (int i = 0; i < C::NST - 1; ++i) bits[i] = bits[i + 1];
+    bits = bits_next;
   }
   tiles_landed();
   l = halves_sum(l);
@@ -610,23 +605,19 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
   const RowReader<C> rows(lane);
   const ColReader<C> cols(lane);
   const KeyBits<C::KT, NW> keys{mask, reinterpret_cast<uint64_t*>(smem + C::NST * C::STAGE), a.Nk, t0, t1, wave, lane};
-  uint64_t bits[C::NST];
   auto fetch = [&](int t, uint64_t b) {  // past the last tile: nothing is read
     char* stage = smem + (t - t0) % C::NST * C::STAGE;
     kl.load(kb + (int64_t)t * C::KT * a.in.k_n, stage, wave_u, b);
     vl.load(vb + (int64_t)t * C::KT * a.in.v_n, stage + C::TILE, wave_u, b);
   };
-#pragma unroll
-  for (int i = 0; i < C::NST - 1; ++i) {
-    bits[i] = keys.of(t0 + i);
-    fetch(t0 + i, bits[i]);
-  }
+  uint64_t bits = keys.of(t0);
+  fetch(t0, bits);
   for (int t = t0; t < t1; ++t) {
     const uint32_t ks_ = (t - t0) % C::NST * C::STAGE, vs_ = ks_ + C::TILE;
-    tile_ready<2 * TileLoader<C, NW>::N * (C::NST - 2)>();
-    bits[C::NST - 1] = keys.of(t + C::NST - 1);
-    fetch(t + C::NST - 1, bits[C::NST - 1]);
-    if (bits[0]) {
+    tile_ready<0>();
+    const uint64_t bits_next = keys.of(t + 1);
+    fetch(t + 1, bits_next);
+    if (bits) {
 #pragma unroll
       for (int j = 0; j < C::NJ; ++j) {
         at_f32x16 s = acc_zero(), dp = minus_delta;
@@ -639,8 +630,8 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
         kf.read(smem, ks_, j, cols, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -L)) * dp[r];
-        if (bits[0] != C::kFull) {
-          const uint64_t mine = bits[0] >> (4 * half);
+        if (bits != C::kFull) {
+          const uint64_t mine = bits >> (4 * half);
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (!((mine >> (32 * j + (r & 3) + 8 * (r >> 2))) & 1)) s[r] = 0.f;
@@ -653,8 +644,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
         }
       }
     }
-#pragma unroll
-    for (int i = 0; i < C::NST - 1; ++i) bits[i] = bits[i + 1];
+    bits = bits_next;
   }
   tiles_landed();
   if (!row_ok) return;
@@ -831,6 +821,216 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 #endif
 }
 
+// ---------------------------------------------------------------------------------------------------------- whole backward
+// Up to 256 keys of up to 64 columns, bf16: a workgroup of 8 waves holds a head's keys and values, 32 keys a wave, and has all of
+// a query row's scores at hand, so that dq is finished here too: 5 products instead of 7, one exponential instead of two, every
+// operand read once.  ds is exchanged between the waves through LDS as [key][64 rows]; a wave then multiplies one 32 x 32 block of
+// dq^T = k^T ds^T over half of the keys, and the two halves are added in a fixed order.  delta is formed from do and o by the
+// threads that a tile's rows are dealt to, one tile ahead.
+__global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef bf16_t T;
+  using C = AttnCfg<T, 64>;
+  constexpr int NW = 8, KEYS = NW * 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr uint32_t kKeys = 0, kRing = KEYS * 128, kDs = kRing + 2 * C::STAGE, kHalf = kDs + KEYS * 128, kStats = kHalf + 4 * 4096;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, wave_u = __builtin_amdgcn_readfirstlane(wave);
+  int head, blk, split;
+  if (!block_coord(a, head, blk, split)) return;
+  const int b = head / a.Hkv, hk = head % a.Hkv;
+  const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.Nk : nullptr;
+  const int key = wave * 32 + (lane & 31);
+  const bool key_ok = key < a.Nk;
+  const int64_t o_n = (int64_t)a.Hkv * a.G * a.D;
+  const T* qb = static_cast<const T*>(a.q) + b * a.in.q_b + (int64_t)hk * a.G * a.in.q_h;
+  const T* gb = static_cast<const T*>(a.dout) + (int64_t)b * a.Nq * o_n + (int64_t)hk * a.G * a.D;
+  const T* ob = static_cast<const T*>(a.o) + (int64_t)b * a.Nq * o_n + (int64_t)hk * a.G * a.D;
+  const int tq = (a.Nq + C::KT - 1) / C::KT, nt = tq * a.G;
+  const TileLoader<C, NW> ql(a.in.q_n, a.D, wave, lane), gl(o_n, a.D, wave, lane), kl(a.in.k_n, a.D, wave, lane);
+  const RowReader<C> rows(lane);
+  const ColReader<C> cols(lane);
+
+  auto fetch = [&](int t) {  // past the last tile: nothing is read
+    const int g = t < nt ? t / tq : 0, r0 = t < nt ? (t - g * tq) * C::KT : 0, n = t < nt ? a.Nq - r0 : 0;
+    const uint64_t bits = n >= C::KT ? C::kFull : (1ull << n) - 1;
+    char* stage = smem + kRing + (t & 1) * C::STAGE;
+    ql.load(qb + g * a.in.q_h + r0 * a.in.q_n, stage, wave_u, bits);
+    gl.load(gb + (int64_t)g * a.D + r0 * o_n, stage + C::TILE, wave_u, bits);
+  };
+  // thread -> row tid / 8 of a tile, chunk tid % 8 of do and o
+  const uint32_t st_off = (tid & 7) * 8 < a.D ? (uint32_t)(tid >> 3) * ((uint32_t)o_n * 2) + (tid & 7) * 16 : kNowhere;
+  at_u32x4 st_g, st_o;
+  float st_L;
+  auto stats_request = [&](int t) {
+    const int g = t < nt ? t / tq : 0, r0 = t < nt ? (t - g * tq) * C::KT : 0, n = t < nt ? a.Nq - r0 : 0;
+    const bool in = (tid >> 3) < n;
+    const int64_t at = (int64_t)g * a.D + r0 * o_n;
+    const __amdgpu_buffer_rsrc_t rg = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(gb + at), 0, kReach, 0x00020000);
+    const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(ob + at), 0, kReach, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc(a.lse + (int64_t)head * a.rows + (int64_t)r0 * a.G + g, 0, kReach, 0x00020000);
+    st_g = __builtin_amdgcn_raw_buffer_load_b128(rg, in ? st_off : kNowhere, 0, 0);
+    st_o = __builtin_amdgcn_raw_buffer_load_b128(ro, in ? st_off : kNowhere, 0, 0);
+    st_L = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rl, in ? (uint32_t)(tid >> 3) * a.G * 4 : kNowhere, 0, 0));
+  };
+  auto stats_store = [&](int t) {
+    float delta = dot16<T>(__builtin_bit_cast(uint4, st_g), __builtin_bit_cast(uint4, st_o));
+    delta += __shfl_xor(delta, 1, 64);
+    delta += __shfl_xor(delta, 2, 64);
+    delta += __shfl_xor(delta, 4, 64);
+    if ((tid & 7) == 0) *reinterpret_cast<uint4*>(smem + kStats + (t & 1) * 1024 + (tid >> 3) * 16) = row_stats(st_L, delta, a.inv_c);
+  };
+
+  stats_request(0);
+  fetch(0);
+  uint4 kf[C::NKS], vf[C::NKS];
+  {
+    const T* kp = static_cast<const T*>(a.k) + b * a.in.k_b + hk * a.in.k_h + (int64_t)key * a.in.k_n;
+    const T* vp = static_cast<const T*>(a.v) + b * a.in.v_b + hk * a.in.v_h + (int64_t)key * a.in.v_n;
+#pragma unroll
+    for (int ks = 0; ks < C::NKS; ++ks) {
+      const int d = (2 * ks + half) * C::E;
+      kf[ks] = vf[ks] = make_uint4(0, 0, 0, 0);
+      if (key_ok && d < a.D) {
+        kf[ks] = *reinterpret_cast<const uint4*>(kp + d);
+        vf[ks] = *reinterpret_cast<const uint4*>(vp + d);
+      }
+    }
+  }
+  const bool see = key_ok && (!mask || mask[key] != 0);
+  const bool wave_sees = __any(see), wave_full = __all(see);
+  {  // the keys that dq multiplies: 64 of them in a step, a masked one as zeros
+    char* to = smem + kKeys;
+    const T* kb = static_cast<const T*>(a.k) + b * a.in.k_b + hk * a.in.k_h;
+#pragma unroll
+    for (int i = 0; i < KEYS / C::KT; ++i) {
+      const int first = i * C::KT + lane;
+      const uint64_t bits = __ballot(first < a.Nk && (!mask || mask[first] != 0));
+      kl.load(kb + (int64_t)i * C::KT * a.in.k_n, to + i * C::TILE, wave_u, bits);
+    }
+  }
+  if (!wave_sees) {  // its part of ds stays zero
+    for (int i = lane; i < 32 * 8; i += 64) *reinterpret_cast<uint4*>(smem + kDs + wave * 4096 + i * 16) = make_uint4(0, 0, 0, 0);
+  }
+  at_f32x16 dk[2], dv[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) dk[i] = dv[i] = acc_zero();
+  const uint4 one_L = half ? make_uint4(0, 0, 0, 0) : make_uint4(0x3f803f80u, 0x00003f80u, 0, 0);
+  const uint4 one_d = half ? make_uint4(0, 0, 0, 0) : make_uint4(0, 0x3f800000u, 0x3f803f80u, 0);
+  stats_store(0);
+  stats_request(1);
+
+  const int qblk = wave & 1, dblk = (wave >> 1) & 1, upper = wave_u >> 2;  // my block of dq^T, my half of the keys
+  char* ds_at = smem + kDs + key * 128 + half * 8;
+  const int ds_swz = chunk_swizzle(key);
+  char* part = smem + kHalf + (wave & 3) * 4096 + lane * 16;
+  at_f32x16 dq = acc_zero();
+  auto dq_store = [&](int t) {  // tile t: the upper half's part was written before the last barrier
+    const int g = t / tq, row = (t - g * tq) * C::KT + 32 * qblk + (lane & 31);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const at_f32x4 x = *reinterpret_cast<const at_f32x4*>(part + i * 1024);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) dq[4 * i + r] += x[r];
+    }
+    if (row < a.Nq) {
+      T* p = static_cast<T*>(a.dq) + b * a.grad.q_b + (int64_t)row * a.grad.q_n + (hk * a.G + g) * a.grad.q_h;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * dblk + 8 * i + 4 * half;
+        if (d < a.D) store4<T>(p + d, dq[4 * i] * a.scale, dq[4 * i + 1] * a.scale, dq[4 * i + 2] * a.scale, dq[4 * i + 3] * a.scale);
+      }
+    }
+  };
+  for (int t = 0; t < nt; ++t) {
+    const uint32_t qs_ = kRing + (t & 1) * C::STAGE, gs_ = qs_ + C::TILE;
+    const char* st_ = smem + kStats + (t & 1) * 1024;
+    tile_ready<0>();
+    stats_store(t + 1);
+    stats_request(t + 2);
+    fetch(t + 1);
+    if (t > 0 && !upper) dq_store(t - 1);
+    if (wave_sees) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint4 both = lds16(st_ + (32 * j + (lane & 31)) * 16);
+        at_f32x16 s = mma(both, one_L, acc_zero(), T()), dp = mma(both, one_d, acc_zero(), T());
+#pragma unroll
+        for (int ks = 0; ks < C::NKS; ++ks) {
+          s = mma(rows.get(smem, qs_, j, ks), kf[ks], s, T());
+          dp = mma(rows.get(smem, gs_, j, ks), vf[ks], dp, T());
+        }
+        ColFrags<T, C> f;  // of do, read while the matrix unit works
+        f.read(smem, gs_, j, cols, lane);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] = __builtin_amdgcn_exp2f(s[r] * a.c);
+          dp[r] *= s[r];
+        }
+        if (!wave_full) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] = see ? dp[r] : 0.f;
+        }
+        uint4 ds[2];
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          ds[cc] = acc_frag(dp, cc, T());
+          const uint4 p = acc_frag(s, cc, T());
+          // rows 32 j + 8 (2 cc) + 4 half + {0..3}, and 8 on: half a chunk each
+          *reinterpret_cast<at_u32x2*>(ds_at + (((4 * j + 2 * cc) ^ ds_swz) << 4)) = at_u32x2{ds[cc].x, ds[cc].y};
+          *reinterpret_cast<at_u32x2*>(ds_at + (((4 * j + 2 * cc + 1) ^ ds_swz) << 4)) = at_u32x2{ds[cc].z, ds[cc].w};
+#pragma unroll
+          for (int i = 0; i < 2; ++i) dv[i] = mma(f.f[cc * 2 + i], p, dv[i], T());
+        }
+        f.read(smem, qs_, j, cols, lane);
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) dk[i] = mma(f.f[cc * 2 + i], ds[cc], dk[i], T());
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // ds is whole (the tiles on their way stay so)
+    asm volatile("" ::: "memory");
+    dq = acc_zero();
+    const uint32_t ka = lds_offset(smem) + kKeys + upper * (KEYS / 2 * 128) + (cols.base[0] ^ (dblk << 6));
+    const uint32_t da = lds_offset(smem) + kDs + upper * (KEYS / 2 * 128) + (cols.base[0] ^ (qblk << 6));
+#pragma unroll
+    for (int i = 0; i < KEYS / 64; ++i) {
+      uint4 f[4];  // 32 keys: of the keys' block, of ds, twice
+      tr_frags4<128>(ka + i * 4096, da + i * 4096, f);
+      dq = mma(f[0], f[1], dq, T());
+      dq = mma(f[2], f[3], dq, T());
+    }
+    if (upper) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<at_f32x4*>(part + i * 1024) = at_f32x4{dq[4 * i], dq[4 * i + 1], dq[4 * i + 2], dq[4 * i + 3]};
+    }
+  }
+  tile_ready<0>();
+  if (nt > 0 && !upper) dq_store(nt - 1);
+  if (!key_ok) return;
+  T* dkp = static_cast<T*>(a.dk) + b * a.grad.k_b + hk * a.grad.k_h + (int64_t)key * a.grad.k_n;
+  T* dvp = static_cast<T*>(a.dv) + b * a.grad.v_b + hk * a.grad.v_h + (int64_t)key * a.grad.v_n;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const int d = 32 * i + 8 * gq + 4 * half;
+      float x[4], y[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {  // a column's sums are its own: a masked key's are dropped here
+        x[r] = see ? dk[i][4 * gq + r] * a.scale : 0.f;
+        y[r] = see ? dv[i][4 * gq + r] : 0.f;
+      }
+      if (d < a.D) {
+        store4<T>(dkp + d, x[0], x[1], x[2], x[3]);
+        store4<T>(dvp + d, y[0], y[1], y[2], y[3]);
+      }
+    }
+#endif
+}
+constexpr int kWholeLds = 256 * 128 + 2 * AttnCfg<bf16_t, 64>::STAGE + 256 * 128 + 4 * 4096 + 2 * 1024;
+
 // ---------------------------------------------------------------------------------------------------------- host
 namespace {
 
@@ -883,6 +1083,13 @@ AttnPlan dq_plan(const eve_attn_shape& s, int cus) {
 AttnPlan dkv_plan(const eve_attn_shape& s, int cus) {
   const int kt = tile_rows(s);
   return plan_of(s.Nk, 4, (int64_t)s.B * s.Hkv, ((int64_t)s.Nq + kt - 1) / kt * (s.H / s.Hkv), (int64_t)cus * 2, 4);
+}
+
+// The backward of whole heads, a workgroup each: where there is one for every other CU at least and their waves have keys.
+// (64 samples x 12 heads, 237 x 237: 80 us against 100 by the two kernels, which win where heads are few: 2 x 12 heads leave it
+// 24 workgroups.)
+bool whole_heads(const eve_attn_shape& s, int cus) {
+  return s.dtype == EVE_BF16 && s.D <= 64 && s.Nk > 128 && s.Nk <= 256 && (int64_t)s.B * s.Hkv >= cus / 2;
 }
 
 size_t fwd_ws(const eve_attn_shape& s, const AttnPlan& p) {
@@ -988,7 +1195,13 @@ int sum_parts(const AttnArgs& a, const float* part, void* g, int64_t g_b, int64_
 }
 
 template <typename T, int DP>
-int bwd_typed(AttnArgs& a, const AttnPlan& pq, const AttnPlan& pk, hipStream_t st) {
+int bwd_typed(AttnArgs& a, bool whole, const AttnPlan& pq, const AttnPlan& pk, hipStream_t st) {
+  if constexpr (sizeof(T) == 2 && DP == 64) {
+    if (whole) {
+      a.nblk = 1;
+      return launch_attn(attn_bwd_whole_kernel, a, 8, kWholeLds, st, "eve_attn_bwd");
+    }
+  }
   if (a.rows > 0) {
     use_plan(a, pq);
     int rc = launch_attn(pq.nw == 1 ? attn_dq_kernel<T, DP, 1> : attn_dq_kernel<T, DP, 4>, a, pq.nw, attn_lds<T, DP>(), st, "eve_attn_bwd (dq)");
@@ -1060,6 +1273,7 @@ extern "C" int eve_attn_bwd(const eve_attn_shape* s, const eve_attn_layout* in, 
   const void* ptrs[8] = {q, k, v, out, dout, dq, dk, dv};
   for (const void* x : ptrs) EVE_REQUIRE(aligned16(x), EVE_ERR_ARG, "eve_attn_bwd: pointers must be 16-byte aligned");
   const AttnPlan pq = dq_plan(*s, attn_cus()), pk = dkv_plan(*s, attn_cus());
+  const bool whole = whole_heads(*s, attn_cus());
   const BwdWs ws = bwd_ws(*s, pq, pk);
   EVE_REQUIRE(ws.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= ws.bytes), EVE_ERR_WORKSPACE,
               "eve_attn_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, ws.bytes);
@@ -1071,6 +1285,6 @@ extern "C" int eve_attn_bwd(const eve_attn_shape* s, const eve_attn_layout* in, 
   a.part_a = reinterpret_cast<float*>(base + ws.part);
   a.part_b = reinterpret_cast<float*>(base + ws.dv);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (s->dtype == EVE_BF16) return s->D <= 64 ? bwd_typed<bf16_t, 64>(a, pq, pk, st) : bwd_typed<bf16_t, 128>(a, pq, pk, st);
-  return s->D <= 64 ? bwd_typed<float, 64>(a, pq, pk, st) : bwd_typed<float, 128>(a, pq, pk, st);
+  if (s->dtype == EVE_BF16) return s->D <= 64 ? bwd_typed<bf16_t, 64>(a, whole, pq, pk, st) : bwd_typed<bf16_t, 128>(a, false, pq, pk, st);
+  return s->D <= 64 ? bwd_typed<float, 64>(a, false, pq, pk, st) : bwd_typed<float, 128>(a, false, pq, pk, st);
 }

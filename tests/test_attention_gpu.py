@@ -75,6 +75,16 @@ def test_forward_and_gradients(case, dtype):
     assert_within(dict(zip(("out", "dq", "dk", "dv"), (out, *grads))), res, "with gradient")
 
 
+# heads enough, and keys few enough, for the backward that keeps a head in one workgroup
+WHOLE = [(44, 33, 129, 3, 3, 64, "holes"), (33, 237, 237, 4, 4, 64, "tail"), (64, 65, 256, 4, 2, 40, "empty"), (32, 1, 140, 8, 4, 64, "none"),
+         (130, 200, 250, 1, 1, 16, "head"), (43, 64, 160, 6, 3, 8, "one")]
+
+
+@pytest.mark.parametrize("case", WHOLE, ids=lambda c: "x".join(map(str, c)))
+def test_many_heads_of_few_keys(case):
+    test_forward_and_gradients(case, BF16)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_packed_product_and_its_gradient(dtype):
     B, N, H, D = 2, 77, 3, 64
@@ -115,9 +125,9 @@ def test_strides_offsets_and_expanded_inputs(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("Nq", [2, 100])
-def test_what_masked_places_hold_takes_no_part(dtype, Nq):
-    B, Nk, H, D = 3, 150, 2, 64
+@pytest.mark.parametrize("B,Nq", [(3, 2), (3, 100), (65, 100)])
+def test_what_masked_places_hold_takes_no_part(dtype, B, Nq):
+    Nk, H, D = 150, 2, 64
     q, k, v, do = _make(B, Nq, Nk, H, H, D, dtype, 11)
     mask = _mask("empty", B, Nk, 11)
     clean = [t.clone().requires_grad_(True) for t in (q, k, v)]
@@ -230,9 +240,9 @@ def test_other_stream_and_repeated_calls_are_bit_equal():
 
 def test_captured_and_replayed():
     """Forward and backward in a graph, several replays with new inputs, each against the eager result."""
-    for Nq in (1, 90):
-        q, k, v, do = _make(2, Nq, 1500, 4, 2, 64, BF16, 25)
-        mask = _mask("holes", 2, 1500, 25)
+    for B, Nq, Nk in ((2, 1, 1500), (2, 90, 1500), (64, 100, 200)):
+        q, k, v, do = _make(B, Nq, Nk, 4, 2, 64, BF16, 25)
+        mask = _mask("holes", B, Nk, 25)
         parts = [t.clone().requires_grad_(True) for t in (q, k, v)]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
@@ -254,7 +264,7 @@ def test_captured_and_replayed():
             want = (out2, *torch.autograd.grad(out2, eager, do))
             torch.cuda.synchronize()
             for a, b in zip((out, *grads), want):
-                assert torch.equal(a, b), (Nq, i)
+                assert torch.equal(a, b), (B, Nq, i)
 
 
 def test_offsets_beyond_32_bits():
