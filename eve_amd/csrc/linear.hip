@@ -4,11 +4,16 @@
 //   dz = dy row_scale gamma act'(z)   (one pass, with the column sums dbias = sum dz, dgamma = sum dy row_scale u)
 //   dx = dz W,   dW = dz^T x.
 //
-// One tile kernel serves the three products.  An operand is row-major (its contraction index is contiguous in memory: x, W in the
-// forward, dz in dx) or k-major (the contraction index is the row: W in dx, dz and x in dW).  Row-major tiles lie in LDS as
-// [rows][128 bytes] and are read as 16-byte fragments; k-major tiles lie as in memory, [k][columns], and are transposed on the
-// way to the matrix unit (bf16: ds_read_b64_tr_b16).  Chunks of 16 bytes are XOR-swizzled so that either read spreads over the
-// banks.  Any size goes: what lies outside an operand arrives as zeros, rows need no alignment.
+// An operand is row-major (its contraction index is contiguous in memory: x, W in the forward, dz in dx) or k-major (the
+// contraction index is the row: W in dx, dz and x in dW).  Row-major tiles lie in LDS row by row and are read as 16-byte fragments;
+// k-major tiles lie as in memory, [k][columns], and are transposed on the way to the matrix unit (bf16: ds_read_b64_tr_b16).
+// Chunks of 16 bytes are XOR-permuted so that either read spreads over the banks.
+//
+// linear_stream_kernel: rows on 16-byte boundaries.  256 x 128 (or 128 x 128) tiles (or 192 or 128 rows), 4 waves, each 128 x 64 of it, so
+// that six fragments feed eight matrix instructions; steps of 64 bytes of the contraction go from memory to LDS directly, two or
+// three steps ahead, 72 KiB for three stages: two workgroups a CU, one of which computes while the other waits.
+// linear_tile_kernel: any size and alignment, and small problems; tiles of 128 or 64, staged through registers with every element
+// outside an operand replaced by zero.
 // dW has few tiles and a long contraction (the rows of the batch): it is split, with fp32 parts added in order.
 #include "act.h"
 #include "common.h"
@@ -27,7 +32,9 @@ struct LinArgs {
   void* C;                 // [M, N] of the type
   float* part;             // LIN_PART: [nsplit][M][N]
   int M, N, K, lda, ldb;
-  int nsplit, ksteps;      // LIN_PART: splits of the contraction, tile steps of each
+  int nsplit, kspan;       // LIN_PART: splits of the contraction, its length in each
+  float* part_bias;        // dW, may be null: [nsplit][M] column sums of A
+  int ngroup;              // linear_stream_kernel: columns of tiles that are walked before the next row of tiles
   const void *bias, *gamma, *row_scale, *residual;  // LIN_FWD, each may be null
   void* z;                 // LIN_FWD: x W^T + bias, or null
   int rows_per_scale, act;
@@ -178,13 +185,117 @@ template <typename T> __device__ __forceinline__ void unpack16(const uint4& w, f
 }
 #endif  // __HIP_DEVICE_COMPILE__
 
+#if defined(__HIP_DEVICE_COMPILE__)
+// The wave's block of the result, rows from m0 and WN columns from n0 on: 32 rows at a time through the wave's own image in LDS,
+// then 8 columns of a row a lane.  The accumulators are those of the transposed product (B first): a lane holds row lane & 31 and
+// four consecutive columns at a time, one 16-byte store into the image instead of four of 4 bytes.
+// AHEAD (bf16, rows of 16 bytes): the residual of the whole block is requested before the first store, so that its latency is paid
+// once a tile.
+template <typename T, int WN, int NTM, int NTN, int MODE, bool AHEAD = false>
+__device__ __forceinline__ void lin_epilogue(const li_f32x16 (&acc)[NTM][NTN], char* smem, const LinArgs& a, int split, int m0, int n0,
+                                             int wave, int lane) {
+  constexpr int E = LT<T>::E, EP = WN + 4;             // floats of an image row
+  constexpr int CH = WN / 8, RPI = 64 / CH;            // chunks of 8 columns of an image row; rows a pass
+  constexpr int PASS = 32 / RPI;
+  float* img = reinterpret_cast<float*>(smem) + wave * 32 * EP;
+  const int ch = lane % CH, n = n0 + ch * 8, nn = a.N - n;
+  uint4 ahead[AHEAD ? NTM * PASS : 1];
+  if constexpr (AHEAD) {
+    if (a.residual) {
+#pragma unroll
+      for (int i = 0; i < NTM * PASS; ++i) {
+        const int m = m0 + i * RPI + lane / CH;
+        ahead[i] = make_uint4(0, 0, 0, 0);
+        if (m < a.M && nn > 0) ahead[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.residual) + (int64_t)m * a.N + n);
+      }
+    }
+  }
+  float bias[8], gamma[8];
+  if constexpr (MODE == LIN_FWD) {
+    if constexpr (AHEAD) {
+      uint4 b = make_uint4(0, 0, 0, 0), g = make_uint4(0, 0, 0, 0);
+      if (a.bias && nn > 0) b = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.bias) + n);
+      if (a.gamma && nn > 0) g = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.gamma) + n);
+      unpack16<T>(b, bias);
+      unpack16<T>(g, gamma);
+      if (!a.gamma) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) gamma[i] = 1.f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        bias[i] = a.bias && i < nn ? to_f32<T>(static_cast<const T*>(a.bias)[n + i]) : 0.f;
+        gamma[i] = a.gamma && i < nn ? to_f32<T>(static_cast<const T*>(a.gamma)[n + i]) : 1.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NTM; ++i) {
+#pragma unroll
+    for (int j = 0; j < NTN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(img + (lane & 31) * EP + 32 * j + 8 * g + 4 * (lane >> 5)) =
+            make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the image is the wave's own: no barrier, but its lanes exchange through it
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int it = 0; it < PASS; ++it) {
+      const int rr = it * RPI + lane / CH, m = m0 + 32 * i + rr;
+      float v[8];
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(img + rr * EP + ch * 8);
+      *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(img + rr * EP + ch * 8 + 4);
+      if (m < a.M && nn > 0) {
+        const int64_t at = (int64_t)m * a.N + n;
+        if constexpr (MODE == LIN_PART) {
+          float* p = a.part + (int64_t)split * a.M * a.N + at;
+          store_some<float>(p, __builtin_bit_cast(uint4, *reinterpret_cast<float4*>(v)), nn);
+          store_some<float>(p + 4, __builtin_bit_cast(uint4, *reinterpret_cast<float4*>(v + 4)), nn - 4);
+        } else {
+          if constexpr (MODE == LIN_FWD) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += bias[e];
+            if (a.z) {
+#pragma unroll
+              for (int e = 0; e < 8; e += E) store_some<T>(static_cast<T*>(a.z) + at + e, pack16<T>(v + e), nn - e);
+            }
+            if (a.act != EVE_ACT_IDENTITY) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = act_of<T>(v[e], a.act);
+            }
+            if (a.gamma || a.row_scale) {
+              const float rs = a.row_scale ? to_f32<T>(static_cast<const T*>(a.row_scale)[m / a.rows_per_scale]) : 1.f;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] *= gamma[e] * rs;
+            }
+            if (a.residual) {
+#pragma unroll
+              for (int e = 0; e < 8; e += E) {
+                float r[E];
+                unpack16<T>(AHEAD ? ahead[i * PASS + it] : load_some<T>(static_cast<const T*>(a.residual) + at + e, nn - e), r);
+#pragma unroll
+                for (int f = 0; f < E; ++f) v[e + f] += r[f];
+              }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; e += E) store_some<T>(static_cast<T*>(a.C) + at + e, pack16<T>(v + e), nn - e);
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+#endif
+
 // BT x BT tile, 4 waves of (BT/2) x (BT/2); two LDS stages, the next step's tiles in registers meanwhile.
 template <typename T, int BT, bool ACOL, bool BCOL, int MODE>
 __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int BK = LT<T>::BK, E = LT<T>::E, NT = BT / 64, NKS = BK / (2 * E);
   constexpr int STAGE = 2 * BT * 128;
-  constexpr int EP = BT / 2 + 4;  // floats of a row of a wave's epilogue image
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   // Workgroups go round-robin over the 8 XCDs: each of them gets a run of tiles, columns fastest, so that the tiles it works on
@@ -195,8 +306,8 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
   if ((int)(blockIdx.x >> 3) >= per || item >= total) return;
   const int split = item / (tm * tn), tile = item % (tm * tn);
   const int m0 = (tile / tn) * BT, n0 = (tile % tn) * BT;
-  const int k0 = MODE == LIN_PART ? split * a.ksteps * BK : 0;
-  const int k1 = MODE == LIN_PART ? min(a.K, k0 + a.ksteps * BK) : a.K;
+  const int k0 = MODE == LIN_PART ? split * a.kspan : 0;
+  const int k1 = MODE == LIN_PART ? min(a.K, k0 + a.kspan) : a.K;
 
   const T* Ap = static_cast<const T*>(a.A) + (ACOL ? (int64_t)k0 * a.lda + m0 : (int64_t)m0 * a.lda + k0);
   const T* Bp = static_cast<const T*>(a.B) + (BCOL ? (int64_t)k0 * a.ldb + n0 : (int64_t)n0 * a.ldb + k0);
@@ -235,76 +346,242 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = lmma(fa[i], fb[j], acc[i][j], T());
+        for (int j = 0; j < NT; ++j) acc[i][j] = lmma(fb[j], fa[i], acc[i][j], T());
     }
   }
   __syncthreads();  // the stages become the waves' epilogue images
 
-  // 32 rows at a time through the wave's own image, then 8 columns of a row a lane
-  constexpr int CH = BT / 2 / 8, RPI = 64 / CH;  // chunks of 8 columns of an image row; rows a pass
-  float* img = reinterpret_cast<float*>(smem) + wave * 32 * EP;
-  const int ch = lane % CH, n = n0 + wn * (BT / 2) + ch * 8, nn = a.N - n;
-  float bias[8], gamma[8];
-  if constexpr (MODE == LIN_FWD) {
+  lin_epilogue<T, BT / 2, NT, NT, MODE>(acc, smem, a, split, m0 + wm * (BT / 2), n0 + wn * (BT / 2), wave, lane);
+#endif
+}
+
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef uint32_t li_u32x4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t kLinNowhere = 0xfffffff0u, kLinReach = 0x80000000u;  // an offset outside every descriptor, and their extent
+
+// One operand's tile of W rows (columns) by 64 bytes of the contraction.
+template <typename T, bool COL, int W> struct StreamTile {
+  static constexpr int E = LT<T>::E, BK = 4 * E;        // contraction indices of a step
+  static constexpr int BYTES = W * 64, N = BYTES / 1024 / 4;  // a wave's transfers of 1 KiB
+  static constexpr int CPR = COL ? W / E : 4;           // chunks of a row of the tile in LDS
+  static constexpr int RB = CPR * 16;
+  uint32_t off[N];
+  int k_of[N];  // the contraction index (COL: the row; else the chunk's first) a lane's chunk belongs to
+  // permutation of the chunks of a row
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (!COL) return (row >> 2) & 3;              // 16 rows of 64 bytes: one chunk each of every 256 bytes
+    else if constexpr (sizeof(T) == 2) return (row & 3) << 2;  // 4 rows: 64 bytes each of every 256
+    else return ((row >> 2) & 1) << 3;                       // rows 4 apart: 128 bytes each
+  }
+  __device__ __forceinline__ StreamTile(int64_t ld, int ext, int wave, int lane) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      bias[i] = a.bias && i < nn ? to_f32<T>(static_cast<const T*>(a.bias)[n + i]) : 0.f;
-      gamma[i] = a.gamma && i < nn ? to_f32<T>(static_cast<const T*>(a.gamma)[n + i]) : 1.f;
+    for (int i = 0; i < N; ++i) {
+      const int p = (i * 4 + wave) * 64 + lane, row = p / CPR, c = (p % CPR) ^ swizzle(row);
+      k_of[i] = COL ? row : c * E;
+      const bool in = COL ? c * E < ext : row < ext;
+      off[i] = in ? (uint32_t)row * ((uint32_t)ld * sizeof(T)) + c * 16 : kLinNowhere;
     }
   }
+  __device__ __forceinline__ void load(const T* p, char* tile, int wave, int krem) const {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, kLinReach, 0x00020000);
+    auto to_lds = [&](int i, uint32_t o) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(tile + (i * 4 + wave) * 1024), 16, o, 0, 0, 0);
+    };
+    if (krem >= BK) {
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
+      for (int i = 0; i < N; ++i) to_lds(i, off[i]);
+    } else {  // the end of the contraction, or past it: zeros
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+      for (int i = 0; i < N; ++i) to_lds(i, k_of[i] < krem ? off[i] : kLinNowhere);
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t lin_lds(const char* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
+
+// Four transposed fragments, read and waited for in one block (through the builtin the compiler would also wait for the
+// transfers in flight): at p0 + D0, p1 + D1, p2 + D2, p3 + D3, their second halves 4 rows on.
+template <int RB, int D0, int D1, int D2, int D3>
+__device__ __forceinline__ void lin_tr4(uint32_t p0, uint32_t p1, uint32_t p2, uint32_t p3, uint4 (&f)[4]) {
+  li_s16x4 v[8];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %2, %9 offset:%14\n\tds_read_b64_tr_b16 %3, %9 offset:%15\n\t"
+      "ds_read_b64_tr_b16 %4, %10 offset:%16\n\tds_read_b64_tr_b16 %5, %10 offset:%17\n\t"
+      "ds_read_b64_tr_b16 %6, %11 offset:%18\n\tds_read_b64_tr_b16 %7, %11 offset:%19\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(p0), "v"(p1), "v"(p2), "v"(p3), "n"(D0), "n"(D0 + 4 * RB), "n"(D1), "n"(D1 + 4 * RB), "n"(D2), "n"(D2 + 4 * RB), "n"(D3),
+        "n"(D3 + 4 * RB)
+      : "memory");
 #pragma unroll
-      for (int r = 0; r < 16; ++r) img[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * EP + 32 * j + (lane & 31)] = acc[i][j][r];
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the image is the wave's own: no barrier, but its lanes exchange through it
-    __builtin_amdgcn_wave_barrier();
+  for (int i = 0; i < 4; ++i) {
+    const li_s16x8 w = __builtin_shufflevector(v[2 * i], v[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+    f[i] = __builtin_bit_cast(uint4, w);
+  }
+}
+
+// Fragments of NT 32-row (column) blocks from r0 on, for both halves of a step: f[ks][i].
+template <typename T, bool COL, int W, int NT> struct StreamReader {
+  using S = StreamTile<T, COL, W>;
+  uint32_t base;  // block 0, first half
+  __device__ __forceinline__ StreamReader(int r0, int lane) {
+    if constexpr (!COL) {
+      const int row = r0 + (lane & 31);
+      base = row * 64 + (((lane >> 5) ^ S::swizzle(row)) << 4);
+    } else if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, q = i >> 2, p = i & 3, e = r0 + 16 * ((lane >> 4) & 1) + 4 * p;
+      base = (8 * (lane >> 5) + q) * S::RB + (((e >> 3) ^ (q << 2)) << 4) + ((e & 7) << 1);
+    } else {
+      const int col = r0 + (lane & 31);
+      base = 4 * (lane >> 5) * S::RB + ((((col >> 2) ^ ((lane >> 5) << 3)) << 4)) + ((col & 3) << 2);
+    }
+  }
+  __device__ __forceinline__ void read(const char* smem, uint32_t tile, int ks, uint4 (&f)[NT]) const {
+    if constexpr (!COL) {
 #pragma unroll
-    for (int it = 0; it < 32 / RPI; ++it) {
-      const int rr = it * RPI + lane / CH, m = m0 + wm * (BT / 2) + 32 * i + rr;
-      float v[8];
-      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(img + rr * EP + ch * 8);
-      *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(img + rr * EP + ch * 8 + 4);
-      if (m < a.M && nn > 0) {
-        const int64_t at = (int64_t)m * a.N + n;
-        if constexpr (MODE == LIN_PART) {
-          float* p = a.part + (int64_t)split * a.M * a.N + at;
-          store_some<float>(p, __builtin_bit_cast(uint4, *reinterpret_cast<float4*>(v)), nn);
-          store_some<float>(p + 4, __builtin_bit_cast(uint4, *reinterpret_cast<float4*>(v + 4)), nn - 4);
-        } else {
-          if constexpr (MODE == LIN_FWD) {
+      for (int i = 0; i < NT; ++i) {
+        const li_u32x4 w = *reinterpret_cast<const li_u32x4*>(smem + (((tile + base) ^ (ks << 5)) + i * 2048));
+        f[i] = make_uint4(w.x, w.y, w.z, w.w);
+      }
+    } else if constexpr (sizeof(T) == 2) {
+      const uint32_t at = lin_lds(smem) + tile + ks * 16 * S::RB;  // block i: chunk 4 i, permuted by q << 2
+      if constexpr (NT == 4) {
+        lin_tr4<S::RB, 0, 0, 0, 0>(at + base, at + (base ^ 64), at + (base ^ 128), at + (base ^ 192), f);
+      } else {
+        static_assert(NT == 2, "two or four blocks");
+        uint4 g[4];  // (the other two are the second half of the step's, read by both())
+        lin_tr4<S::RB, 0, 0, 16 * S::RB, 16 * S::RB>(at + base, at + (base ^ 64), at + base, at + (base ^ 64), g);
+        f[0] = g[0];
+        f[1] = g[1];
+      }
+    } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += bias[e];
-            if (a.z) {
+      for (int i = 0; i < NT; ++i) {
+        uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < 8; e += E) store_some<T>(static_cast<T*>(a.z) + at + e, pack16<T>(v + e), nn - e);
-            }
-            if (a.act != EVE_ACT_IDENTITY) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = act_of<T>(v[e], a.act);
-            }
-            const float rs = a.row_scale ? to_f32<T>(static_cast<const T*>(a.row_scale)[m / a.rows_per_scale]) : 1.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= gamma[e] * rs;
-            if (a.residual) {
-#pragma unroll
-              for (int e = 0; e < 8; e += E) {
-                float r[E];
-                unpack16<T>(load_some<T>(static_cast<const T*>(a.residual) + at + e, nn - e), r);
-#pragma unroll
-                for (int f = 0; f < E; ++f) v[e + f] += r[f];
-              }
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 8; e += E) store_some<T>(static_cast<T*>(a.C) + at + e, pack16<T>(v + e), nn - e);
-        }
+        for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint32_t*>(smem + (tile + (base ^ (i << 7)) + (ks * 8 + t) * S::RB));  // block i: chunk 8 i, permuted
+        f[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
   }
+  // both halves at once
+  __device__ __forceinline__ void both(const char* smem, uint32_t tile, uint4 (&f)[2][NT]) const {
+    if constexpr (COL && sizeof(T) == 2 && NT == 2) {
+      const uint32_t at = lin_lds(smem) + tile;
+      uint4 g[4];
+      lin_tr4<S::RB, 0, 0, 16 * S::RB, 16 * S::RB>(at + base, at + (base ^ 64), at + base, at + (base ^ 64), g);
+      f[0][0] = g[0];
+      f[0][1] = g[1];
+      f[1][0] = g[2];
+      f[1][1] = g[3];
+    } else {
+      read(smem, tile, 0, f[0]);
+      read(smem, tile, 1, f[1]);
+    }
+  }
+};
+
+template <typename T> __device__ __forceinline__ float frag_sum(const uint4& w, float s) {
+  float v[LT<T>::E];
+  unpack16<T>(w, v);
+#pragma unroll
+  for (int i = 0; i < LT<T>::E; ++i) s += v[i];
+  return s;
+}
+#endif  // __HIP_DEVICE_COMPILE__
+
+constexpr int kStreamN = 128;
+template <int BM> constexpr int stream_stages() { return BM == 192 ? 4 : 3; }
+template <int BM> constexpr int stream_lds() { return stream_stages<BM>() * (BM + kStreamN) * 64; }
+
+template <typename T, int BM, bool ACOL, bool BCOL, int MODE>
+__global__ __launch_bounds__(256, 2) void linear_stream_kernel(LinArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int BN = kStreamN, NTM = BM / 64, NTN = 2, STAGE = (BM + BN) * 64, NST = stream_stages<BM>();
+  static_assert(BM != 192 || !ACOL, "192-row tiles: row-major A");
+  using TA = StreamTile<T, ACOL, BM>;
+  using TB = StreamTile<T, BCOL, BN>;
+  constexpr int BK = TA::BK;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1, wave_u = __builtin_amdgcn_readfirstlane(wave);
+  // Workgroups go round-robin over the 8 XCDs: each of them gets a run of tiles.  A run walks ngroup columns of tiles (their part
+  // of B stays in the XCD's L2) row by row of A.
+  const int tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN, total = tm * tn * a.nsplit;
+  const int per = (total + 7) >> 3;
+  const int item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || item >= total) return;
+  const int split = item / (tm * tn), tile = item % (tm * tn);
+  const int grp = tile / (tm * a.ngroup), in_grp = tile - grp * tm * a.ngroup, width = min(a.ngroup, tn - grp * a.ngroup);
+  const int m0 = in_grp / width * BM, n0 = (grp * a.ngroup + in_grp % width) * BN;
+  const int k0 = MODE == LIN_PART ? split * a.kspan : 0;
+  const int k1 = MODE == LIN_PART ? min(a.K, k0 + a.kspan) : a.K;
+
+  const T* Ap = static_cast<const T*>(a.A) + (ACOL ? (int64_t)k0 * a.lda + m0 : (int64_t)m0 * a.lda + k0);
+  const T* Bp = static_cast<const T*>(a.B) + (BCOL ? (int64_t)k0 * a.ldb + n0 : (int64_t)n0 * a.ldb + k0);
+  const int64_t sa = ACOL ? (int64_t)BK * a.lda : BK, sb = BCOL ? (int64_t)BK * a.ldb : BK;
+  const TA ta(a.lda, a.M - m0, wave, lane);
+  const TB tb(a.ldb, a.N - n0, wave, lane);
+  const StreamReader<T, ACOL, BM, NTM> ra(wm * (BM / 2), lane);
+  const StreamReader<T, BCOL, BN, NTN> rb(wn * (BN / 2), lane);
+
+  li_f32x16 acc[NTM][NTN];
+#pragma unroll
+  for (int i = 0; i < NTM; ++i)
+#pragma unroll
+    for (int j = 0; j < NTN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  float colsum[NTM];
+#pragma unroll
+  for (int i = 0; i < NTM; ++i) colsum[i] = 0.f;
+  const bool sums = ACOL && a.part_bias && n0 == 0 && wn == 0;
+
+  const int steps = (k1 - k0 + BK - 1) / BK;
+  int slot_in = 0;
+  auto fetch = [&](int t) {  // past the last step: zeros, nothing is read
+    char* stage = smem + slot_in * STAGE;
+    slot_in = slot_in == NST - 1 ? 0 : slot_in + 1;
+    const int krem = k1 - k0 - t * BK;
+    ta.load(Ap + t * sa, stage, wave_u, krem);
+    tb.load(Bp + t * sb, stage + BM * 64, wave_u, krem);
+  };
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i) fetch(i);
+  uint32_t at = 0;
+  for (int t = 0; t < steps; ++t) {
+    // this step's transfers have landed (the next ones' may be in flight), and everybody has read what the next fetch overwrites
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * (TA::N + TB::N)) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    fetch(t + NST - 1);
+    uint4 fa[NTM], fb[2][NTN];
+    rb.both(smem, at + BM * 64, fb);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      ra.read(smem, at, ks, fa);
+      if (sums) {
+#pragma unroll
+        for (int i = 0; i < NTM; ++i) colsum[i] = frag_sum<T>(fa[i], colsum[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < NTM; ++i)
+#pragma unroll
+        for (int j = 0; j < NTN; ++j) acc[i][j] = lmma(fb[ks][j], fa[i], acc[i][j], T());
+    }
+    at = at == (NST - 1) * STAGE ? 0 : at + STAGE;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no transfer may meet the images
+  __syncthreads();
+  if (sums) {
+#pragma unroll
+    for (int i = 0; i < NTM; ++i) {
+      const float s = colsum[i] + __shfl_xor(colsum[i], 32, 64);
+      const int m = m0 + wm * (BM / 2) + 32 * i + (lane & 31);
+      if (lane < 32 && m < a.M) a.part_bias[(int64_t)split * a.M + m] = s;
+    }
+  }
+  lin_epilogue<T, BN / 2, NTM, NTN, MODE, MODE == LIN_FWD && sizeof(T) == 2>(acc, smem, a, split, m0 + wm * (BM / 2), n0 + wn * (BN / 2), wave, lane);
 #endif
 }
 
@@ -348,15 +625,14 @@ __global__ __launch_bounds__(256) void linear_few_kernel(LinArgs a) {
 #endif
 }
 
-// dz and the column sums of its terms.  Block: 32 chunks of 8 columns x 8 row lanes, over kDzRows rows; the row lanes are added
+// dz and the column sums of its terms.  Block: 32 chunks of 8 columns x 8 row lanes, over `rows` rows; the row lanes are added
 // in order and each block row leaves one part.
 struct DzArgs {
   const void *dy, *z, *gamma, *row_scale;
   void* dz;                 // may be null (dz = dy)
   float *part_b, *part_g;   // [parts][N], either may be null
-  int M, N, rows_per_scale, act;
+  int M, N, rows_per_scale, act, rows;  // rows: of a block
 };
-constexpr int kDzRows = 128;
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -370,7 +646,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
     gamma[i] = a.gamma && i < nn ? to_f32<T>(static_cast<const T*>(a.gamma)[n + i]) : 1.f;
     sb[i] = sg[i] = 0.f;
   }
-  const int r0 = blockIdx.y * kDzRows, r1 = min(a.M, r0 + kDzRows);
+  const int r0 = blockIdx.y * a.rows, r1 = min(a.M, r0 + a.rows);
   if (nn > 0) {
     for (int m = r0 + ry; m < r1; m += 8) {
       const int64_t at = (int64_t)m * a.N + n;
@@ -415,19 +691,57 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
 #endif
 }
 
-// out[i] = sum over the parts, in order; blockIdx.y picks one of two problems
-struct SumArgs { const float* part[2]; void* out[2]; int64_t n; int parts; };
+// The sums that close a backward, one launch: dW as the sum of its splits (blocks from 0 on, 1024 elements each), and the column
+// sums dbias and dgamma, many parts of few columns (32 columns a block, 8 runs of parts); each in a fixed order.
+struct SumArgs {
+  const float *part_w, *part_c[2];
+  void *dw, *dc[2];  // null: not asked for
+  int64_t n_w;
+  int parts_w, n_c, parts_c, blocks_w, blocks_c;
+};
 template <typename T>
 __global__ __launch_bounds__(256) void linear_sum_kernel(SumArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  const float* p = blockIdx.y ? a.part[1] : a.part[0];
-  T* o = static_cast<T*>(blockIdx.y ? a.out[1] : a.out[0]);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (!o || i >= a.n) return;
+  __shared__ float red[8][32];
+  if ((int)blockIdx.x < a.blocks_w) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (i + 4 <= a.n_w && (a.n_w & 3) == 0) {
+#pragma unroll 4
+      for (int q = 0; q < a.parts_w; ++q) {
+        const float4 x = *reinterpret_cast<const float4*>(a.part_w + q * a.n_w + i);
+        s[0] += x.x;
+        s[1] += x.y;
+        s[2] += x.z;
+        s[3] += x.w;
+      }
+    } else {
+      for (int e = 0; e < 4; ++e)
+        if (i + e < a.n_w)
+          for (int q = 0; q < a.parts_w; ++q) s[e] += a.part_w[q * a.n_w + i + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < a.n_w) static_cast<T*>(a.dw)[i + e] = from_f32<T>(s[e]);
+    return;
+  }
+  const int bid = blockIdx.x - a.blocks_w, which = bid / a.blocks_c;
+  const float* p = which ? a.part_c[1] : a.part_c[0];
+  T* o = static_cast<T*>(which ? a.dc[1] : a.dc[0]);
+  if (!o) return;
+  const int c = threadIdx.x & 31, run = threadIdx.x >> 5, n = bid % a.blocks_c * 32 + c, len = (a.parts_c + 7) / 8;
   float s = 0.f;
+  if (n < a.n_c) {
 #pragma unroll 8
-  for (int q = 0; q < a.parts; ++q) s += p[q * a.n + i];
-  o[i] = from_f32<T>(s);
+    for (int q = run * len; q < min(a.parts_c, (run + 1) * len); ++q) s += p[(int64_t)q * a.n_c + n];
+  }
+  red[run][c] = s;
+  __syncthreads();
+  if (run == 0 && n < a.n_c) {
+#pragma unroll
+    for (int r = 1; r < 8; ++r) s += red[r][c];
+    o[n] = from_f32<T>(s);
+  }
 #endif
 }
 
@@ -457,8 +771,32 @@ int check_dims(int rows, int T, int K, int N, int act, int dtype) {
   return EVE_OK;
 }
 
-int tile_edge(int64_t M, int64_t N, int64_t splits, int cus) {
-  return ((M + 127) / 128) * ((N + 127) / 128) * splits >= cus ? 128 : 64;
+// Which kernel a product runs on: the rows of the streaming kernel's tile, or (negative) the edge of the general one's.
+// The streaming kernel wants 16-byte rows.  Its tile is the one whose fullest CU has the least to do: 15168 x 768 of a 768- or
+// 2304-long contraction is 360 tiles of 256 rows (two on some CUs, one on others), 474 of 192, 714 of 128 (2.8 a CU, but of 15 %
+// more LDS traffic).  Problems of fewer tiles go to the general kernel's 64 x 64 tiles.
+bool rows16(const void* p, int ld, int size) { return ((uintptr_t)p & 15) == 0 && (int64_t)ld * size % 16 == 0 && ld < (1 << 20); }
+int choose_tile(bool aligned, bool acol, int64_t M, int64_t N, int64_t splits, int cus) {
+  const int64_t tn = (N + 127) / 128 * splits;
+  if ((M + 127) / 128 * tn < cus / 2) return -64;
+  if (!aligned) return -128;
+  const struct { int rows, cost; } tiles[3] = {{256, 100}, {192, 74}, {128, 57}};
+  int best = 0;
+  int64_t least = 0;
+  for (const auto& t : tiles) {
+    if (t.rows == 192 && acol) continue;
+    const int64_t n = (M + t.rows - 1) / t.rows * tn, cost = (n + cus - 1) / cus * t.cost;
+    if (!best || cost < least) {
+      best = t.rows;
+      least = cost;
+    }
+  }
+  return best;
+}
+bool product_aligned(const LinArgs& a, bool acol, bool bcol, int size) {
+  // (a k-major operand's chunks run along its rows or columns of the result)
+  return rows16(a.A, a.lda, size) && rows16(a.B, a.ldb, size) && rows16(a.C, a.N, size) && (int64_t)a.K * size % 16 * (acol && bcol ? 0 : 1) == 0 &&
+         (!acol || (int64_t)a.M * size % 16 == 0) && rows16(a.residual, a.N, size) && rows16(a.z, a.N, size) && rows16(a.bias, a.N, size) && rows16(a.gamma, a.N, size);
 }
 
 template <typename T, int BT, bool ACOL, bool BCOL, int MODE>
@@ -470,9 +808,37 @@ int launch_tile(const LinArgs& a, hipStream_t st) {
   EVE_CHECK_LAUNCH("eve_linear (product)");
   return EVE_OK;
 }
+template <typename T, int BM, bool ACOL, bool BCOL, int MODE>
+int launch_stream(LinArgs a, hipStream_t st) {
+  const int tn = ceil_div(a.N, kStreamN);
+  const int64_t total = (int64_t)ceil_div(a.M, BM) * tn * a.nsplit;
+  EVE_REQUIRE(total <= 0x7ffffff0LL, EVE_ERR_UNSUPPORTED, "eve_linear: too many tiles");
+  // half an L2 (2 MiB) of B a group, and groups of equal width
+  const int64_t panel = (int64_t)kStreamN * (MODE == LIN_PART ? a.kspan : a.K) * (int)sizeof(T);
+  int width = (int)((2 << 20) / (panel > 0 ? panel : 1));
+  width = width < 1 ? 1 : width > tn ? tn : width;
+  a.ngroup = ceil_div(tn, ceil_div(tn, width));
+  constexpr int lds = stream_lds<BM>();
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(linear_stream_kernel<T, BM, ACOL, BCOL, MODE>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    EVE_REQUIRE(e == hipSuccess, EVE_ERR_LAUNCH, "eve_linear: %d bytes of LDS: %s", lds, hipGetErrorString(e));
+  }
+  linear_stream_kernel<T, BM, ACOL, BCOL, MODE><<<dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), lds, st>>>(a);
+  EVE_CHECK_LAUNCH("eve_linear (product)");
+  return EVE_OK;
+}
 template <typename T, bool ACOL, bool BCOL, int MODE>
-int product(const LinArgs& a, int edge, hipStream_t st) {
-  return edge == 128 ? launch_tile<T, 128, ACOL, BCOL, MODE>(a, st) : launch_tile<T, 64, ACOL, BCOL, MODE>(a, st);
+int product(const LinArgs& a, int tile, hipStream_t st) {
+  switch (tile) {
+    case 256: return launch_stream<T, 256, ACOL, BCOL, MODE>(a, st);
+    case 192:
+      if constexpr (!ACOL) return launch_stream<T, 192, ACOL, BCOL, MODE>(a, st);
+      [[fallthrough]];
+    case 128: return launch_stream<T, 128, ACOL, BCOL, MODE>(a, st);
+    case -128: return launch_tile<T, 128, ACOL, BCOL, MODE>(a, st);
+    default: return launch_tile<T, 64, ACOL, BCOL, MODE>(a, st);
+  }
 }
 
 template <typename T>
@@ -486,31 +852,31 @@ int fwd_typed(const LinArgs& a, hipStream_t st) {
     EVE_CHECK_LAUNCH("eve_linear_fwd (few rows)");
     return EVE_OK;
   }
-  return product<T, false, false, LIN_FWD>(a, tile_edge(a.M, a.N, 1, lin_cus()), st);
+  return product<T, false, false, LIN_FWD>(a, choose_tile(product_aligned(a, false, false, sizeof(T)), false, a.M, a.N, 1, lin_cus()), st);
 }
 
-struct BwdPlan { int parts, edge_w, nsplit, ksteps; size_t dz, part_b, part_g, part_w, bytes; };
+struct BwdPlan { int dz_rows, parts, nsplit, kspan; size_t dz, part_b, part_g, part_w, part_s, bytes; };
 
 BwdPlan bwd_plan(int rows, int K, int N, int dtype, int cus) {
   BwdPlan p;
   const size_t size = dtype == EVE_BF16 ? 2 : 4;
-  const int bk = dtype == EVE_BF16 ? 64 : 32;
-  p.parts = ceil_div(rows, kDzRows);
-  const int steps = ceil_div(rows, bk);
-  // dW [N, K]: the contraction over the rows is split until there are about two tiles a CU, with at least four steps each
-  const int64_t t128 = (int64_t)ceil_div(N, 128) * ceil_div(K, 128);
-  int64_t want = t128 > 0 ? 2 * (int64_t)cus / t128 : 1;
-  if (want > steps / 4) want = steps / 4;
+  p.dz_rows = 32;  // (128 a block: 29 us for 15168 x 768 of bf16, too few workgroups)
+  while (ceil_div(rows, p.dz_rows) > 32768) p.dz_rows *= 2;
+  p.parts = ceil_div(rows, p.dz_rows);
+  // dW [N, K]: the contraction over the rows is split until there are about two tiles of 256 x 128 a CU, with 256 rows each at least
+  const int64_t tiles = (int64_t)ceil_div(N, 256) * ceil_div(K, 128);
+  int64_t want = tiles > 0 ? 2 * (int64_t)cus / tiles : 1;
+  if (want > rows / 256) want = rows / 256;
   if (want < 1) want = 1;
-  p.edge_w = tile_edge(N, K, want, cus);
-  p.ksteps = (int)((steps + want - 1) / want);
-  if (p.ksteps < 1) p.ksteps = 1;
-  p.nsplit = steps > 0 ? ceil_div(steps, p.ksteps) : 1;
+  p.kspan = (int)align_up((size_t)((rows + want - 1) / want), 64);
+  if (p.kspan < 64) p.kspan = 64;
+  p.nsplit = rows > 0 ? ceil_div(rows, p.kspan) : 1;
   p.dz = 0;
   p.part_b = p.dz + align_up((size_t)rows * N * size, 256);
   p.part_g = p.part_b + align_up((size_t)p.parts * N * 4, 256);
   p.part_w = p.part_g + align_up((size_t)p.parts * N * 4, 256);
-  p.bytes = p.part_w + (p.nsplit > 1 ? align_up((size_t)p.nsplit * N * K * 4, 256) : 0);
+  p.part_s = p.part_w + (p.nsplit > 1 ? align_up((size_t)p.nsplit * N * K * 4, 256) : 0);
+  p.bytes = p.part_s + align_up((size_t)p.nsplit * N * 4, 256);
   return p;
 }
 
@@ -519,36 +885,47 @@ int bwd_typed(const DzArgs& dzin, const void* x, const void* w, void* dx, void* 
               const BwdPlan& p, hipStream_t st) {
   DzArgs d = dzin;
   const int rows = d.M, N = d.N;
+  d.rows = p.dz_rows;
   const bool plain = d.act == EVE_ACT_IDENTITY && !d.gamma && !d.row_scale;  // dz = dy
+  LinArgs w_ = {};
+  w_.A = plain ? d.dy : ws + p.dz; w_.B = x; w_.C = dw; w_.M = N; w_.N = K; w_.K = rows; w_.lda = N; w_.ldb = K;
+  w_.nsplit = p.nsplit; w_.kspan = p.kspan; w_.part = reinterpret_cast<float*>(ws + p.part_w);
+  const int tile_w = choose_tile(product_aligned(w_, true, true, sizeof(T)), true, N, K, p.nsplit, lin_cus());
+  // dz = dy: dbias is summed by the dW product while it has dy in registers, where the streaming kernel runs it
+  const bool with_dw = plain && dbias && dw && !dgamma && tile_w > 0 && rows > 0 && N > 0 && K > 0;
+  if (with_dw) w_.part_bias = reinterpret_cast<float*>(ws + p.part_s);
   d.dz = plain || !(dx || dw) ? nullptr : ws + p.dz;
-  d.part_b = dbias ? reinterpret_cast<float*>(ws + p.part_b) : nullptr;
+  d.part_b = dbias && !with_dw ? reinterpret_cast<float*>(ws + p.part_b) : nullptr;
   d.part_g = dgamma ? reinterpret_cast<float*>(ws + p.part_g) : nullptr;
-  if (N > 0 && rows > 0 && (d.dz || dbias || dgamma)) {
+  if (N > 0 && rows > 0 && (d.dz || d.part_b || d.part_g)) {
     linear_dz_kernel<T><<<dim3(ceil_div(N, 256), p.parts), dim3(256), 0, st>>>(d);
     EVE_CHECK_LAUNCH("eve_linear_bwd (dz)");
-  }
-  if (N > 0 && (dbias || dgamma)) {
-    SumArgs s = {{d.part_b, d.part_g}, {dbias, dgamma}, N, p.parts};
-    linear_sum_kernel<T><<<dim3(ceil_div(N, 256), 2), dim3(256), 0, st>>>(s);
-    EVE_CHECK_LAUNCH("eve_linear_bwd (column sums)");
   }
   const void* dz = plain ? d.dy : d.dz;
   if (dx && rows > 0 && K > 0) {
     LinArgs a = {};
     a.A = dz; a.B = w; a.C = dx; a.M = rows; a.N = K; a.K = N; a.lda = N; a.ldb = K; a.nsplit = 1;
-    const int rc = product<T, false, true, LIN_PLAIN>(a, tile_edge(rows, K, 1, lin_cus()), st);
+    const int rc = product<T, false, true, LIN_PLAIN>(a, choose_tile(product_aligned(a, false, true, sizeof(T)), false, rows, K, 1, lin_cus()), st);
     if (rc != EVE_OK) return rc;
   }
   if (dw && N > 0 && K > 0) {
-    LinArgs a = {};
-    a.A = dz; a.B = x; a.C = dw; a.M = N; a.N = K; a.K = rows; a.lda = N; a.ldb = K;
-    a.nsplit = p.nsplit; a.ksteps = p.ksteps; a.part = reinterpret_cast<float*>(ws + p.part_w);
-    if (p.nsplit == 1) return product<T, true, true, LIN_PLAIN>(a, p.edge_w, st);
-    const int rc = product<T, true, true, LIN_PART>(a, p.edge_w, st);
+    int rc = p.nsplit == 1 ? product<T, true, true, LIN_PLAIN>(w_, tile_w, st) : product<T, true, true, LIN_PART>(w_, tile_w, st);
     if (rc != EVE_OK) return rc;
-    SumArgs s = {{a.part, nullptr}, {dw, nullptr}, (int64_t)N * K, p.nsplit};
-    linear_sum_kernel<T><<<dim3((unsigned)(((int64_t)N * K + 255) / 256)), dim3(256), 0, st>>>(s);
-    EVE_CHECK_LAUNCH("eve_linear_bwd (sum of the splits)");
+  }
+  SumArgs s = {};
+  if (dw && N > 0 && K > 0 && p.nsplit > 1) {
+    s.part_w = w_.part; s.dw = dw; s.n_w = (int64_t)N * K; s.parts_w = p.nsplit;
+    s.blocks_w = (int)((s.n_w + 1023) / 1024);
+  }
+  s.blocks_c = 1;
+  if (N > 0 && (dbias || dgamma)) {
+    s.part_c[0] = with_dw ? w_.part_bias : d.part_b; s.part_c[1] = d.part_g; s.dc[0] = dbias; s.dc[1] = dgamma;
+    s.n_c = N; s.parts_c = with_dw ? p.nsplit : p.parts; s.blocks_c = ceil_div(N, 32);
+  }
+  const int64_t blocks = s.blocks_w + (s.n_c ? 2 * (int64_t)s.blocks_c : 0);
+  if (blocks > 0) {
+    linear_sum_kernel<T><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(s);
+    EVE_CHECK_LAUNCH("eve_linear_bwd (sums)");
   }
   return EVE_OK;
 }
