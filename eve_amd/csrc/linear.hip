@@ -189,45 +189,59 @@ template <typename T> __device__ __forceinline__ void unpack16(const uint4& w, f
 // The wave's block of the result, rows from m0 and WN columns from n0 on: 32 rows at a time through the wave's own image in LDS,
 // then 8 columns of a row a lane.  The accumulators are those of the transposed product (B first): a lane holds row lane & 31 and
 // four consecutive columns at a time, one 16-byte store into the image instead of four of 4 bytes.
-// AHEAD (bf16, rows of 16 bytes): the residual of the whole block is requested before the first store, so that its latency is paid
-// once a tile.
-template <typename T, int WN, int NTM, int NTN, int MODE, bool AHEAD = false>
+//
+// VEC (rows on 16-byte boundaries): all accesses go through buffer descriptors, where a lane outside the result has an offset
+// outside, without a branch.  Behind a branch around a store the compiler cannot count it and waits for its completion before the
+// next value that it has loaded: 2000 cycles a pass, twelve times a tile.  For bf16 the residual and the row factors of the whole
+// block are requested before the first store.
+typedef uint32_t li_u32x4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t kLinNowhere = 0xfffffff0u, kLinReach = 0x80000000u;  // an offset outside every descriptor, and their extent
+template <typename T, int WN, int NTM, int NTN, int MODE, bool VEC>
 __device__ __forceinline__ void lin_epilogue(const li_f32x16 (&acc)[NTM][NTN], char* smem, const LinArgs& a, int split, int m0, int n0,
                                              int wave, int lane) {
   constexpr int E = LT<T>::E, EP = WN + 4;             // floats of an image row
   constexpr int CH = WN / 8, RPI = 64 / CH;            // chunks of 8 columns of an image row; rows a pass
   constexpr int PASS = 32 / RPI;
+  constexpr bool AHEAD = VEC && MODE == LIN_FWD && sizeof(T) == 2;
+  constexpr int OSIZE = MODE == LIN_PART ? 4 : (int)sizeof(T);
   float* img = reinterpret_cast<float*>(smem) + wave * 32 * EP;
   const int ch = lane % CH, n = n0 + ch * 8, nn = a.N - n;
-  uint4 ahead[AHEAD ? NTM * PASS : 1];
+  // VEC: descriptors from the block's first element on, a lane's offset for row r of the block
+  auto rsrc = [&](const void* p, int64_t size) {
+    const uint64_t x = reinterpret_cast<uint64_t>(p) + ((int64_t)m0 * a.N + n0) * size;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), 0, p ? kLinReach : 0u, 0x00020000);
+  };
+  auto offset = [&](int r, int e, int size) {
+    return m0 + r < a.M && e < nn ? ((uint32_t)r * (uint32_t)a.N + ch * 8 + e) * size : kLinNowhere;
+  };
+  __amdgpu_buffer_rsrc_t to, to_z, from;
+  if constexpr (VEC) {
+    to = rsrc(MODE == LIN_PART ? a.part + (int64_t)split * a.M * a.N : a.C, OSIZE);
+    to_z = rsrc(a.z, sizeof(T));
+    from = rsrc(a.residual, sizeof(T));
+  }
+  li_u32x4 res[AHEAD ? NTM * PASS : 1];
+  float rs[AHEAD ? NTM * PASS : 1];
   if constexpr (AHEAD) {
-    if (a.residual) {
 #pragma unroll
-      for (int i = 0; i < NTM * PASS; ++i) {
-        const int m = m0 + i * RPI + lane / CH;
-        ahead[i] = make_uint4(0, 0, 0, 0);
-        if (m < a.M && nn > 0) ahead[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.residual) + (int64_t)m * a.N + n);
-      }
+    for (int i = 0; i < NTM * PASS; ++i) {
+      const int r = i * RPI + lane / CH;
+      res[i] = __builtin_amdgcn_raw_buffer_load_b128(from, offset(r, 0, sizeof(T)), 0, 0);
+      rs[i] = 1.f;
+    }
+    if (a.row_scale) {
+#pragma unroll
+      for (int i = 0; i < NTM * PASS; ++i)
+        rs[i] = to_f32<T>(static_cast<const T*>(a.row_scale)[min(m0 + i * RPI + lane / CH, a.M - 1) / a.rows_per_scale]);
     }
   }
   float bias[8], gamma[8];
   if constexpr (MODE == LIN_FWD) {
-    if constexpr (AHEAD) {
-      uint4 b = make_uint4(0, 0, 0, 0), g = make_uint4(0, 0, 0, 0);
-      if (a.bias && nn > 0) b = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.bias) + n);
-      if (a.gamma && nn > 0) g = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.gamma) + n);
-      unpack16<T>(b, bias);
-      unpack16<T>(g, gamma);
-      if (!a.gamma) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) gamma[i] = 1.f;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        bias[i] = a.bias && i < nn ? to_f32<T>(static_cast<const T*>(a.bias)[n + i]) : 0.f;
-        gamma[i] = a.gamma && i < nn ? to_f32<T>(static_cast<const T*>(a.gamma)[n + i]) : 1.f;
-      }
+    for (int i = 0; i < 8; ++i) {
+      bias[i] = a.bias && i < nn ? to_f32<T>(static_cast<const T*>(a.bias)[n + i]) : 0.f;
+      gamma[i] = a.gamma && i < nn ? to_f32<T>(static_cast<const T*>(a.gamma)[n + i]) : 1.f;
     }
   }
 #pragma unroll
@@ -242,46 +256,65 @@ __device__ __forceinline__ void lin_epilogue(const li_f32x16 (&acc)[NTM][NTN], c
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int it = 0; it < PASS; ++it) {
-      const int rr = it * RPI + lane / CH, m = m0 + 32 * i + rr;
+      const int rr = it * RPI + lane / CH, r = 32 * i + rr, m = m0 + r;
       float v[8];
       *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(img + rr * EP + ch * 8);
       *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(img + rr * EP + ch * 8 + 4);
-      if (m < a.M && nn > 0) {
-        const int64_t at = (int64_t)m * a.N + n;
-        if constexpr (MODE == LIN_PART) {
-          float* p = a.part + (int64_t)split * a.M * a.N + at;
-          store_some<float>(p, __builtin_bit_cast(uint4, *reinterpret_cast<float4*>(v)), nn);
-          store_some<float>(p + 4, __builtin_bit_cast(uint4, *reinterpret_cast<float4*>(v + 4)), nn - 4);
-        } else {
-          if constexpr (MODE == LIN_FWD) {
+      const int64_t at = (int64_t)m * a.N + n;
+      const bool in = m < a.M && nn > 0;
+      auto put = [&](const __amdgpu_buffer_rsrc_t& d, void* p, int e, const uint4& w) {  // 16 bytes from column e of the eight on
+        if constexpr (VEC) __builtin_amdgcn_raw_buffer_store_b128(li_u32x4{w.x, w.y, w.z, w.w}, d, offset(r, e, OSIZE), 0, 0);
+        else if (in) store_some<T>(static_cast<T*>(p) + at + e, w, nn - e);
+      };
+      if constexpr (MODE == LIN_PART) {
+        float* p = a.part + (int64_t)split * a.M * a.N + at;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += bias[e];
-            if (a.z) {
+        for (int e = 0; e < 8; e += 4) {
+          const uint4 w = __builtin_bit_cast(uint4, *reinterpret_cast<float4*>(v + e));
+          if constexpr (VEC) put(to, nullptr, e, w);
+          else if (in) store_some<float>(p + e, w, nn - e);
+        }
+      } else {
+        if constexpr (MODE == LIN_FWD) {
 #pragma unroll
-              for (int e = 0; e < 8; e += E) store_some<T>(static_cast<T*>(a.z) + at + e, pack16<T>(v + e), nn - e);
-            }
-            if (a.act != EVE_ACT_IDENTITY) {
+          for (int e = 0; e < 8; ++e) v[e] += bias[e];
+          if (a.z) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = act_of<T>(v[e], a.act);
-            }
-            if (a.gamma || a.row_scale) {
-              const float rs = a.row_scale ? to_f32<T>(static_cast<const T*>(a.row_scale)[m / a.rows_per_scale]) : 1.f;
+            for (int e = 0; e < 8; e += E) put(to_z, a.z, e, pack16<T>(v + e));
+          }
+          if (a.act != EVE_ACT_IDENTITY) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] *= gamma[e] * rs;
-            }
-            if (a.residual) {
+            for (int e = 0; e < 8; ++e) v[e] = act_of<T>(v[e], a.act);
+          }
+          if (a.gamma || a.row_scale) {
+            float f = 1.f;
+            if constexpr (AHEAD) f = rs[i * PASS + it];
+            else if (a.row_scale && in) f = to_f32<T>(static_cast<const T*>(a.row_scale)[m / a.rows_per_scale]);
 #pragma unroll
-              for (int e = 0; e < 8; e += E) {
-                float r[E];
-                unpack16<T>(AHEAD ? ahead[i * PASS + it] : load_some<T>(static_cast<const T*>(a.residual) + at + e, nn - e), r);
+            for (int e = 0; e < 8; ++e) v[e] *= gamma[e] * f;
+          }
+          if (a.residual) {
 #pragma unroll
-                for (int f = 0; f < E; ++f) v[e + f] += r[f];
+            for (int e = 0; e < 8; e += E) {
+              uint4 w = make_uint4(0, 0, 0, 0);
+              if constexpr (AHEAD) {
+                const li_u32x4 x = res[i * PASS + it];
+                w = make_uint4(x.x, x.y, x.z, x.w);
+              } else if constexpr (VEC) {
+                const li_u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(from, offset(r, e, sizeof(T)), 0, 0);
+                w = make_uint4(x.x, x.y, x.z, x.w);
+              } else if (in) {
+                w = load_some<T>(static_cast<const T*>(a.residual) + at + e, nn - e);
               }
+              float x[E];
+              unpack16<T>(w, x);
+#pragma unroll
+              for (int f = 0; f < E; ++f) v[e + f] += x[f];
             }
           }
-#pragma unroll
-          for (int e = 0; e < 8; e += E) store_some<T>(static_cast<T*>(a.C) + at + e, pack16<T>(v + e), nn - e);
         }
+#pragma unroll
+        for (int e = 0; e < 8; e += E) put(to, a.C, e, pack16<T>(v + e));
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -351,14 +384,11 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
   }
   __syncthreads();  // the stages become the waves' epilogue images
 
-  lin_epilogue<T, BT / 2, NT, NT, MODE>(acc, smem, a, split, m0 + wm * (BT / 2), n0 + wn * (BT / 2), wave, lane);
+  lin_epilogue<T, BT / 2, NT, NT, MODE, false>(acc, smem, a, split, m0 + wm * (BT / 2), n0 + wn * (BT / 2), wave, lane);
 #endif
 }
 
 #if defined(__HIP_DEVICE_COMPILE__)
-typedef uint32_t li_u32x4 __attribute__((ext_vector_type(4)));
-constexpr uint32_t kLinNowhere = 0xfffffff0u, kLinReach = 0x80000000u;  // an offset outside every descriptor, and their extent
-
 // One operand's tile of W rows (columns) by 64 bytes of the contraction.
 template <typename T, bool COL, int W> struct StreamTile {
   static constexpr int E = LT<T>::E, BK = 4 * E;        // contraction indices of a step
@@ -382,18 +412,10 @@ template <typename T, bool COL, int W> struct StreamTile {
       off[i] = in ? (uint32_t)row * ((uint32_t)ld * sizeof(T)) + c * 16 : kLinNowhere;
     }
   }
-  __device__ __forceinline__ void load(const T* p, char* tile, int wave, int krem) const {
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, kLinReach, 0x00020000);
-    auto to_lds = [&](int i, uint32_t o) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(tile + (i * 4 + wave) * 1024), 16, o, 0, 0, 0);
-    };
-    if (krem >= BK) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) to_lds(i, off[i]);
-    } else {  // the end of the contraction, or past it: zeros
-#pragma unroll
-      for (int i = 0; i < N; ++i) to_lds(i, k_of[i] < krem ? off[i] : kLinNowhere);
-    }
+  // the wave's transfer i; from the end of the contraction on (krem indices left) zeros
+  __device__ __forceinline__ void piece(int i, __amdgpu_buffer_rsrc_t r, char* tile, int wave, int krem) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(tile + (i * 4 + wave) * 1024), 16,
+                                             k_of[i] < krem ? off[i] : kLinNowhere, 0, 0, 0);
   }
 };
 
@@ -538,37 +560,62 @@ __global__ __launch_bounds__(256, 2) void linear_stream_kernel(LinArgs a) {
   const bool sums = ACOL && a.part_bias && n0 == 0 && wn == 0;
 
   const int steps = (k1 - k0 + BK - 1) / BK;
-  int slot_in = 0;
-  auto fetch = [&](int t) {  // past the last step: zeros, nothing is read
-    char* stage = smem + slot_in * STAGE;
-    slot_in = slot_in == NST - 1 ? 0 : slot_in + 1;
-    const int krem = k1 - k0 - t * BK;
-    ta.load(Ap + t * sa, stage, wave_u, krem);
-    tb.load(Bp + t * sb, stage + BM * 64, wave_u, krem);
+  constexpr int NP = TA::N + TB::N;  // a wave's transfers of a step
+  __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b;
+  char* into = smem;
+  int krem;
+  auto fetch_begin = [&](int t) {
+    rsrc_a = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(Ap + t * sa), 0, kLinReach, 0x00020000);
+    rsrc_b = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(Bp + t * sb), 0, kLinReach, 0x00020000);
+    krem = k1 - k0 - t * BK;  // past the last step: zeros, nothing is read
   };
+  auto fetch_piece = [&](int i) {
+    if (i < TA::N) ta.piece(i, rsrc_a, into, wave_u, krem);
+    else tb.piece(i - TA::N, rsrc_b, into + BM * 64, wave_u, krem);
+  };
+  auto fetch_end = [&]() { into = into == smem + (NST - 1) * STAGE ? smem : into + STAGE; };
 #pragma unroll
-  for (int i = 0; i < NST - 1; ++i) fetch(i);
+  for (int i = 0; i < NST - 1; ++i) {
+    fetch_begin(i);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) fetch_piece(j);
+    fetch_end();
+  }
   uint32_t at = 0;
   for (int t = 0; t < steps; ++t) {
     // this step's transfers have landed (the next ones' may be in flight), and everybody has read what the next fetch overwrites
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * (TA::N + TB::N)) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * NP) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    fetch(t + NST - 1);
-    uint4 fa[NTM], fb[2][NTN];
+    fetch_begin(t + NST - 1);
+    uint4 fa[2][NTM], fb[2][NTN];
     rb.both(smem, at + BM * 64, fb);
+    ra.read(smem, at, 0, fa[0]);
+    if constexpr (!ACOL) ra.read(smem, at, 1, fa[1]);
+    // The transfers are issued between the matrix instructions: the CU takes one in 16 cycles or more, and a wave that issues them in
+    // a row waits there (400 of a step's 1350 cycles) with nothing for the matrix unit to do.
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      ra.read(smem, at, ks, fa);
+      if constexpr (ACOL)
+        if (ks) ra.read(smem, at, 1, fa[1]);
       if (sums) {
 #pragma unroll
-        for (int i = 0; i < NTM; ++i) colsum[i] = frag_sum<T>(fa[i], colsum[i]);
+        for (int i = 0; i < NTM; ++i) colsum[i] = frag_sum<T>(fa[ks][i], colsum[i]);
       }
 #pragma unroll
-      for (int i = 0; i < NTM; ++i)
+      for (int i = 0; i < NTM; ++i) {
 #pragma unroll
-        for (int j = 0; j < NTN; ++j) acc[i][j] = lmma(fb[ks][j], fa[i], acc[i][j], T());
+        for (int j = 0; j < NTN; ++j) acc[i][j] = lmma(fb[ks][j], fa[ks][i], acc[i][j], T());
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int SLOTS = 2 * NTM;
+        const int slot = ks * NTM + i;
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+          if (q * SLOTS / NP == slot) fetch_piece(q);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
+    fetch_end();
     at = at == (NST - 1) * STAGE ? 0 : at + STAGE;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no transfer may meet the images
@@ -581,7 +628,7 @@ __global__ __launch_bounds__(256, 2) void linear_stream_kernel(LinArgs a) {
       if (lane < 32 && m < a.M) a.part_bias[(int64_t)split * a.M + m] = s;
     }
   }
-  lin_epilogue<T, BN / 2, NTM, NTN, MODE, MODE == LIN_FWD && sizeof(T) == 2>(acc, smem, a, split, m0 + wm * (BM / 2), n0 + wn * (BN / 2), wave, lane);
+  lin_epilogue<T, BN / 2, NTM, NTN, MODE, true>(acc, smem, a, split, m0 + wm * (BM / 2), n0 + wn * (BN / 2), wave, lane);
 #endif
 }
 
