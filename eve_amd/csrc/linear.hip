@@ -9,9 +9,10 @@
 // k-major tiles lie as in memory, [k][columns], and are transposed on the way to the matrix unit (bf16: ds_read_b64_tr_b16).
 // Chunks of 16 bytes are XOR-permuted so that either read spreads over the banks.
 //
-// linear_stream_kernel: rows on 16-byte boundaries.  256 x 128 (or 128 x 128) tiles (or 192 or 128 rows), 4 waves, each 128 x 64 of it, so
-// that six fragments feed eight matrix instructions; steps of 64 bytes of the contraction go from memory to LDS directly, two or
-// three steps ahead, 72 KiB for three stages: two workgroups a CU, one of which computes while the other waits.
+// linear_stream_kernel: rows on 16-byte boundaries.  Tiles of 192 x 128 (256 x 128 of a k-major A, 128 x 128 of smaller problems),
+// 4 waves, each half the rows and half the columns, so that five fragments feed six matrix instructions; steps of 64 bytes of the
+// contraction go from memory to LDS directly, two or three steps ahead: two workgroups a CU, one of which computes while the other
+// waits.
 // linear_tile_kernel: any size and alignment, and small problems; tiles of 128 or 64, staged through registers with every element
 // outside an operand replaced by zero.
 // dW has few tiles and a long contraction (the rows of the batch): it is split, with fp32 parts added in order.
@@ -26,6 +27,7 @@ typedef __attribute__((ext_vector_type(8))) short li_s16x8;
 typedef __attribute__((ext_vector_type(16))) float li_f32x16;
 
 enum { LIN_FWD = 0, LIN_PLAIN = 1, LIN_PART = 2 };
+constexpr int kActRuntime = -1;  // the activation is LinArgs::act
 
 struct LinArgs {
   const void *A, *B;       // operands; rows of the result come from A, columns from B
@@ -196,7 +198,7 @@ template <typename T> __device__ __forceinline__ void unpack16(const uint4& w, f
 // block are requested before the first store.
 typedef uint32_t li_u32x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kLinNowhere = 0xfffffff0u, kLinReach = 0x80000000u;  // an offset outside every descriptor, and their extent
-template <typename T, int WN, int NTM, int NTN, int MODE, bool VEC>
+template <typename T, int WN, int NTM, int NTN, int MODE, int ACT, bool VEC>
 __device__ __forceinline__ void lin_epilogue(const li_f32x16 (&acc)[NTM][NTN], char* smem, const LinArgs& a, int split, int m0, int n0,
                                              int wave, int lane) {
   constexpr int E = LT<T>::E, EP = WN + 4;             // floats of an image row
@@ -239,9 +241,26 @@ __device__ __forceinline__ void lin_epilogue(const li_f32x16 (&acc)[NTM][NTN], c
   float bias[8], gamma[8];
   if constexpr (MODE == LIN_FWD) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      bias[i] = a.bias && i < nn ? to_f32<T>(static_cast<const T*>(a.bias)[n + i]) : 0.f;
-      gamma[i] = a.gamma && i < nn ? to_f32<T>(static_cast<const T*>(a.gamma)[n + i]) : 1.f;
+    for (int e = 0; e < 8; e += E) {
+      uint4 b = make_uint4(0, 0, 0, 0), g = make_uint4(0, 0, 0, 0);
+      if constexpr (VEC) {
+        const uint32_t o = e < nn ? (uint32_t)(n + e) * (uint32_t)sizeof(T) : kLinNowhere;
+        const li_u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.bias), 0, a.bias ? kLinReach : 0u, 0x00020000), o, 0, 0);
+        const li_u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.gamma), 0, a.gamma ? kLinReach : 0u, 0x00020000), o, 0, 0);
+        b = make_uint4(x.x, x.y, x.z, x.w);
+        g = make_uint4(y.x, y.y, y.z, y.w);
+      } else {
+        if (a.bias) b = load_some<T>(static_cast<const T*>(a.bias) + n + e, nn - e);
+        if (a.gamma) g = load_some<T>(static_cast<const T*>(a.gamma) + n + e, nn - e);
+      }
+      unpack16<T>(b, bias + e);
+      unpack16<T>(g, gamma + e);
+    }
+    if (!a.gamma) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) gamma[e] = 1.f;
     }
   }
 #pragma unroll
@@ -282,9 +301,14 @@ __device__ __forceinline__ void lin_epilogue(const li_f32x16 (&acc)[NTM][NTN], c
 #pragma unroll
             for (int e = 0; e < 8; e += E) put(to_z, a.z, e, pack16<T>(v + e));
           }
-          if (a.act != EVE_ACT_IDENTITY) {
+          if constexpr (ACT == kActRuntime) {
+            if (a.act != EVE_ACT_IDENTITY) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = act_of<T>(v[e], a.act);
+              for (int e = 0; e < 8; ++e) v[e] = act_of<T>(v[e], a.act);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = act_fwd<ACT, sizeof(T) == 2>(v[e]);
           }
           if (a.gamma || a.row_scale) {
             float f = 1.f;
@@ -384,7 +408,7 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
   }
   __syncthreads();  // the stages become the waves' epilogue images
 
-  lin_epilogue<T, BT / 2, NT, NT, MODE, false>(acc, smem, a, split, m0 + wm * (BT / 2), n0 + wn * (BT / 2), wave, lane);
+  lin_epilogue<T, BT / 2, NT, NT, MODE, kActRuntime, false>(acc, smem, a, split, m0 + wm * (BT / 2), n0 + wn * (BT / 2), wave, lane);
 #endif
 }
 
@@ -517,7 +541,8 @@ constexpr int kStreamN = 128;
 template <int BM> constexpr int stream_stages() { return BM == 192 ? 4 : 3; }
 template <int BM> constexpr int stream_lds() { return stream_stages<BM>() * (BM + kStreamN) * 64; }
 
-template <typename T, int BM, bool ACOL, bool BCOL, int MODE>
+// (The activation is a parameter of the kernel: with all of them in it, twelve times over, its code does not fit the instruction cache.)
+template <typename T, int BM, bool ACOL, bool BCOL, int MODE, int ACT>
 __global__ __launch_bounds__(256, 2) void linear_stream_kernel(LinArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int BN = kStreamN, NTM = BM / 64, NTN = 2, STAGE = (BM + BN) * 64, NST = stream_stages<BM>();
@@ -628,7 +653,7 @@ __global__ __launch_bounds__(256, 2) void linear_stream_kernel(LinArgs a) {
       if (lane < 32 && m < a.M) a.part_bias[(int64_t)split * a.M + m] = s;
     }
   }
-  lin_epilogue<T, BN / 2, NTM, NTN, MODE, true>(acc, smem, a, split, m0 + wm * (BM / 2), n0 + wn * (BN / 2), wave, lane);
+  lin_epilogue<T, BN / 2, NTM, NTN, MODE, ACT, true>(acc, smem, a, split, m0 + wm * (BM / 2), n0 + wn * (BN / 2), wave, lane);
 #endif
 }
 
@@ -819,26 +844,17 @@ int check_dims(int rows, int T, int K, int N, int act, int dtype) {
 }
 
 // Which kernel a product runs on: the rows of the streaming kernel's tile, or (negative) the edge of the general one's.
-// The streaming kernel wants 16-byte rows.  Its tile is the one whose fullest CU has the least to do: 15168 x 768 of a 768- or
-// 2304-long contraction is 360 tiles of 256 rows (two on some CUs, one on others), 474 of 192, 714 of 128 (2.8 a CU, but of 15 %
-// more LDS traffic).  Problems of fewer tiles go to the general kernel's 64 x 64 tiles.
+// The streaming kernel wants 16-byte rows.  Its tile -- 192 rows (256 of a k-major A) or 128, which has 15 % more LDS traffic a row --
+// is the one whose fullest CU has less to do: 15168 x 768 is 474 tiles of 192 rows (64 us for a contraction of 2304), 714 of 128
+// (70 us), 360 of 256 (74 us: two on some CUs, one on others).  Problems of fewer tiles go to the general kernel's 64 x 64 tiles.
 bool rows16(const void* p, int ld, int size) { return ((uintptr_t)p & 15) == 0 && (int64_t)ld * size % 16 == 0 && ld < (1 << 20); }
 int choose_tile(bool aligned, bool acol, int64_t M, int64_t N, int64_t splits, int cus) {
   const int64_t tn = (N + 127) / 128 * splits;
   if ((M + 127) / 128 * tn < cus / 2) return -64;
   if (!aligned) return -128;
-  const struct { int rows, cost; } tiles[3] = {{256, 100}, {192, 74}, {128, 57}};
-  int best = 0;
-  int64_t least = 0;
-  for (const auto& t : tiles) {
-    if (t.rows == 192 && acol) continue;
-    const int64_t n = (M + t.rows - 1) / t.rows * tn, cost = (n + cus - 1) / cus * t.cost;
-    if (!best || cost < least) {
-      best = t.rows;
-      least = cost;
-    }
-  }
-  return best;
+  const int large = acol ? 256 : 192;
+  const int64_t n_large = (M + large - 1) / large * tn, n_small = (M + 127) / 128 * tn;
+  return (n_large + cus - 1) / cus * large * 100 <= (n_small + cus - 1) / cus * 128 * 115 ? large : 128;
 }
 bool product_aligned(const LinArgs& a, bool acol, bool bcol, int size) {
   // (a k-major operand's chunks run along its rows or columns of the result)
@@ -855,7 +871,7 @@ int launch_tile(const LinArgs& a, hipStream_t st) {
   EVE_CHECK_LAUNCH("eve_linear (product)");
   return EVE_OK;
 }
-template <typename T, int BM, bool ACOL, bool BCOL, int MODE>
+template <typename T, int BM, bool ACOL, bool BCOL, int MODE, int ACT = EVE_ACT_IDENTITY>
 int launch_stream(LinArgs a, hipStream_t st) {
   const int tn = ceil_div(a.N, kStreamN);
   const int64_t total = (int64_t)ceil_div(a.M, BM) * tn * a.nsplit;
@@ -867,22 +883,32 @@ int launch_stream(LinArgs a, hipStream_t st) {
   a.ngroup = ceil_div(tn, ceil_div(tn, width));
   constexpr int lds = stream_lds<BM>();
   if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(linear_stream_kernel<T, BM, ACOL, BCOL, MODE>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(linear_stream_kernel<T, BM, ACOL, BCOL, MODE, ACT>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     EVE_REQUIRE(e == hipSuccess, EVE_ERR_LAUNCH, "eve_linear: %d bytes of LDS: %s", lds, hipGetErrorString(e));
   }
-  linear_stream_kernel<T, BM, ACOL, BCOL, MODE><<<dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), lds, st>>>(a);
+  linear_stream_kernel<T, BM, ACOL, BCOL, MODE, ACT><<<dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), lds, st>>>(a);
   EVE_CHECK_LAUNCH("eve_linear (product)");
   return EVE_OK;
 }
+template <typename T, int BM, bool ACOL, bool BCOL, int MODE>
+int launch_stream_act(const LinArgs& a, hipStream_t st) {
+  if constexpr (MODE == LIN_FWD) {
+    switch (a.act) {
+      case EVE_ACT_QUICK_GELU: return launch_stream<T, BM, ACOL, BCOL, MODE, EVE_ACT_QUICK_GELU>(a, st);
+      case EVE_ACT_GELU: return launch_stream<T, BM, ACOL, BCOL, MODE, EVE_ACT_GELU>(a, st);
+      case EVE_ACT_RELU: return launch_stream<T, BM, ACOL, BCOL, MODE, EVE_ACT_RELU>(a, st);
+      default: break;
+    }
+  }
+  return launch_stream<T, BM, ACOL, BCOL, MODE>(a, st);
+}
 template <typename T, bool ACOL, bool BCOL, int MODE>
 int product(const LinArgs& a, int tile, hipStream_t st) {
+  constexpr int LARGE = ACOL ? 256 : 192;
   switch (tile) {
-    case 256: return launch_stream<T, 256, ACOL, BCOL, MODE>(a, st);
-    case 192:
-      if constexpr (!ACOL) return launch_stream<T, 192, ACOL, BCOL, MODE>(a, st);
-      [[fallthrough]];
-    case 128: return launch_stream<T, 128, ACOL, BCOL, MODE>(a, st);
+    case LARGE: return launch_stream_act<T, LARGE, ACOL, BCOL, MODE>(a, st);
+    case 128: return launch_stream_act<T, 128, ACOL, BCOL, MODE>(a, st);
     case -128: return launch_tile<T, 128, ACOL, BCOL, MODE>(a, st);
     default: return launch_tile<T, 64, ACOL, BCOL, MODE>(a, st);
   }
