@@ -68,14 +68,20 @@ class _AttentionFn(torch.autograd.Function):
         return dq, dk, dv, None, None
 
 
+def _readable_parts(qkv):
+    parts = qkv.unbind(2)
+    if any(ops.attn_readable(t) is not t for t in parts):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+        parts = qkv.unbind(2)
+    return qkv, parts
+
+
 class _SelfAttentionFn(torch.autograd.Function):
     """The three parts of one [B, N, 3, H, D] product, read where they lie; their gradient in one tensor of that shape."""
 
     @staticmethod
     def forward(ctx, qkv, key_mask, scale):  # type: ignore[override]
-        if qkv.numel() and (qkv.stride(4) != 1 or any(ops.attn_readable(t) is not t for t in qkv.unbind(2))):
-            qkv = qkv.contiguous() if not qkv.is_contiguous() else qkv.clone()
-        q, k, v = qkv.unbind(2)
+        qkv, (q, k, v) = _readable_parts(qkv)
         need = ctx.needs_input_grad[0]
         out, lse = ops.attn_fwd(q, k, v, key_mask, scale, want_lse=need)
         if need:
@@ -101,7 +107,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor] = None
     -> [B, Nq, H, D].  A sample without a visible key gives zeros and passes no gradient; masked keys and values may hold
     anything, NaN included.  Scores and sums are float32; results do not depend on the order of execution."""
     key_mask, scale = _check(q, k, v, key_mask, scale)
-    return _AttentionFn.apply(q, k, v, key_mask, scale)
+    if ops._tracks(q, k, v):
+        return _AttentionFn.apply(q, k, v, key_mask, scale)
+    return ops.attn_fwd(ops.attn_readable(q), ops.attn_readable(k), ops.attn_readable(v), key_mask, scale, want_lse=False)[0]
 
 
 def self_attention(qkv: Tensor, key_mask: Optional[Tensor] = None, scale: Optional[float] = None) -> Tensor:
@@ -109,4 +117,6 @@ def self_attention(qkv: Tensor, key_mask: Optional[Tensor] = None, scale: Option
     if qkv.dim() != 5 or qkv.shape[2] != 3:
         raise ValueError(f"eve_amd.self_attention: `qkv` must be [B, N, 3, heads, width], got {tuple(qkv.shape)}")
     key_mask, scale = _check(*qkv.unbind(2), key_mask, scale)
-    return _SelfAttentionFn.apply(qkv, key_mask, scale)
+    if ops._tracks(qkv):
+        return _SelfAttentionFn.apply(qkv, key_mask, scale)
+    return ops.attn_fwd(*_readable_parts(qkv)[1], key_mask, scale, want_lse=False)[0]

@@ -14,23 +14,27 @@ from torch.autograd.function import once_differentiable
 from . import ops
 
 
+def _rows(x, weight, bias, gamma, row_scale, residual):
+    """The tensors as the kernels take them, contiguous and with the leading dimensions in one, and the rows of a sample."""
+    N, K = weight.shape
+    rows = math.prod(x.shape[:-1])
+    small = [None if t is None else t.contiguous() for t in (bias, gamma, row_scale)]
+    res2 = None if residual is None else residual.contiguous().view(rows, N)
+    per = max(1, rows // max(1, x.shape[0])) if row_scale is not None else 1
+    return (x.contiguous().view(rows, K), weight.contiguous(), *small, res2, per)
+
+
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, gamma, row_scale, residual, act):  # type: ignore[override]
-        N, K = weight.shape
-        rows = math.prod(x.shape[:-1])
-        x2 = x.contiguous().view(rows, K)
-        weight = weight.contiguous()
-        bias, gamma, row_scale = (None if t is None else t.contiguous() for t in (bias, gamma, row_scale))
-        res2 = None if residual is None else residual.contiguous().view(rows, N)
-        per = max(1, rows // max(1, x.shape[0])) if row_scale is not None else 1
+        x2, weight, bias, gamma, row_scale, res2, per = _rows(x, weight, bias, gamma, row_scale, residual)
         need = ctx.needs_input_grad
         save_z = need[3] or (act != ops.ACTS["identity"] and any(need[:3]))
         y, z = ops.linear_fwd(x2, weight, bias, gamma, row_scale, res2, per, act, save_z=save_z)
         if any(need[:4]):
             ctx.save_for_backward(x2, weight, z, gamma, row_scale)
         ctx.how = (x.shape, per, act, need)
-        return y.view(x.shape[:-1] + (N,))
+        return y.view(x.shape[:-1] + (weight.shape[0],))
 
     @staticmethod
     @once_differentiable
@@ -58,22 +62,27 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activ
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"eve_amd.fused_linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not belong together")
     ops._dt(x)
+    dtype, device, lead = x.dtype, x.device, x.shape[:-1]
     N = weight.shape[0]
-    want = {"bias": (N,), "gamma": (N,), "row_scale": tuple(x.shape[:1]), "residual": tuple(x.shape[:-1]) + (N,)}
-    parts = {"weight": weight, "bias": bias, "gamma": gamma, "row_scale": row_scale, "residual": residual}
-    for name, t in parts.items():
+    parts = (("weight", weight, weight.shape), ("bias", bias, (N,)), ("gamma", gamma, (N,)), ("row_scale", row_scale, x.shape[:1]),
+             ("residual", residual, lead + (N,)))
+    elsewhere = "" if not x.is_cuda else None
+    for name, t, shape in parts:
         if t is None:
             continue
-        if t.dtype != x.dtype:
-            raise TypeError(f"eve_amd.fused_linear: `{name}` is {t.dtype}, x {x.dtype}")
-        if name in want and tuple(t.shape) != want[name]:
-            raise ValueError(f"eve_amd.fused_linear: `{name}` has shape {tuple(t.shape)}, {want[name]} is needed")
+        if t.dtype != dtype:
+            raise TypeError(f"eve_amd.fused_linear: `{name}` is {t.dtype}, x {dtype}")
+        if t.shape != shape:
+            raise ValueError(f"eve_amd.fused_linear: `{name}` has shape {tuple(t.shape)}, {tuple(shape)} is needed")
+        if t.device != device:
+            elsewhere = f", `{name}` on {t.device}"
     if row_scale is not None and x.dim() < 2:
         raise ValueError("eve_amd.fused_linear: row_scale needs samples: x with two dimensions or more")
     if row_scale is not None and row_scale.requires_grad:
         raise ValueError("eve_amd.fused_linear: row_scale is a mask and has no gradient")
-    for name, t in parts.items():
-        if not x.is_cuda or (t is not None and t.device != x.device):
-            raise RuntimeError(f"eve_amd.fused_linear runs on one MI355X (x on {x.device}"
-                               + (f", `{name}` on {t.device}" if t is not None else "") + "); no CPU fallback")
-    return _LinearFn.apply(x, weight, bias, gamma, row_scale, residual, ops.ACTS[activation])
+    if elsewhere is not None:
+        raise RuntimeError(f"eve_amd.fused_linear runs on one MI355X (x on {device}{elsewhere}); no CPU fallback")
+    act = ops.ACTS[activation]
+    if ops._tracks(x, weight, bias, gamma, residual):
+        return _LinearFn.apply(x, weight, bias, gamma, row_scale, residual, act)
+    return ops.linear_fwd(*_rows(x, weight, bias, gamma, row_scale, residual), act)[0].view(lead + (N,))
