@@ -13,28 +13,9 @@ from torch.autograd.function import once_differentiable
 from . import ops
 
 
-def _check_mask(key_mask: Optional[Tensor], B: int, Nk: int, device) -> Optional[Tensor]:
-    if key_mask is None:
-        return None
-    if tuple(key_mask.shape) != (B, Nk):
-        raise ValueError(f"eve_amd.attention: `key_mask` has shape {tuple(key_mask.shape)}, the keys need {(B, Nk)}")
-    if key_mask.device != device:
-        raise RuntimeError(f"eve_amd.attention: `key_mask` is on {key_mask.device}, the queries on {device}")
-    return key_mask.bool().contiguous()
-
-
-def _check(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor], scale: Optional[float]):
-    """-> (key_mask, scale) as the kernels take them; shapes and types first, then the device."""
-    for t, n in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != 4:
-            raise ValueError(f"eve_amd.attention: `{n}` must be [B, N, heads, width], got {tuple(t.shape)}")
-    ops._dt(q)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"eve_amd.attention: q, k and v have types {q.dtype}, {k.dtype}, {v.dtype}: one is needed")
-    B, _, H, D = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
-        raise ValueError(f"eve_amd.attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not belong together")
-    Nk, Hkv = k.shape[1], k.shape[2]
+def _check(q: Tensor, Nk: int, Hkv: int, key_mask: Optional[Tensor], scale: Optional[float], on: bool):
+    """-> (key_mask, scale) as the kernels take them; q [.., H, D] with the batch in front.  Shapes first, then the device."""
+    B, H, D = q.shape[0], q.shape[-2], q.shape[-1]
     if H < 1 or Hkv < 1 or H % Hkv:
         raise ValueError(f"eve_amd.attention: {H} query heads cannot share {Hkv} key/value heads")
     if D % 8 or not 8 <= D <= 128:
@@ -42,9 +23,14 @@ def _check(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor], scale: O
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"eve_amd.attention: scale {scale} (must be positive and finite)")
-    key_mask = _check_mask(key_mask, B, Nk, q.device)
-    if not q.is_cuda or k.device != q.device or v.device != q.device:
-        raise RuntimeError(f"eve_amd.attention runs on one MI355X (inputs on {q.device}, {k.device}, {v.device}); no CPU fallback")
+    if key_mask is not None:
+        if key_mask.shape != (B, Nk):
+            raise ValueError(f"eve_amd.attention: `key_mask` has shape {tuple(key_mask.shape)}, the keys need {(B, Nk)}")
+        if key_mask.device != q.device:
+            raise RuntimeError(f"eve_amd.attention: `key_mask` is on {key_mask.device}, the queries on {q.device}")
+        key_mask = key_mask.bool().contiguous()
+    if not on:
+        raise RuntimeError(f"eve_amd.attention runs on one MI355X (queries on {q.device}); no CPU fallback")
     return key_mask, scale
 
 
@@ -63,17 +49,9 @@ class _AttentionFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):  # type: ignore[override]
         q, k, v, key_mask, out, lse = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         ops.attn_bwd(dout.contiguous(), q, k, v, key_mask, out, lse, ctx.scale, dq, dk, dv)
         return dq, dk, dv, None, None
-
-
-def _readable_parts(qkv):
-    parts = qkv.unbind(2)
-    if any(ops.attn_readable(t) is not t for t in parts):
-        qkv = qkv.clone(memory_format=torch.contiguous_format)
-        parts = qkv.unbind(2)
-    return qkv, parts
 
 
 class _SelfAttentionFn(torch.autograd.Function):
@@ -81,9 +59,9 @@ class _SelfAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, key_mask, scale):  # type: ignore[override]
-        qkv, (q, k, v) = _readable_parts(qkv)
+        qkv = ops.attn_readable(qkv)
         need = ctx.needs_input_grad[0]
-        out, lse = ops.attn_fwd(q, k, v, key_mask, scale, want_lse=need)
+        out, lse = ops.attn_qkv_fwd(qkv, key_mask, scale, want_lse=need)
         if need:
             ctx.save_for_backward(qkv, key_mask, out, lse)
             ctx.scale = scale
@@ -93,8 +71,8 @@ class _SelfAttentionFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):  # type: ignore[override]
         qkv, key_mask, out, lse = ctx.saved_tensors
-        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        ops.attn_bwd(dout.contiguous(), *qkv.unbind(2), key_mask, out, lse, ctx.scale, *dqkv.unbind(2))
+        dqkv = qkv.new_empty(qkv.shape)
+        ops.attn_qkv_bwd(dout.contiguous(), qkv, key_mask, out, lse, ctx.scale, dqkv)
         return dqkv, None, None
 
 
@@ -106,7 +84,16 @@ def attention(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor] = None
     D is a multiple of 8 up to 128.  key_mask [B, Nk]: nonzero = visible.  scale: D ** -0.5 unless given, positive.
     -> [B, Nq, H, D].  A sample without a visible key gives zeros and passes no gradient; masked keys and values may hold
     anything, NaN included.  Scores and sums are float32; results do not depend on the order of execution."""
-    key_mask, scale = _check(q, k, v, key_mask, scale)
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 4:
+            raise ValueError(f"eve_amd.attention: `{n}` must be [B, N, heads, width], got {tuple(t.shape)}")
+    ops._dt(q)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"eve_amd.attention: q, k and v have types {q.dtype}, {k.dtype}, {v.dtype}: one is needed")
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"eve_amd.attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not belong together")
+    on = q.is_cuda and k.device == q.device and v.device == q.device
+    key_mask, scale = _check(q, k.shape[1], k.shape[2], key_mask, scale, on)
     if ops._tracks(q, k, v):
         return _AttentionFn.apply(q, k, v, key_mask, scale)
     return ops.attn_fwd(ops.attn_readable(q), ops.attn_readable(k), ops.attn_readable(v), key_mask, scale, want_lse=False)[0]
@@ -116,7 +103,8 @@ def self_attention(qkv: Tensor, key_mask: Optional[Tensor] = None, scale: Option
     """`attention` over the three parts of one product qkv [B, N, 3, H, D] -> [B, N, H, D]; the gradient comes in qkv's shape."""
     if qkv.dim() != 5 or qkv.shape[2] != 3:
         raise ValueError(f"eve_amd.self_attention: `qkv` must be [B, N, 3, heads, width], got {tuple(qkv.shape)}")
-    key_mask, scale = _check(*qkv.unbind(2), key_mask, scale)
+    ops._dt(qkv)
+    key_mask, scale = _check(qkv, qkv.shape[1], qkv.shape[3], key_mask, scale, qkv.is_cuda)
     if ops._tracks(qkv):
         return _SelfAttentionFn.apply(qkv, key_mask, scale)
-    return ops.attn_fwd(*_readable_parts(qkv)[1], key_mask, scale, want_lse=False)[0]
+    return ops.attn_qkv_fwd(ops.attn_readable(qkv), key_mask, scale, want_lse=False)[0]

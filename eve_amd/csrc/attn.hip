@@ -674,8 +674,8 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
 // ---------------------------------------------------------------------------------------------------------- dk, dv
 // Columns are keys, held in registers; tiles of query rows (head after head of those that share the keys) pass by.
 //
-// Here L_i and delta_i belong to a row, that is, to a register, the same in 32 lanes.  The products start from -L_i / c and -delta_i:
-// p = 2^(c acc), ds = p acc'.  These starts are themselves a matrix product: a row's 16 bytes hold both values as three bf16 each
+// Here L_i and delta_i belong to a row, that is, to a register, the same in 32 lanes.  The products are given -L_i / c and -delta_i on top:
+// p = 2^(c acc), ds = p acc'.  These terms are themselves a matrix product: a row's 16 bytes hold both values as three bf16 each
 // (exactly, 24 bits), which multiply ones; read as values, four at a time, they would be a third of the loop's LDS traffic.
 // A row past the end is all zeros: p = 1 there, and its q and do, which p and ds multiply, are zero.
 template <typename T, int DP, int NW>
@@ -748,12 +748,14 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 #pragma unroll
       for (int j = 0; j < C::NJ; ++j) {
         const uint4 both = lds16(st_ + (32 * j + (lane & 31)) * 16);
-        at_f32x16 s = mma(both, one_L, acc_zero(), bf16_t()), dp = mma(both, one_d, acc_zero(), bf16_t());
+        at_f32x16 s = acc_zero(), dp = acc_zero();
 #pragma unroll
         for (int ks = 0; ks < C::NKS; ++ks) {
           s = mma(rows.get(smem, qs_, j, ks), kf[ks], s, T());
           dp = mma(rows.get(smem, gs_, j, ks), vf[ks], dp, T());
         }
+        s = mma(both, one_L, s, bf16_t());  // last: L / c is large, and every term added to it would be rounded at its size
+        dp = mma(both, one_d, dp, bf16_t());
         ColFrags<T, C> f;  // of do, read while the matrix unit works
         f.read(smem, gs_, j, cols, lane);
 #pragma unroll

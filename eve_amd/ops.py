@@ -424,59 +424,98 @@ def _on(device):
     return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def _attn_strides(t: torch.Tensor):
-    """Element strides of the first three dimensions of [B,N,H,D]; a dimension of one element has none to speak of."""
+def _attn_at(t: torch.Tensor):
+    """Address and element strides of the first three dimensions of [B,N,H,D]; a dimension of one element has none to speak of."""
     b, n, h, _ = t.shape
     sb, sn, sh, _ = t.stride()
-    return 0 if b == 1 else sb, 0 if n == 1 else sn, 0 if h == 1 else sh
+    return t.data_ptr(), 0 if b == 1 else sb, 0 if n == 1 else sn, 0 if h == 1 else sh
+
+
+def _attn_parts_at(t: torch.Tensor):
+    """The same of the three parts of [B,N,3,H,D]."""
+    b, n, _, h, _ = t.shape
+    sb, sn, step, sh, _ = t.stride()
+    at, step = t.data_ptr(), step * t.element_size()
+    rest = 0 if b == 1 else sb, 0 if n == 1 else sn, 0 if h == 1 else sh
+    return (at, *rest), (at + step, *rest), (at + 2 * step, *rest)
+
+
+def _attn_reads(at, unit: int) -> bool:
+    p, sb, sn, sh = at
+    return not (p % 16 or sb % unit or sn % unit or sh % unit or sn > 1 << 22)
 
 
 def attn_readable(t: torch.Tensor) -> torch.Tensor:
-    """`t` [B,N,H,D] as the kernels can read it: the last dimension contiguous, rows on 16-byte boundaries and at most 2^22
-    elements apart; else a copy."""
+    """`t` [B,N,H,D] (or [B,N,3,H,D], three of them) as the kernels can read it: the last dimension contiguous, rows on 16-byte
+    boundaries and at most 2^22 elements apart; else a copy."""
     unit = 16 // t.element_size()
-    sb, sn, sh = _attn_strides(t)
-    if (t.stride(3) != 1 or t.data_ptr() % 16 or sn > 1 << 22 or sb % unit or sn % unit or sh % unit) and t.numel():
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _attn_args(q, k, v, scale: float):
-    B, Nq, H, D = q.shape
-    Nk, Hkv = k.shape[1], k.shape[2]
-    return (_lib.AttnShape(B, Nq, Nk, H, Hkv, D, _dt(q), scale),
-            _lib.AttnLayout(*_attn_strides(q), *_attn_strides(k), *_attn_strides(v)))
+    parts = (_attn_at(t),) if t.dim() == 4 else _attn_parts_at(t)
+    if t.stride(-1) == 1 and all(_attn_reads(at, unit) for at in parts) or not t.numel():
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def attn_fwd(q, k, v, key_mask, scale: float, want_lse: bool = True):
     """q [B,Nq,H,D]; k, v [B,Nk,Hkv,D] (attn_readable); key_mask [B,Nk] bool | None -> (out [B,Nq,H,D], lse [B,H,Nq] | None).
     The order inside lse is the kernels' own."""
-    _chk(key_mask, "key_mask", torch.bool)
-    B, Nq, H, D = q.shape
-    with _on(q.device):
-        shape, layout = _attn_args(q, k, v, scale)
-        out = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device)
-        lse = torch.empty(B, H, Nq, dtype=torch.float32, device=q.device) if want_lse else None
-        ref = _lib.ctypes.addressof(shape)
-        nbytes = _lib.load().eve_attn_fwd_workspace_bytes(ref)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        PROFILE.call("eve_attn_fwd", ref, _lib.ctypes.addressof(layout), _p(q), _p(k), _p(v), _p(key_mask), _p(out), _p(lse),
-                     _p(ws), nbytes, _stream(), tag=f"N={Nq}x{k.shape[1]}")
-    return out, lse
+    return _attn_fwd((*q.shape[:3], *k.shape[1:]), (_attn_at(q), _attn_at(k), _attn_at(v)), q, key_mask, scale, want_lse)
+
+
+def attn_qkv_fwd(qkv, key_mask, scale: float, want_lse: bool = True):
+    """attn_fwd of the three parts of qkv [B,N,3,H,D]."""
+    B, N, _, H, D = qkv.shape
+    return _attn_fwd((B, N, H, N, H, D), _attn_parts_at(qkv), qkv, key_mask, scale, want_lse)
 
 
 def attn_bwd(dout, q, k, v, key_mask, out, lse, scale: float, dq, dk, dv) -> None:
     """Writes the gradients into dq, dk, dv, which have q's, k's, v's shapes and lie as attn_readable says."""
-    _chk(dout, "dout", q.dtype), _chk(out, "out", q.dtype), _chk(lse, "lse", torch.float32)
-    with _on(q.device):
-        shape, layout = _attn_args(q, k, v, scale)
-        grads = _lib.AttnLayout(*_attn_strides(dq), *_attn_strides(dk), *_attn_strides(dv))
+    _attn_bwd((*q.shape[:3], *k.shape[1:]), (_attn_at(q), _attn_at(k), _attn_at(v)), dout, key_mask, out, lse, scale,
+              (_attn_at(dq), _attn_at(dk), _attn_at(dv)))
+
+
+def attn_qkv_bwd(dout, qkv, key_mask, out, lse, scale: float, dqkv) -> None:
+    """attn_bwd of the three parts of qkv [B,N,3,H,D] into those of dqkv."""
+    B, N, _, H, D = qkv.shape
+    _attn_bwd((B, N, H, N, H, D), _attn_parts_at(qkv), dout, key_mask, out, lse, scale, _attn_parts_at(dqkv))
+
+
+def _attn_shape(dims, dtype, scale):
+    B, Nq, H, Nk, Hkv, D = dims
+    return _lib.AttnShape(B, Nq, Nk, H, Hkv, D, _DTYPES[dtype], scale)
+
+
+def _attn_layout(at):
+    (_, *a), (_, *b), (_, *c) = at
+    return _lib.AttnLayout(*a, *b, *c)
+
+
+def _attn_fwd(dims, at, like, key_mask, scale, want_lse):
+    _chk(key_mask, "key_mask", torch.bool)
+    B, Nq, H, Nk, _, D = dims
+    device = like.device
+    with _on(device):
+        shape, layout = _attn_shape(dims, like.dtype, scale), _attn_layout(at)
+        out = like.new_empty((B, Nq, H, D))
+        lse = torch.empty(B, H, Nq, dtype=torch.float32, device=device) if want_lse else None
+        ref = _lib.ctypes.addressof(shape)
+        nbytes = _lib.load().eve_attn_fwd_workspace_bytes(ref)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        PROFILE.call("eve_attn_fwd", ref, _lib.ctypes.addressof(layout), at[0][0], at[1][0], at[2][0], _p(key_mask), out.data_ptr(),
+                     _p(lse), _p(ws), nbytes, _stream(), tag=f"N={Nq}x{Nk}")
+    return out, lse
+
+
+def _attn_bwd(dims, at, dout, key_mask, out, lse, scale, grads_at):
+    _chk(dout, "dout", out.dtype), _chk(out, "out"), _chk(lse, "lse", torch.float32)
+    device = out.device
+    with _on(device):
+        shape, layout, grads = _attn_shape(dims, out.dtype, scale), _attn_layout(at), _attn_layout(grads_at)
         ref = _lib.ctypes.addressof(shape)
         nbytes = _lib.load().eve_attn_bwd_workspace_bytes(ref)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        PROFILE.call("eve_attn_bwd", ref, _lib.ctypes.addressof(layout), _lib.ctypes.addressof(grads), _p(q), _p(k), _p(v),
-                     _p(key_mask), _p(out), _p(lse), _p(dout), _p(dq), _p(dk), _p(dv), _p(ws), nbytes, _stream(),
-                     tag=f"N={q.shape[1]}x{k.shape[1]}")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        PROFILE.call("eve_attn_bwd", ref, _lib.ctypes.addressof(layout), _lib.ctypes.addressof(grads), at[0][0], at[1][0], at[2][0],
+                     _p(key_mask), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), grads_at[0][0], grads_at[1][0], grads_at[2][0],
+                     _p(ws), nbytes, _stream(), tag=f"N={dims[1]}x{dims[3]}")
 
 
 # ----------------------------------------------------------------------------- linear layer with its epilogue fused
