@@ -8,7 +8,6 @@ from typing import Optional
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -46,7 +45,7 @@ class _AttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @ops.once_differentiable
     def backward(ctx, dout):  # type: ignore[override]
         q, k, v, key_mask, out, lse = ctx.saved_tensors
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
@@ -68,7 +67,7 @@ class _SelfAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @ops.once_differentiable
     def backward(ctx, dout):  # type: ignore[override]
         qkv, key_mask, out, lse = ctx.saved_tensors
         dqkv = qkv.new_empty(qkv.shape)

@@ -9,7 +9,6 @@ from typing import Optional
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -29,19 +28,21 @@ class _LinearFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, gamma, row_scale, residual, act):  # type: ignore[override]
         x2, weight, bias, gamma, row_scale, res2, per = _rows(x, weight, bias, gamma, row_scale, residual)
         need = ctx.needs_input_grad
-        save_z = need[3] or (act != ops.ACTS["identity"] and any(need[:3]))
-        y, z = ops.linear_fwd(x2, weight, bias, gamma, row_scale, res2, per, act, save_z=save_z)
-        if any(need[:4]):
+        product = need[0] or need[1] or need[2]
+        y, z = ops.linear_fwd(x2, weight, bias, gamma, row_scale, res2, per, act,
+                              save_z=need[3] or (product and act != ops.ACTS["identity"]))
+        if product or need[3]:
             ctx.save_for_backward(x2, weight, z, gamma, row_scale)
-        ctx.how = (x.shape, per, act, need)
+        ctx.how = (x.shape, per, act)
         return y.view(x.shape[:-1] + (weight.shape[0],))
 
     @staticmethod
-    @once_differentiable
+    @ops.once_differentiable
     def backward(ctx, dy):  # type: ignore[override]
-        shape, per, act, need = ctx.how
+        shape, per, act = ctx.how
+        need = ctx.needs_input_grad
         dx = dw = db = dg = None
-        if any(need[:4]):
+        if need[0] or need[1] or need[2] or need[3]:
             x2, weight, z, gamma, row_scale = ctx.saved_tensors
             dx, dw, db, dg = ops.linear_bwd(dy.contiguous().view(x2.shape[0], weight.shape[0]), x2, weight, z, gamma, row_scale, per, act,
                                             need[:4])

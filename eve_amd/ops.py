@@ -6,11 +6,12 @@ kernels on the current stream.  No function here has a CPU implementation.
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
 from dataclasses import dataclass
+from functools import wraps
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable as _once_differentiable
 
 from . import _lib
 
@@ -46,6 +47,16 @@ def _p(t: Optional[torch.Tensor]):
 def _stream():
     # the current stream's handle; torch.cuda.current_stream() makes a Stream object of it, 2.8 us a call instead of 0.4
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def once_differentiable(backward):
+    """torch's decorator of this name, whose wrapping is done only where a graph of the gradient is wanted."""
+    wrapped = _once_differentiable(backward)
+
+    @wraps(backward)
+    def first(ctx, *grads):
+        return (wrapped if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return first
 
 
 def _tracks(*tensors) -> bool:
@@ -419,9 +430,19 @@ def scale_residual_bwd(dout, x, gamma, row_scale, T: int):
 
 
 # ----------------------------------------------------------------------------------- attention of the encoder layer
-def _on(device):
-    """Calls are enqueued on the current stream of the tensors' device, whichever device is current."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _on_device_of(which: int):
+    """Decorates a wrapper: its calls are enqueued on the current stream of the device of argument `which`, whichever device is
+    current."""
+    def wrap(f):
+        @wraps(f)
+        def on_device(*args, **kwargs):
+            device = args[which].get_device()
+            if device == torch.cuda.current_device():
+                return f(*args, **kwargs)
+            with torch.cuda.device(device):
+                return f(*args, **kwargs)
+        return on_device
+    return wrap
 
 
 def _attn_at(t: torch.Tensor):
@@ -489,63 +510,64 @@ def _attn_layout(at):
     return _lib.AttnLayout(*a, *b, *c)
 
 
+@_on_device_of(2)
 def _attn_fwd(dims, at, like, key_mask, scale, want_lse):
     _chk(key_mask, "key_mask", torch.bool)
     B, Nq, H, Nk, _, D = dims
     device = like.device
-    with _on(device):
-        shape, layout = _attn_shape(dims, like.dtype, scale), _attn_layout(at)
-        out = like.new_empty((B, Nq, H, D))
-        lse = torch.empty(B, H, Nq, dtype=torch.float32, device=device) if want_lse else None
-        ref = _lib.ctypes.addressof(shape)
-        nbytes = _lib.load().eve_attn_fwd_workspace_bytes(ref)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        PROFILE.call("eve_attn_fwd", ref, _lib.ctypes.addressof(layout), at[0][0], at[1][0], at[2][0], _p(key_mask), out.data_ptr(),
-                     _p(lse), _p(ws), nbytes, _stream(), tag=f"N={Nq}x{Nk}")
+    shape, layout = _attn_shape(dims, like.dtype, scale), _attn_layout(at)
+    out = like.new_empty((B, Nq, H, D))
+    lse = torch.empty(B, H, Nq, dtype=torch.float32, device=device) if want_lse else None
+    ref = _lib.ctypes.addressof(shape)
+    nbytes = _lib.load().eve_attn_fwd_workspace_bytes(ref)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    PROFILE.call("eve_attn_fwd", ref, _lib.ctypes.addressof(layout), at[0][0], at[1][0], at[2][0], _p(key_mask), out.data_ptr(),
+                 _p(lse), _p(ws), nbytes, _stream(), tag=f"N={Nq}x{Nk}")
     return out, lse
 
 
+@_on_device_of(2)
 def _attn_bwd(dims, at, dout, key_mask, out, lse, scale, grads_at):
     _chk(dout, "dout", out.dtype), _chk(out, "out"), _chk(lse, "lse", torch.float32)
     device = out.device
-    with _on(device):
-        shape, layout, grads = _attn_shape(dims, out.dtype, scale), _attn_layout(at), _attn_layout(grads_at)
-        ref = _lib.ctypes.addressof(shape)
-        nbytes = _lib.load().eve_attn_bwd_workspace_bytes(ref)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        PROFILE.call("eve_attn_bwd", ref, _lib.ctypes.addressof(layout), _lib.ctypes.addressof(grads), at[0][0], at[1][0], at[2][0],
-                     _p(key_mask), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), grads_at[0][0], grads_at[1][0], grads_at[2][0],
-                     _p(ws), nbytes, _stream(), tag=f"N={dims[1]}x{dims[3]}")
+    shape, layout, grads = _attn_shape(dims, out.dtype, scale), _attn_layout(at), _attn_layout(grads_at)
+    ref = _lib.ctypes.addressof(shape)
+    nbytes = _lib.load().eve_attn_bwd_workspace_bytes(ref)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    PROFILE.call("eve_attn_bwd", ref, _lib.ctypes.addressof(layout), _lib.ctypes.addressof(grads), at[0][0], at[1][0], at[2][0],
+                 _p(key_mask), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), grads_at[0][0], grads_at[1][0], grads_at[2][0],
+                 _p(ws), nbytes, _stream(), tag=f"N={dims[1]}x{dims[3]}")
 
 
 # ----------------------------------------------------------------------------- linear layer with its epilogue fused
+@_on_device_of(0)
 def linear_fwd(x, w, bias, gamma, row_scale, residual, rows_per_scale: int, act: int, save_z: bool = False):
     """x [S,K]; w [N,K]; bias, gamma [N] | None; row_scale [S / rows_per_scale] | None; residual [S,N] | None
     -> (residual + row_scale * gamma * act(x w^T + bias) [S,N], z = x w^T + bias [S,N] | None)."""
+    dtype = x.dtype
     for t, n in ((x, "x"), (w, "weight"), (bias, "bias"), (gamma, "gamma"), (row_scale, "row_scale"), (residual, "residual")):
+        if t is not None:
+            _chk(t, n, dtype)
+    S, K = x.shape
+    N = w.shape[0]
+    y = x.new_empty((S, N))
+    z = x.new_empty((S, N)) if save_z else None
+    PROFILE.call("eve_linear_fwd", _p(x), _p(w), _p(bias), _p(gamma), _p(row_scale), _p(residual), _p(y), _p(z), S,
+                 rows_per_scale, K, N, act, _dt(x), _stream(), tag=f"{S}x{K}x{N}")
+    return y, z
+
+
+@_on_device_of(0)
+def linear_bwd(dy, x, w, z, gamma, row_scale, rows_per_scale: int, act: int, want):
+    """-> (dx, dw, dbias, dgamma), None where `want` (four truth values) does not ask for one."""
+    for t, n in ((dy, "dy"), (w, "weight"), (z, "z"), (gamma, "gamma"), (row_scale, "row_scale")):
         if t is not None:
             _chk(t, n, x.dtype)
     S, K = x.shape
     N = w.shape[0]
-    with _on(x.device):
-        y = torch.empty(S, N, dtype=x.dtype, device=x.device)
-        z = torch.empty_like(y) if save_z else None
-        PROFILE.call("eve_linear_fwd", _p(x), _p(w), _p(bias), _p(gamma), _p(row_scale), _p(residual), _p(y), _p(z), S,
-                     rows_per_scale, K, N, act, _dt(x), _stream(), tag=f"{S}x{K}x{N}")
-    return y, z
-
-
-def linear_bwd(dy, x, w, z, gamma, row_scale, rows_per_scale: int, act: int, want):
-    """-> (dx, dw, dbias, dgamma), None where `want` (four truth values) does not ask for one."""
-    for t, n in ((dy, "dy"), (w, "weight"), (z, "z"), (gamma, "gamma"), (row_scale, "row_scale")):
-        _chk(t, n, x.dtype)
-    S, K = x.shape
-    N = w.shape[0]
-    with _on(x.device):
-        shapes = ((S, K), (N, K), (N,), (N,))
-        outs = [torch.empty(s, dtype=x.dtype, device=x.device) if yes else None for s, yes in zip(shapes, want)]
-        nbytes = _lib.load().eve_linear_bwd_workspace_bytes(S, K, N, _dt(x))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        PROFILE.call("eve_linear_bwd", _p(dy), _p(x), _p(w), _p(z), _p(gamma), _p(row_scale), *(_p(o) for o in outs), S,
-                     rows_per_scale, K, N, act, _dt(x), _p(ws), nbytes, _stream(), tag=f"{S}x{K}x{N}")
+    outs = [x.new_empty(s) if yes else None for s, yes in zip(((S, K), (N, K), (N,), (N,)), want)]
+    nbytes = _lib.load().eve_linear_bwd_workspace_bytes(S, K, N, _dt(x))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    PROFILE.call("eve_linear_bwd", _p(dy), _p(x), _p(w), _p(z), _p(gamma), _p(row_scale), *(_p(o) for o in outs), S,
+                 rows_per_scale, K, N, act, _dt(x), _p(ws), nbytes, _stream(), tag=f"{S}x{K}x{N}")
     return outs
