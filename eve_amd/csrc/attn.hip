@@ -155,13 +155,17 @@ template <typename C> __device__ __forceinline__ uint4 col_frag_f32(const char* 
 // The column fragments of 32-row block j of a tile: f[c ND + i]
 template <typename T, typename C> struct ColFrags {
   uint4 f[C::PC * C::ND];
+  // bf16: of column blocks 2 pair and 2 pair + 1, g[2 chunk + block]
+  static __device__ __forceinline__ void read_pair(const char* smem, uint32_t at, int j, int pair, const ColReader<C>& r, uint4 (&g)[4]) {
+    const uint32_t tile = lds_offset(smem) + at + j * 32 * C::RB + pair * 128;
+    tr_frags4<C::RB>(tile + r.base[0], tile + r.base[1], g);
+  }
   __device__ __forceinline__ void read(const char* smem, uint32_t at, int j, const ColReader<C>& r, int lane) {
     if constexpr (sizeof(T) == 2) {
-      const uint32_t tile = lds_offset(smem) + at + j * 32 * C::RB;
 #pragma unroll
       for (int pair = 0; pair < C::ND / 2; ++pair) {
         uint4 g[4];
-        tr_frags4<C::RB>(tile + r.base[0] + pair * 128, tile + r.base[1] + pair * 128, g);
+        read_pair(smem, at, j, pair, r, g);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -749,6 +753,34 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
       for (int j = 0; j < C::NJ; ++j) {
         const uint4 both = lds16(st_ + (32 * j + (lane & 31)) * 16);
         at_f32x16 s = acc_zero(), dp = acc_zero();
+        if constexpr (sizeof(T) == 2 && DP == 128) {  // one after the other, a pair of column blocks at a time: all at once spills
+#pragma unroll
+          for (int ks = 0; ks < C::NKS; ++ks) s = mma(rows.get(smem, qs_, j, ks), kf[ks], s, T());
+          s = mma(both, one_L, s, bf16_t());
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * a.c);
+          uint4 x[2] = {acc_frag(s, 0, T()), acc_frag(s, 1, T())}, f[4];
+#pragma unroll
+          for (int i = 0; i < C::ND; ++i) {
+            if (i % 2 == 0) ColFrags<T, C>::read_pair(smem, gs_, j, i / 2, cols, f);
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) dv[i] = mma(f[2 * cc + i % 2], x[cc], dv[i], T());
+          }
+#pragma unroll
+          for (int ks = 0; ks < C::NKS; ++ks) dp = mma(rows.get(smem, gs_, j, ks), vf[ks], dp, T());
+          dp = mma(both, one_d, dp, bf16_t());
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+          x[0] = acc_frag(dp, 0, T());
+          x[1] = acc_frag(dp, 1, T());
+#pragma unroll
+          for (int i = 0; i < C::ND; ++i) {
+            if (i % 2 == 0) ColFrags<T, C>::read_pair(smem, qs_, j, i / 2, cols, f);
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) dk[i] = mma(f[2 * cc + i % 2], x[cc], dk[i], T());
+          }
+          continue;
+        }
 #pragma unroll
         for (int ks = 0; ks < C::NKS; ++ks) {
           s = mma(rows.get(smem, qs_, j, ks), kf[ks], s, T());
