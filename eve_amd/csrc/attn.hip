@@ -19,9 +19,8 @@
 //
 // LDS.  Tiles go from memory to LDS directly (buffer_load ... lds, 1 KiB a wave instruction) into a ring of stages, one tile
 // ahead of the one that is worked on.  A masked row is an offset outside the descriptor, for which the hardware delivers zeros.
-// The 16-byte chunks of a row are permuted by ((row & 3) << 1 | row >> 2 & 1) -- on the source side, since the transfer writes LDS
-// in lane order -- so that both ways of reading spread over all banks: the same chunk of eight consecutive rows (row fragments),
-// and a pair of chunks of four consecutive rows (transposed fragments).
+// The 16-byte chunks of a row are permuted (AttnCfg::swizzle) -- on the source side, since the transfer writes LDS in lane order --
+// so that both ways of reading, row fragments and transposed ones, spread over all banks.
 // No atomics: dq and dk/dv have a kernel each (7 products instead of 5), so results do not depend on the order of execution.
 #include <math.h>
 
@@ -72,6 +71,13 @@ template <typename T, int DP> struct AttnCfg {
   static constexpr int PC = 32 / (2 * E);               // fragments of a 32-row accumulator
   static constexpr int ND = DP / 32;
   static constexpr int NJ = KT / 32;
+  // Chunk c of a row lies at c ^ swizzle(row).  The banks are 256 bytes wide: 16 rows' fragments (a chunk each) take different ones,
+  // as do four rows' 64 bytes (bf16 columns) or a row's 128 bytes and those of the row four further on (fp32 columns).
+  static constexpr int swizzle(int row) {
+    return RB == 128 ? (row >> 1 & 1) << 2 | (row >> 2 & 1) << 1 | (row >> 3 & 1)
+           : sizeof(T) == 2 ? (row & 3) << 2 | (row >> 2 & 3)
+                            : (row >> 2 & 1) << 3 | (row & 3) << 1 | (row >> 3 & 1);
+  }
 };
 
 constexpr int kBitTiles = 64;  // tiles whose mask words a workgroup holds
@@ -95,7 +101,6 @@ __device__ __forceinline__ uint4 lds16(const char* p) {
   const at_u32x4 w = *reinterpret_cast<const at_u32x4*>(p);
   return make_uint4(w.x, w.y, w.z, w.w);
 }
-__device__ __forceinline__ int chunk_swizzle(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
 __device__ __forceinline__ uint32_t lds_offset(const char* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
 
 // A lane's place in the row fragments of a tile (at smem + tile, a multiple of 128 bytes): row lane & 31 of 32-row block j, step ks.
@@ -103,10 +108,11 @@ template <typename C> struct RowReader {
   uint32_t base;
   __device__ __forceinline__ explicit RowReader(int lane) {
     const int row = lane & 31;
-    base = row * C::RB + (((lane >> 5) ^ chunk_swizzle(row)) << 4);
+    base = row * C::RB + (((lane >> 5) ^ C::swizzle(row)) << 4);
   }
   __device__ __forceinline__ uint4 get(const char* smem, uint32_t tile, int j, int ks) const {
-    return lds16(smem + (((tile + base) ^ ((ks & 3) << 5)) + (ks >> 2) * 128 + j * 32 * C::RB));
+    constexpr int W = C::RB == 128 ? 4 : 8;  // steps whose chunks are permuted among themselves
+    return lds16(smem + (((tile + base) ^ ((ks % W) << 5)) + ks / W * 256 + j * 32 * C::RB));
   }
 };
 
@@ -114,16 +120,18 @@ template <typename C> struct RowReader {
 // 4 h + {0..3}, then 8 + 4 h + {0..3}).  Fragments -- of the two 16-row chunks of 32 rows, two column blocks -- are read and
 // waited for in one block: through the builtin the compiler would also wait for the tiles in flight, which it cannot tell apart
 // from what is read.
-template <int RB> __device__ __forceinline__ void tr_frags4(uint32_t a0, uint32_t a1, uint4 (&f)[4]) {  // f[2 chunk + column block]
+template <typename C> __device__ __forceinline__ void tr_frags4(const char* smem, uint32_t a0, uint32_t a1, uint4 (&f)[4]) {  // f[2 chunk + column block]
+  constexpr int RB = C::RB, X = (C::swizzle(8) ^ C::swizzle(0)) << 4;  // eight rows on
+  const uint32_t at = lds_offset(smem);
   at_s16x4 v[8];
   asm volatile(
-      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
-      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%10\n\t"
-      "ds_read_b64_tr_b16 %4, %8 offset:%11\n\tds_read_b64_tr_b16 %5, %8 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %6, %9 offset:%11\n\tds_read_b64_tr_b16 %7, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %8 offset:%13\n\tds_read_b64_tr_b16 %5, %10 offset:%14\n\t"
+      "ds_read_b64_tr_b16 %6, %9 offset:%13\n\tds_read_b64_tr_b16 %7, %11 offset:%14\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
-      : "v"(a0), "v"(a1), "n"(8 * RB), "n"(16 * RB), "n"(24 * RB)
+      : "v"(at + a0), "v"(at + a1), "v"(at + (a0 ^ X)), "v"(at + (a1 ^ X)), "n"(8 * RB), "n"(16 * RB), "n"(24 * RB)
       : "memory");
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -131,13 +139,13 @@ template <int RB> __device__ __forceinline__ void tr_frags4(uint32_t a0, uint32_
     f[i] = __builtin_bit_cast(uint4, w);
   }
 }
-// A lane's place in them: column blocks 0 and 1 (block i: (i & 1), + 128 (i >> 1) bytes)
+// A lane's place in them: column blocks 0 and 1 (those of pair p: 128 p bytes on, permuted)
 template <typename C> struct ColReader {
   uint32_t base[2];
   __device__ __forceinline__ explicit ColReader(int lane) {
     const int i = lane & 15, q = i >> 2, p = i & 3, h = lane >> 5;
     const int c = 2 * ((lane >> 4) & 1) + (p >> 1);
-    base[0] = (4 * h + q) * C::RB + ((c ^ (q << 1 | h)) << 4) + (p & 1) * 8;
+    base[0] = (4 * h + q) * C::RB + ((c ^ C::swizzle(4 * h + q)) << 4) + (p & 1) * 8;
     base[1] = base[0] ^ 64;
   }
 };
@@ -148,7 +156,7 @@ template <typename C> __device__ __forceinline__ uint4 col_frag_f32(const char* 
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     const int row = r0 + 8 * c + 4 * h + t;
-    w[t] = *reinterpret_cast<const uint32_t*>(smem + (tile + row * C::RB + (((col >> 2) ^ (t << 1 | h)) << 4) + (col & 3) * 4));
+    w[t] = *reinterpret_cast<const uint32_t*>(smem + (tile + row * C::RB + (((col >> 2) ^ C::swizzle(row)) << 4) + (col & 3) * 4));
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -157,8 +165,8 @@ template <typename T, typename C> struct ColFrags {
   uint4 f[C::PC * C::ND];
   // bf16: of column blocks 2 pair and 2 pair + 1, g[2 chunk + block]
   static __device__ __forceinline__ void read_pair(const char* smem, uint32_t at, int j, int pair, const ColReader<C>& r, uint4 (&g)[4]) {
-    const uint32_t tile = lds_offset(smem) + at + j * 32 * C::RB + pair * 128;
-    tr_frags4<C::RB>(tile + r.base[0], tile + r.base[1], g);
+    const uint32_t tile = at + j * 32 * C::RB;
+    tr_frags4<C>(smem, (tile + r.base[0]) ^ pair * 128, (tile + r.base[1]) ^ pair * 128, g);
   }
   __device__ __forceinline__ void read(const char* smem, uint32_t at, int j, const ColReader<C>& r, int lane) {
     if constexpr (sizeof(T) == 2) {
@@ -282,7 +290,7 @@ template <typename C, int NW> struct TileLoader {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       row[i] = (i * NW + wave) * (64 / C::CPR) + lane / C::CPR;
-      const int c = (lane % C::CPR) ^ chunk_swizzle(row[i]);
+      const int c = (lane % C::CPR) ^ C::swizzle(row[i]);
       off[i] = c * C::E < D ? (uint32_t)row[i] * ((uint32_t)stride * (16 / C::E)) + c * 16 : kNowhere;
     }
   }
@@ -955,7 +963,7 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
 
   const int qblk = wave & 1, dblk = (wave >> 1) & 1, upper = wave_u >> 2;  // my block of dq^T, my half of the keys
   char* ds_at = smem + kDs + key * 128 + half * 8;
-  const int ds_swz = chunk_swizzle(key);
+  const int ds_swz = C::swizzle(key);
   char* part = smem + kHalf + (wave & 3) * 4096 + lane * 16;
   at_f32x16 dq = acc_zero();
   auto dq_store = [&](int t) {  // tile t: the upper half's part was written before the last barrier
@@ -1026,12 +1034,12 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
     __builtin_amdgcn_s_barrier();  // ds is whole (the tiles on their way stay so)
     asm volatile("" ::: "memory");
     dq = acc_zero();
-    const uint32_t ka = lds_offset(smem) + kKeys + upper * (KEYS / 2 * 128) + (cols.base[0] ^ (dblk << 6));
-    const uint32_t da = lds_offset(smem) + kDs + upper * (KEYS / 2 * 128) + (cols.base[0] ^ (qblk << 6));
+    const uint32_t ka = kKeys + upper * (KEYS / 2 * 128) + (cols.base[0] ^ (dblk << 6));
+    const uint32_t da = kDs + upper * (KEYS / 2 * 128) + (cols.base[0] ^ (qblk << 6));
 #pragma unroll
     for (int i = 0; i < KEYS / 64; ++i) {
       uint4 f[4];  // 32 keys: of the keys' block, of ds, twice
-      tr_frags4<128>(ka + i * 4096, da + i * 4096, f);
+      tr_frags4<C>(smem, ka + i * 4096, da + i * 4096, f);
       dq = mma(f[0], f[1], dq, T());
       dq = mma(f[2], f[3], dq, T());
     }
