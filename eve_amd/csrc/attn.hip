@@ -395,10 +395,18 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
       for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[j][r]);
-      const float m_new = fmaxf(m, halves_max(mt) * a.c);
-      const float ms = m_new == -INFINITY ? 0.f : m_new;  // nothing visible so far: 2^(-inf - 0) = 0
-      const float alpha = __builtin_amdgcn_exp2f(m - ms);
-      m = m_new;
+      // m is any number that keeps the sums in range: it follows the maximum only where that is 2^8 ahead, so that rows rarely rescale
+      const float mx = halves_max(mt) * a.c;
+      if (__any(mx > m + 8.f)) {
+        const float m_new = fmaxf(m, mx), alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < C::ND; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+      }
+      const float ms = m == -INFINITY ? 0.f : m;  // nothing visible so far: 2^(-inf - 0) = 0
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < C::NJ; ++j)
@@ -407,13 +415,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
           s[j][r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], a.c, -ms));
           sum += s[j][r];
         }
-      l = fmaf(l, alpha, sum);
-      if (__any(alpha != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < C::ND; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
-      }
+      l += sum;
 #pragma unroll
       for (int j = 0; j < C::NJ; ++j) {
         if (j > 0) vf.read(smem, vs_, j, cols, lane);
