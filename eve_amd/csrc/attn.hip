@@ -24,6 +24,8 @@
 // No atomics: dq and dk/dv have a kernel each (7 products instead of 5), so results do not depend on the order of execution.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace eve {
@@ -890,6 +892,7 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
   const T* gb = static_cast<const T*>(a.dout) + (int64_t)b * a.Nq * o_n + (int64_t)hk * a.G * a.D;
   const T* ob = static_cast<const T*>(a.o) + (int64_t)b * a.Nq * o_n + (int64_t)hk * a.G * a.D;
   const int tq = (a.Nq + C::KT - 1) / C::KT, nt = tq * a.G;
+  const uint8_t mine = !key_ok ? 0 : mask ? mask[key] : 1;
   const TileLoader<C, NW> ql(a.in.q_n, a.D, wave, lane), gl(o_n, a.D, wave, lane), kl(a.in.k_n, a.D, wave, lane);
   const RowReader<C> rows(lane);
   const ColReader<C> cols(lane);
@@ -918,14 +921,23 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
   };
   auto stats_store = [&](int t) {
     float delta = dot16<T>(__builtin_bit_cast(uint4, st_g), __builtin_bit_cast(uint4, st_o));
-    delta += __shfl_xor(delta, 1, 64);
-    delta += __shfl_xor(delta, 2, 64);
-    delta += __shfl_xor(delta, 4, 64);
+    auto from = [&](auto pattern) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(delta), decltype(pattern)::value, 0xf, 0xf, true)); };
+    delta += from(std::integral_constant<int, 0xb1>());   // lane ^ 1
+    delta += from(std::integral_constant<int, 0x4e>());   // lane ^ 2
+    delta += from(std::integral_constant<int, 0x141>());  // 7 - lane of the eight
     if ((tid & 7) == 0) *reinterpret_cast<uint4*>(smem + kStats + (t & 1) * 1024 + (tid >> 3) * 16) = row_stats(st_L, delta, a.inv_c);
   };
 
   stats_request(0);
   fetch(0);
+  {  // the keys that dq multiplies, 64 of them in a step
+    const T* kb = static_cast<const T*>(a.k) + b * a.in.k_b + hk * a.in.k_h;
+#pragma unroll
+    for (int i = 0; i < KEYS / C::KT; ++i) {
+      const int n = a.Nk - i * C::KT;
+      kl.load(kb + (int64_t)i * C::KT * a.in.k_n, smem + kKeys + i * C::TILE, wave_u, n >= C::KT ? C::kFull : n > 0 ? (1ull << n) - 1 : 0);
+    }
+  }
   uint4 kf[C::NKS], vf[C::NKS];
   {
     const T* kp = static_cast<const T*>(a.k) + b * a.in.k_b + hk * a.in.k_h + (int64_t)key * a.in.k_n;
@@ -940,18 +952,7 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
       }
     }
   }
-  const bool see = key_ok && (!mask || mask[key] != 0);
-  const bool wave_sees = __any(see), wave_full = __all(see);
-  {  // the keys that dq multiplies: 64 of them in a step, a masked one as zeros
-    char* to = smem + kKeys;
-    const T* kb = static_cast<const T*>(a.k) + b * a.in.k_b + hk * a.in.k_h;
-#pragma unroll
-    for (int i = 0; i < KEYS / C::KT; ++i) {
-      const int first = i * C::KT + lane;
-      const uint64_t bits = __ballot(first < a.Nk && (!mask || mask[first] != 0));
-      kl.load(kb + (int64_t)i * C::KT * a.in.k_n, to + i * C::TILE, wave_u, bits);
-    }
-  }
+  const bool see = mine != 0, wave_sees = __any(see), wave_full = __all(see);
   if (!wave_sees) {  // its part of ds stays zero
     for (int i = lane; i < 32 * 8; i += 64) *reinterpret_cast<uint4*>(smem + kDs + wave * 4096 + i * 16) = make_uint4(0, 0, 0, 0);
   }
@@ -989,9 +990,13 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
     const uint32_t qs_ = kRing + (t & 1) * C::STAGE, gs_ = qs_ + C::TILE;
     const char* st_ = smem + kStats + (t & 1) * 1024;
     tile_ready<0>();
+    fetch(t + 1);
+    if (t == 0 && !see) {  // a masked key, which may hold anything: its ds is zero
+#pragma unroll
+      for (int c = 0; c < 4; ++c) *reinterpret_cast<at_u32x4*>(smem + kKeys + key * C::RB + half * 64 + c * 16) = at_u32x4{0, 0, 0, 0};
+    }
     stats_store(t + 1);
     stats_request(t + 2);
-    fetch(t + 1);
     if (t > 0 && !upper) dq_store(t - 1);
     if (wave_sees) {
 #pragma unroll
