@@ -347,7 +347,7 @@ __device__ __forceinline__ void lin_epilogue(const li_f32x16 (&acc)[NTM][NTN], c
 }
 #endif
 
-// BT x BT tile, 4 waves of (BT/2) x (BT/2); two LDS stages, the next step's tiles in registers meanwhile.
+// BT x BT tile, 4 waves of (BT/2) x (BT/2); two LDS stages, the next two steps' tiles in registers meanwhile.
 template <typename T, int BT, bool ACOL, bool BCOL, int MODE>
 __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -378,32 +378,36 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  LinTile<T, ACOL, BT> ta;
-  LinTile<T, BCOL, BT> tb;
+  LinTile<T, ACOL, BT> ta[2];
+  LinTile<T, BCOL, BT> tb[2];
   const int steps = (k1 - k0 + BK - 1) / BK;
-  auto fetch = [&](int t) {
-    ta.load(Ap + t * sa, a.lda, a.M - m0, k1 - k0 - t * BK, tid);
-    tb.load(Bp + t * sb, a.ldb, a.N - n0, k1 - k0 - t * BK, tid);
+  auto fetch = [&](int t, int i) {  // past the last step: zeros
+    ta[i].load(Ap + t * sa, a.lda, a.M - m0, k1 - k0 - t * BK, tid);
+    tb[i].load(Bp + t * sb, a.ldb, a.N - n0, k1 - k0 - t * BK, tid);
   };
-  if (steps > 0) fetch(0);
-  for (int t = 0; t < steps; ++t) {
-    char* as = smem + (t & 1) * STAGE;
-    char* bs = as + BT * 128;
-    ta.store(as, tid);
-    tb.store(bs, tid);
-    __syncthreads();
-    if (t + 1 < steps) fetch(t + 1);
+  fetch(0, 0);
+  fetch(1, 1);
+  for (int t = 0; t < steps; t += 2) {
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      uint4 fa[NT], fb[NT];
+    for (int u = 0; u < 2; ++u) {
+      char* as = smem + u * STAGE;
+      char* bs = as + BT * 128;
+      ta[u].store(as, tid);
+      tb[u].store(bs, tid);
+      __syncthreads();
+      fetch(t + u + 2, u);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) fa[i] = lfrag<T, ACOL, BT>(as, wm * (BT / 2) + 32 * i, ks, lane);
+      for (int ks = 0; ks < NKS; ++ks) {
+        uint4 fa[NT], fb[NT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) fb[j] = lfrag<T, BCOL, BT>(bs, wn * (BT / 2) + 32 * j, ks, lane);
+        for (int i = 0; i < NT; ++i) fa[i] = lfrag<T, ACOL, BT>(as, wm * (BT / 2) + 32 * i, ks, lane);
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+        for (int j = 0; j < NT; ++j) fb[j] = lfrag<T, BCOL, BT>(bs, wn * (BT / 2) + 32 * j, ks, lane);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = lmma(fb[j], fa[i], acc[i][j], T());
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = lmma(fb[j], fa[i], acc[i][j], T());
+      }
     }
   }
   __syncthreads();  // the stages become the waves' epilogue images
