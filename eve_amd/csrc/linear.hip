@@ -661,6 +661,18 @@ __global__ __launch_bounds__(256, 2) void linear_stream_kernel(LinArgs a) {
 #endif
 }
 
+// the epilogue of one element
+template <typename T> __device__ __forceinline__ void lin_finish(const LinArgs& a, int m, int n, float v) {
+  const int64_t at = (int64_t)m * a.N + n;
+  if (a.bias) v += to_f32<T>(static_cast<const T*>(a.bias)[n]);
+  if (a.z) static_cast<T*>(a.z)[at] = from_f32<T>(v);
+  v = act_of<T>(v, a.act);
+  if (a.gamma) v *= to_f32<T>(static_cast<const T*>(a.gamma)[n]);
+  if (a.row_scale) v *= to_f32<T>(static_cast<const T*>(a.row_scale)[m / a.rows_per_scale]);
+  if (a.residual) v += to_f32<T>(static_cast<const T*>(a.residual)[at]);
+  static_cast<T*>(a.C)[at] = from_f32<T>(v);
+}
+
 // A few rows: one wave a column, the weight's row read once for all of them.
 template <typename T, int R>
 __global__ __launch_bounds__(256) void linear_few_kernel(LinArgs a) {
@@ -689,14 +701,96 @@ __global__ __launch_bounds__(256) void linear_few_kernel(LinArgs a) {
 #pragma unroll
   for (int r = 1; r < R; ++r) v = lane == r ? acc[r] : v;
   if (lane < R && lane < a.M) {
-    const int64_t at = (int64_t)lane * a.N + n;
-    if (a.bias) v += to_f32<T>(static_cast<const T*>(a.bias)[n]);
-    if (a.z) static_cast<T*>(a.z)[at] = from_f32<T>(v);
-    v = act_of<T>(v, a.act);
-    if (a.gamma) v *= to_f32<T>(static_cast<const T*>(a.gamma)[n]);
-    if (a.row_scale) v *= to_f32<T>(static_cast<const T*>(a.row_scale)[lane / a.rows_per_scale]);
-    if (a.residual) v += to_f32<T>(static_cast<const T*>(a.residual)[at]);
-    static_cast<T*>(a.C)[at] = from_f32<T>(v);
+    lin_finish<T>(a, lane, n, v);
+  }
+#endif
+}
+
+// A long contraction and few tiles: 8 waves of a workgroup share one tile's contraction and add their sums through LDS, in order.
+// Tile: R x R with R = 16 NTL.  Fragments come from memory as they are (16 rows by 64 bytes, neighbouring lines in the next steps of
+// a wave), one unit of U steps ahead; a row past the end is the last one again, whose results are not kept.
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef __attribute__((ext_vector_type(4))) float li_f32x4;
+__device__ __forceinline__ li_f32x4 lmma16(const uint4& a, const uint4& b, li_f32x4 acc, bf16_t) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(li_bf16x8, a), __builtin_bit_cast(li_bf16x8, b), acc, 0, 0, 0);
+}
+__device__ __forceinline__ li_f32x4 lmma16(const uint4& a, const uint4& b, li_f32x4 acc, float) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.x), __uint_as_float(b.x), acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.y), __uint_as_float(b.y), acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.z), __uint_as_float(b.z), acc, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w), __uint_as_float(b.w), acc, 0, 0, 0);
+}
+#endif
+template <typename T, int NTL>
+__global__ __launch_bounds__(512, 2) void linear_shared_kernel(LinArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int E = LT<T>::E, NW = 8, R = 16 * NTL, U = NTL == 1 ? 4 : 2, UK = U * 4 * E;
+  __shared__ __attribute__((aligned(16))) float red[NW][R][R + 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, quad = lane >> 4;
+  // a run of tiles an XCD, rows fastest: the weight's rows, which are the many, are read into one L2
+  const int tm = (a.M + R - 1) / R, total = tm * ((a.N + R - 1) / R), per = (total + 7) >> 3;
+  const int item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || item >= total) return;
+  const int m0 = item % tm * R, n0 = item / tm * R;
+  const T *ap[NTL], *bp[NTL];
+  li_f32x4 acc[NTL][NTL];
+#pragma unroll
+  for (int i = 0; i < NTL; ++i) {
+    ap[i] = static_cast<const T*>(a.A) + (int64_t)min(m0 + 16 * i + l16, a.M - 1) * a.lda + quad * E;
+    bp[i] = static_cast<const T*>(a.B) + (int64_t)min(n0 + 16 * i + l16, a.N - 1) * a.ldb + quad * E;
+#pragma unroll
+    for (int j = 0; j < NTL; ++j) acc[i][j] = li_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int units = (a.K + UK - 1) / UK;
+  struct Unit { uint4 a[U][NTL], b[U][NTL]; } one, two;
+  auto load = [&](int u, Unit& f) {  // past the last unit: zeros
+    const int k = u * UK;
+    if (k + UK <= a.K) {
+#pragma unroll
+      for (int s = 0; s < U; ++s)
+#pragma unroll
+        for (int i = 0; i < NTL; ++i) {
+          __builtin_memcpy(&f.a[s][i], ap[i] + k + s * 4 * E, 16);
+          __builtin_memcpy(&f.b[s][i], bp[i] + k + s * 4 * E, 16);
+        }
+    } else {
+#pragma unroll
+      for (int s = 0; s < U; ++s)
+#pragma unroll
+        for (int i = 0; i < NTL; ++i) {
+          const int at = k + s * 4 * E;
+          f.a[s][i] = load_some<T>(ap[i] + at, a.K - at - quad * E);
+          f.b[s][i] = load_some<T>(bp[i] + at, a.K - at - quad * E);
+        }
+    }
+  };
+  auto add = [&](const Unit& f) {
+#pragma unroll
+    for (int s = 0; s < U; ++s)
+#pragma unroll
+      for (int i = 0; i < NTL; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) acc[i][j] = lmma16(f.b[s][j], f.a[s][i], acc[i][j], T());
+  };
+  int u = wave;
+  load(u, one);
+  for (; u < units; u += 2 * NW) {
+    load(u + NW, two);
+    add(one);
+    load(u + 2 * NW, one);
+    add(two);
+  }
+#pragma unroll
+  for (int i = 0; i < NTL; ++i)
+#pragma unroll
+    for (int j = 0; j < NTL; ++j) *reinterpret_cast<li_f32x4*>(&red[wave][16 * i + l16][16 * j + 4 * quad]) = acc[i][j];
+  __syncthreads();
+  for (int e = tid; e < R * R; e += NW * 64) {
+    const int i = e / R, j = e % R, m = m0 + i, n = n0 + j;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += red[w][i][j];
+    if (m < a.M && n < a.N) lin_finish<T>(a, m, n, v);
   }
 #endif
 }
@@ -824,7 +918,7 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(SumArgs a) {
 // ---------------------------------------------------------------------------------------------------------- host
 namespace {
 
-constexpr int kFewRows = 8;
+constexpr int kFewRows = 4;
 
 int lin_cus() {
   static thread_local int cached_dev = -1, cached = 0;
@@ -918,18 +1012,42 @@ int product(const LinArgs& a, int tile, hipStream_t st) {
   }
 }
 
+// Problems of few 64 x 64 tiles leave CUs idle while a long contraction goes by; then tiles of 16 or 32, whose contraction a
+// workgroup's waves share, are quicker.  A round of tiles over the CUs costs 10 (16 x 16), 21 (32 x 32) and 41 or, in float32, 72
+// (64 x 64): 40 rows of 4096 -> 1024 in bf16 take 9.6, 17 and 29 us, in float32 17, 33 and 101; 400 rows 52, 31 and 35 us.
+// -> 1 or 2 (tiles of 16 of a side), 0: the general kernel.  A larger tile is kept unless a tenth is gained.
+int shared_tiles(int64_t M, int64_t N, int cost64, int cus) {
+  auto cost = [&](int r, int round) { return ((M + r - 1) / r * ((N + r - 1) / r) + cus - 1) / cus * round; };
+  const int64_t c64 = cost(64, cost64), c32 = cost(32, 21), c16 = cost(16, 10);
+  const int ntl = c32 * 11 < c64 * 10 ? 2 : 0;
+  return c16 * 11 < (ntl ? c32 : c64) * 10 ? 1 : ntl;
+}
+template <typename T, int NTL>
+int launch_shared(const LinArgs& a, hipStream_t st) {
+  constexpr int R = 16 * NTL;
+  const int total = (a.M + R - 1) / R * ((a.N + R - 1) / R);  // below 4096: 128 x 128 tiles fill less than half of the CUs
+  linear_shared_kernel<T, NTL><<<dim3((total + 7) / 8 * 8), dim3(512), 0, st>>>(a);
+  EVE_CHECK_LAUNCH("eve_linear_fwd (shared contraction)");
+  return EVE_OK;
+}
+
 template <typename T>
 int fwd_typed(const LinArgs& a, hipStream_t st) {
   if (a.M <= kFewRows) {
     const dim3 grid((a.N + 3) / 4), block(256);
     if (a.M == 1) linear_few_kernel<T, 1><<<grid, block, 0, st>>>(a);
     else if (a.M == 2) linear_few_kernel<T, 2><<<grid, block, 0, st>>>(a);
-    else if (a.M <= 4) linear_few_kernel<T, 4><<<grid, block, 0, st>>>(a);
-    else linear_few_kernel<T, 8><<<grid, block, 0, st>>>(a);
+    else linear_few_kernel<T, 4><<<grid, block, 0, st>>>(a);
     EVE_CHECK_LAUNCH("eve_linear_fwd (few rows)");
     return EVE_OK;
   }
-  return product<T, false, false, LIN_FWD>(a, choose_tile(product_aligned(a, false, false, sizeof(T)), false, a.M, a.N, 1, lin_cus()), st);
+  const int tile = choose_tile(product_aligned(a, false, false, sizeof(T)), false, a.M, a.N, 1, lin_cus());
+  if (tile == -64) {
+    const int ntl = shared_tiles(a.M, a.N, sizeof(T) == 2 ? 41 : 72, lin_cus());
+    if (ntl == 1) return launch_shared<T, 1>(a, st);
+    if (ntl == 2) return launch_shared<T, 2>(a, st);
+  }
+  return product<T, false, false, LIN_FWD>(a, tile, st);
 }
 
 struct BwdPlan { int dz_rows, parts, nsplit, kspan; size_t dz, part_b, part_g, part_w, part_s, bytes; };

@@ -233,3 +233,20 @@ def test_other_stream_repeats_and_replays_are_bit_equal():
         eager = step(p, "quick_gelu", dout)
         torch.cuda.synchronize()
         assert all(torch.equal(held[n], eager[n]) for n in eager), i
+
+
+# few tiles and a long contraction (5 to some hundred rows; unaligned rows, tails of the contraction, one column), then problems of
+# enough tiles for the streaming kernels, their last rows, columns and contraction steps partly filled
+LONG = [(1, 5, 1000, 70), (2, 8, 2056, 24), (2, 20, 2049, 515), (1, 200, 1024, 1000), (3, 70, 301, 333), (1, 6, 31, 1), (2, 400, 2000, 260)]
+MANY = [(20, 400, 136, 520), (30, 500, 72, 1096), (9, 999, 200, 776)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", LONG + MANY, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("act", ["identity", "quick_gelu"])
+def test_long_contractions_and_many_tiles(size, act, dtype):
+    p, dout = make(*size, dtype, seed=sum(size) + 1)
+    ref = reference(p, act, dout)
+    with torch.no_grad():
+        assert_within({"y": call(p, act)}, ref, "without gradient")
+    assert_within(step(p, act, dout), ref, "with gradient")
