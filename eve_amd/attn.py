@@ -49,7 +49,7 @@ class _AttentionFn(torch.autograd.Function):
     def backward(ctx, dout):  # type: ignore[override]
         q, k, v, key_mask, out, lse = ctx.saved_tensors
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        ops.attn_bwd(dout.contiguous(), q, k, v, key_mask, out, lse, ctx.scale, dq, dk, dv)
+        ops.attn_bwd(ops.attn_dense(dout), q, k, v, key_mask, out, lse, ctx.scale, dq, dk, dv)
         return dq, dk, dv, None, None
 
 
@@ -71,7 +71,7 @@ class _SelfAttentionFn(torch.autograd.Function):
     def backward(ctx, dout):  # type: ignore[override]
         qkv, key_mask, out, lse = ctx.saved_tensors
         dqkv = qkv.new_empty(qkv.shape)
-        ops.attn_qkv_bwd(dout.contiguous(), qkv, key_mask, out, lse, ctx.scale, dqkv)
+        ops.attn_qkv_bwd(ops.attn_dense(dout), qkv, key_mask, out, lse, ctx.scale, dqkv)
         return dqkv, None, None
 
 

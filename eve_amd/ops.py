@@ -476,6 +476,12 @@ def attn_readable(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def attn_dense(t: torch.Tensor) -> torch.Tensor:
+    """`t` contiguous and on a 16-byte boundary (a contiguous part of another tensor may lie anywhere); else a copy."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def attn_fwd(q, k, v, key_mask, scale: float, want_lse: bool = True):
     """q [B,Nq,H,D]; k, v [B,Nk,Hkv,D] (attn_readable); key_mask [B,Nk] bool | None -> (out [B,Nq,H,D], lse [B,H,Nq] | None).
     The order inside lse is the kernels' own."""

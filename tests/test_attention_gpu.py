@@ -278,3 +278,20 @@ def test_offsets_beyond_32_bits():
     out = eve_amd.attention(*parts)
     grads = torch.autograd.grad(out, parts, do)
     assert_within(dict(zip(("out", "dq", "dk", "dv"), (out, *grads))), attention64(q, k, v, dout=do), "far rows")
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_gradient_that_starts_off_a_16_byte_boundary(packed):
+    """The gradient of a result that was concatenated behind something else is a contiguous part of a larger tensor, wherever that
+    starts; it gives what the same numbers give on a boundary."""
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn(2, 19, 3, 2, 16, generator=g).to(torch.bfloat16).to(DEV).requires_grad_(True)
+    dout = torch.randn(1 + 2 * 19 * 2 * 16, generator=g).to(torch.bfloat16).to(DEV)
+
+    def out():
+        return eve_amd.self_attention(qkv) if packed else eve_amd.attention(*qkv.unbind(2))
+
+    want, = torch.autograd.grad(out(), qkv, dout[1:].clone().view(2, 19, 2, 16))
+    joined = torch.cat((torch.zeros(1, dtype=torch.bfloat16, device=DEV), out().flatten()))
+    got, = torch.autograd.grad(joined, qkv, dout)
+    assert torch.equal(got, want)
