@@ -801,6 +801,7 @@ struct DzArgs {
   const void *dy, *z, *gamma, *row_scale;
   void* dz;                 // may be null (dz = dy)
   float *part_b, *part_g;   // [parts][N], either may be null
+  void *db, *dg;            // where there is one part: the column sums themselves, either may be null
   int M, N, rows_per_scale, act, rows;  // rows: of a block
 };
 template <typename T>
@@ -830,7 +831,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float du = dy[e] * rs;
-        if (a.part_g) sg[e] = fmaf(du, act_of<T>(z[e], a.act), sg[e]);
+        if (a.part_g || a.dg) sg[e] = fmaf(du, act_of<T>(z[e], a.act), sg[e]);
         dy[e] = du * gamma[e];
         if (a.act != EVE_ACT_IDENTITY) dy[e] *= act_slope<T>(z[e], a.act);
         sb[e] += dy[e];
@@ -857,6 +858,8 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
     }
     if (a.part_b) a.part_b[(int64_t)blockIdx.y * a.N + nc] = b;
     if (a.part_g) a.part_g[(int64_t)blockIdx.y * a.N + nc] = g;
+    if (a.db) static_cast<T*>(a.db)[nc] = from_f32<T>(b);
+    if (a.dg) static_cast<T*>(a.dg)[nc] = from_f32<T>(g);
   }
 #endif
 }
@@ -1055,7 +1058,7 @@ struct BwdPlan { int dz_rows, parts, nsplit, kspan; size_t dz, part_b, part_g, p
 BwdPlan bwd_plan(int rows, int K, int N, int dtype, int cus) {
   BwdPlan p;
   const size_t size = dtype == EVE_BF16 ? 2 : 4;
-  p.dz_rows = 32;  // (128 a block: 29 us for 15168 x 768 of bf16, too few workgroups)
+  p.dz_rows = rows <= 64 ? 64 : 32;  // (128 a block: 29 us for 15168 x 768 of bf16, too few workgroups); one part: no launch for sums
   while (ceil_div(rows, p.dz_rows) > 32768) p.dz_rows *= 2;
   p.parts = ceil_div(rows, p.dz_rows);
   // dW [N, K]: the contraction over the rows is split until there are about two tiles of 256 x 128 a CU, with 256 rows each at least
@@ -1090,9 +1093,12 @@ int bwd_typed(const DzArgs& dzin, const void* x, const void* w, void* dx, void* 
   const bool with_dw = plain && dbias && dw && !dgamma && tile_w > 0 && rows > 0 && N > 0 && K > 0;
   if (with_dw) w_.part_bias = reinterpret_cast<float*>(ws + p.part_s);
   d.dz = plain || !(dx || dw) ? nullptr : ws + p.dz;
-  d.part_b = dbias && !with_dw ? reinterpret_cast<float*>(ws + p.part_b) : nullptr;
-  d.part_g = dgamma ? reinterpret_cast<float*>(ws + p.part_g) : nullptr;
-  if (N > 0 && rows > 0 && (d.dz || d.part_b || d.part_g)) {
+  const bool direct = p.parts == 1 && !with_dw;
+  d.db = direct ? dbias : nullptr;
+  d.dg = direct ? dgamma : nullptr;
+  d.part_b = dbias && !with_dw && !direct ? reinterpret_cast<float*>(ws + p.part_b) : nullptr;
+  d.part_g = dgamma && !direct ? reinterpret_cast<float*>(ws + p.part_g) : nullptr;
+  if (N > 0 && rows > 0 && (d.dz || d.part_b || d.part_g || d.db || d.dg)) {
     linear_dz_kernel<T><<<dim3(ceil_div(N, 256), p.parts), dim3(256), 0, st>>>(d);
     EVE_CHECK_LAUNCH("eve_linear_bwd (dz)");
   }
@@ -1113,7 +1119,7 @@ int bwd_typed(const DzArgs& dzin, const void* x, const void* w, void* dx, void* 
     s.blocks_w = (int)((s.n_w + 1023) / 1024);
   }
   s.blocks_c = 1;
-  if (N > 0 && (dbias || dgamma)) {
+  if (N > 0 && (dbias || dgamma) && !direct) {
     s.part_c[0] = with_dw ? w_.part_bias : d.part_b; s.part_c[1] = d.part_g; s.dc[0] = dbias; s.dc[1] = dgamma;
     s.n_c = N; s.parts_c = with_dw ? p.nsplit : p.parts; s.blocks_c = ceil_div(N, 32);
   }

@@ -528,7 +528,7 @@ def _attn_fwd(dims, at, like, key_mask, scale, want_lse):
     nbytes = _lib.load().eve_attn_fwd_workspace_bytes(ref)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     PROFILE.call("eve_attn_fwd", ref, _lib.ctypes.addressof(layout), at[0][0], at[1][0], at[2][0], _p(key_mask), out.data_ptr(),
-                 _p(lse), _p(ws), nbytes, _stream(), tag=f"N={Nq}x{Nk}")
+                 _p(lse), _p(ws), nbytes, _stream(), tag=PROFILE.on and f"N={Nq}x{Nk}")
     return out, lse
 
 
@@ -542,38 +542,32 @@ def _attn_bwd(dims, at, dout, key_mask, out, lse, scale, grads_at):
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     PROFILE.call("eve_attn_bwd", ref, _lib.ctypes.addressof(layout), _lib.ctypes.addressof(grads), at[0][0], at[1][0], at[2][0],
                  _p(key_mask), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), grads_at[0][0], grads_at[1][0], grads_at[2][0],
-                 _p(ws), nbytes, _stream(), tag=f"N={dims[1]}x{dims[3]}")
+                 _p(ws), nbytes, _stream(), tag=PROFILE.on and f"N={dims[1]}x{dims[3]}")
 
 
 # ----------------------------------------------------------------------------- linear layer with its epilogue fused
 @_on_device_of(0)
 def linear_fwd(x, w, bias, gamma, row_scale, residual, rows_per_scale: int, act: int, save_z: bool = False):
     """x [S,K]; w [N,K]; bias, gamma [N] | None; row_scale [S / rows_per_scale] | None; residual [S,N] | None
-    -> (residual + row_scale * gamma * act(x w^T + bias) [S,N], z = x w^T + bias [S,N] | None)."""
-    dtype = x.dtype
-    for t, n in ((x, "x"), (w, "weight"), (bias, "bias"), (gamma, "gamma"), (row_scale, "row_scale"), (residual, "residual")):
-        if t is not None:
-            _chk(t, n, dtype)
+    -> (residual + row_scale * gamma * act(x w^T + bias) [S,N], z = x w^T + bias [S,N] | None).  All contiguous and of one type, as
+    fused_linear has seen to."""
     S, K = x.shape
     N = w.shape[0]
     y = x.new_empty((S, N))
     z = x.new_empty((S, N)) if save_z else None
     PROFILE.call("eve_linear_fwd", _p(x), _p(w), _p(bias), _p(gamma), _p(row_scale), _p(residual), _p(y), _p(z), S,
-                 rows_per_scale, K, N, act, _dt(x), _stream(), tag=f"{S}x{K}x{N}")
+                 rows_per_scale, K, N, act, _dt(x), _stream(), tag=PROFILE.on and f"{S}x{K}x{N}")
     return y, z
 
 
 @_on_device_of(0)
 def linear_bwd(dy, x, w, z, gamma, row_scale, rows_per_scale: int, act: int, want):
-    """-> (dx, dw, dbias, dgamma), None where `want` (four truth values) does not ask for one."""
-    for t, n in ((dy, "dy"), (w, "weight"), (z, "z"), (gamma, "gamma"), (row_scale, "row_scale")):
-        if t is not None:
-            _chk(t, n, x.dtype)
+    """-> (dx, dw, dbias, dgamma), None where `want` (four truth values) does not ask for one; arguments as linear_fwd's."""
     S, K = x.shape
     N = w.shape[0]
     outs = [x.new_empty(s) if yes else None for s, yes in zip(((S, K), (N, K), (N,), (N,)), want)]
     nbytes = _lib.load().eve_linear_bwd_workspace_bytes(S, K, N, _dt(x))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     PROFILE.call("eve_linear_bwd", _p(dy), _p(x), _p(w), _p(z), _p(gamma), _p(row_scale), *(_p(o) for o in outs), S,
-                 rows_per_scale, K, N, act, _dt(x), _p(ws), nbytes, _stream(), tag=f"{S}x{K}x{N}")
+                 rows_per_scale, K, N, act, _dt(x), _p(ws), nbytes, _stream(), tag=PROFILE.on and f"{S}x{K}x{N}")
     return outs
