@@ -1061,9 +1061,12 @@ BwdPlan bwd_plan(int rows, int K, int N, int dtype, int cus) {
   p.dz_rows = rows <= 64 ? 64 : 32;  // (128 a block: 29 us for 15168 x 768 of bf16, too few workgroups); one part: no launch for sums
   while (ceil_div(rows, p.dz_rows) > 32768) p.dz_rows *= 2;
   p.parts = ceil_div(rows, p.dz_rows);
-  // dW [N, K]: the contraction over the rows is split until there are about two tiles of 256 x 128 a CU, with 256 rows each at least
+  // dW [N, K]: the contraction over the rows is split until there is a tile of 256 x 128 a CU, if that leaves few idle, else about
+  // two a CU; 256 rows each at least.  15168 rows, 768 x 768 (18 tiles): 14 splits 30 us and 9 for the sums, 28 splits 30 and 11;
+  // 2304 x 768 (54 tiles): 9 splits 69 and 11 us, 4 splits 105 and 6.
   const int64_t tiles = (int64_t)ceil_div(N, 256) * ceil_div(K, 128);
-  int64_t want = tiles > 0 ? 2 * (int64_t)cus / tiles : 1;
+  int64_t want = tiles > 0 ? cus / tiles : 1;
+  if (want * tiles * 20 < (int64_t)cus * 19) want = tiles > 0 ? 2 * (int64_t)cus / tiles : 1;
   if (want > rows / 256) want = rows / 256;
   if (want < 1) want = 1;
   p.kspan = (int)align_up((size_t)((rows + want - 1) / want), 64);
