@@ -1058,7 +1058,11 @@ struct BwdPlan { int dz_rows, parts, nsplit, kspan; size_t dz, part_b, part_g, p
 BwdPlan bwd_plan(int rows, int K, int N, int dtype, int cus) {
   BwdPlan p;
   const size_t size = dtype == EVE_BF16 ? 2 : 4;
-  p.dz_rows = rows <= 64 ? 64 : 32;  // (128 a block: 29 us for 15168 x 768 of bf16, too few workgroups); one part: no launch for sums
+  // rows of a dz block: 32 (128: 29 us for 15168 x 768 of bf16, too few workgroups), fewer until there are four workgroups a CU
+  // (1899 x 1001 of float32: 32 rows 21.7 us, 8 rows 14.1); up to 64 rows are one part, which needs no launch for sums
+  p.dz_rows = 32;
+  while (p.dz_rows > 8 && (int64_t)ceil_div(N, 256) * ceil_div(rows, p.dz_rows) < 4 * (int64_t)cus) p.dz_rows /= 2;
+  if (rows <= 64) p.dz_rows = 64;
   while (ceil_div(rows, p.dz_rows) > 32768) p.dz_rows *= 2;
   p.parts = ceil_div(rows, p.dz_rows);
   // dW [N, K]: the contraction over the rows is split until there is a tile of 256 x 128 a CU, if that leaves few idle, else about
