@@ -60,12 +60,12 @@ template <typename T> struct AT;
 template <> struct AT<bf16_t> { static constexpr int E = 8; };
 template <> struct AT<float> { static constexpr int E = 4; };
 
-template <typename T, int DP> struct AttnCfg {
+template <typename T, int DP, bool LONG = false> struct AttnCfg {
   static constexpr int E = AT<T>::E;
   static constexpr int NKS = DP / (2 * E);              // contraction steps over the head width
   static constexpr int CPR = DP / E;                    // 16-byte chunks of a row
   static constexpr int RB = DP * (int)sizeof(T);        // bytes of a row: 128, 256 or 512
-  static constexpr int KT = RB == 128 ? 64 : 32;        // rows of a staged tile
+  static constexpr int KT = RB == 128 || LONG ? 64 : 32;  // rows of a staged tile
   static constexpr uint64_t kFull = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
   static constexpr int TILE = KT * RB;
   static constexpr int STAGE = 2 * TILE;                // keys and values, or queries and gradients
@@ -325,10 +325,13 @@ __device__ __forceinline__ void tiles_landed() { asm volatile("s_waitcnt vmcnt(0
 // Block: NW waves of 32 rows each; the key tiles are staged for all of them.
 // The bounds on waves keep the register budget at 256, where the compiler holds accumulators in plain registers: in the larger
 // budget it moves them to and from accumulation registers, a third of the instructions of the loop.
+// (bf16 of width 65 to 128: tiles of 64 keys, half as many waits: 36 us instead of 41 for 3 x 16 heads on 4, 1001 x 1001.  The
+// gradients' kernels gain nothing by them, float32 loses its splits, one wave a workgroup its place for three in a CU.)
+template <typename T, int DP, int NW> using FwdCfg = AttnCfg<T, DP, NW == 4 && sizeof(T) == 2 && DP == 128>;
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) == 2 ? 4 : 3) void attn_fwd_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using C = AttnCfg<T, DP>;
+  using C = FwdCfg<T, DP, NW>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, wave_u = __builtin_amdgcn_readfirstlane(wave);
   int head, blk, split;
@@ -526,9 +529,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 // Adds the splits of a gradient in their order: g = factor * sum_s part[head, s, row].  Four columns a thread; for dq a row is
 // query row / G of query head (key head) G + row % G, for dk and dv (G = 1) a key.
 struct AttnSum { const float* part; void* g; int64_t g_b, g_n, g_h; int64_t total; int Hkv, G, D, rows, nsplit; float factor; };
+struct AttnSums { AttnSum s[2]; };  // by blockIdx.y
 template <typename T>
-__global__ __launch_bounds__(256) void attn_sum_kernel(AttnSum a) {
+__global__ __launch_bounds__(256) void attn_sum_kernel(AttnSums sums) {
 #if defined(__HIP_DEVICE_COMPILE__)
+  const AttnSum a = sums.s[blockIdx.y];
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= a.total) return;
   const int cols = a.D / 4, d = (int)(i % cols) * 4;
@@ -1116,22 +1121,22 @@ AttnPlan plan_of(int64_t rows, int nw, int64_t heads, int64_t tiles, int64_t wan
 
 int64_t q_rows(const eve_attn_shape& s) { return (int64_t)s.Nq * (s.H / s.Hkv); }
 int tile_rows(const eve_attn_shape& s) { return s.dtype == EVE_BF16 && s.D <= 64 ? 64 : 32; }
-int64_t key_tiles(const eve_attn_shape& s) { return ((int64_t)s.Nk + tile_rows(s) - 1) / tile_rows(s); }
+int64_t tiles_of(int n, int rows) { return ((int64_t)n + rows - 1) / rows; }
 
 // Few rows against many keys: the key tiles are split until the launch fills the CUs, and the parts are joined.  Up to 64 rows a
 // head go to blocks of one wave, of which three fit a CU.
 AttnPlan fwd_plan(const eve_attn_shape& s, int cus) {
   const int nw = q_rows(s) <= 64 ? 1 : 4;
-  return plan_of(q_rows(s), nw, (int64_t)s.B * s.Hkv, key_tiles(s), (int64_t)cus * (nw == 4 ? 2 : 3), 4);
+  const int kt = nw == 4 && s.dtype == EVE_BF16 ? 64 : tile_rows(s);  // FwdCfg
+  return plan_of(q_rows(s), nw, (int64_t)s.B * s.Hkv, tiles_of(s.Nk, kt), (int64_t)cus * (nw == 4 ? 2 : 3), 4);
 }
 AttnPlan dq_plan(const eve_attn_shape& s, int cus) {
   const int nw = q_rows(s) <= 64 ? 1 : 4;
-  return plan_of(q_rows(s), nw, (int64_t)s.B * s.Hkv, key_tiles(s), (int64_t)cus * (nw == 4 ? 2 : 3), 4);
+  return plan_of(q_rows(s), nw, (int64_t)s.B * s.Hkv, tiles_of(s.Nk, tile_rows(s)), (int64_t)cus * (nw == 4 ? 2 : 3), 4);
 }
 // The row tiles are counted head by head of a group, as the kernel walks them.
 AttnPlan dkv_plan(const eve_attn_shape& s, int cus) {
-  const int kt = tile_rows(s);
-  return plan_of(s.Nk, 4, (int64_t)s.B * s.Hkv, ((int64_t)s.Nq + kt - 1) / kt * (s.H / s.Hkv), (int64_t)cus * 2, 4);
+  return plan_of(s.Nk, 4, (int64_t)s.B * s.Hkv, tiles_of(s.Nq, tile_rows(s)) * (s.H / s.Hkv), (int64_t)cus * 2, 4);
 }
 
 // The backward of whole heads, a workgroup each: where there is one for every other CU at least and their waves have keys.
@@ -1199,7 +1204,7 @@ AttnArgs base_args(const eve_attn_shape& s) {
 }
 
 // the ring, and behind it the mask's words or the rows' statistics
-template <typename T, int DP> constexpr int attn_lds() { return AttnCfg<T, DP>::NST * AttnCfg<T, DP>::STAGE + kBitTiles * 8; }
+template <typename C> constexpr int attn_lds() { return C::NST * C::STAGE + kBitTiles * 8; }
 template <typename T, int DP> constexpr int dkv_lds() { return AttnCfg<T, DP>::NST * (AttnCfg<T, DP>::STAGE + 1024); }
 
 int launch_attn(void (*kern)(AttnArgs), AttnArgs& a, int nw, int lds, hipStream_t st, const char* name) {
@@ -1225,7 +1230,8 @@ void use_plan(AttnArgs& a, const AttnPlan& p) {
 template <typename T, int DP>
 int fwd_typed(AttnArgs& a, const AttnPlan& p, hipStream_t st) {
   use_plan(a, p);
-  const int rc = launch_attn(p.nw == 1 ? attn_fwd_kernel<T, DP, 1> : attn_fwd_kernel<T, DP, 4>, a, p.nw, attn_lds<T, DP>(), st, "eve_attn_fwd");
+  const int rc = launch_attn(p.nw == 1 ? attn_fwd_kernel<T, DP, 1> : attn_fwd_kernel<T, DP, 4>, a, p.nw,
+                             p.nw == 1 ? attn_lds<FwdCfg<T, DP, 1>>() : attn_lds<FwdCfg<T, DP, 4>>(), st, "eve_attn_fwd");
   if (rc != EVE_OK || a.nsplit == 1) return rc;
   EVE_REQUIRE((int64_t)a.heads * a.rows <= 0x7fffffffLL, EVE_ERR_UNSUPPORTED, "eve_attn_fwd: too many rows");
   attn_join_kernel<T><<<dim3((unsigned)(a.heads * a.rows)), dim3(256), 0, st>>>(a);
@@ -1233,12 +1239,14 @@ int fwd_typed(AttnArgs& a, const AttnPlan& p, hipStream_t st) {
   return EVE_OK;
 }
 
+AttnSum sum_of(const AttnArgs& a, const float* part, void* g, int64_t g_b, int64_t g_n, int64_t g_h, int G, int rows, float factor) {
+  return {part, g, g_b, g_n, g_h, (int64_t)a.heads * rows * (a.D / 4), a.Hkv, G, a.D, rows, a.nsplit, factor};
+}
 template <typename T>
-int sum_parts(const AttnArgs& a, const float* part, void* g, int64_t g_b, int64_t g_n, int64_t g_h, int G, int rows, float factor, hipStream_t st) {
-  AttnSum s = {part, g, g_b, g_n, g_h, (int64_t)a.heads * rows * (a.D / 4), a.Hkv, G, a.D, rows, a.nsplit, factor};
-  const int64_t grid = (s.total + 255) / 256;
+int sum_parts(const AttnSums& s, int n, hipStream_t st) {  // n of one size
+  const int64_t grid = (s.s[0].total + 255) / 256;
   EVE_REQUIRE(grid <= 0x7fffffffLL, EVE_ERR_UNSUPPORTED, "eve_attn_bwd: too many rows");
-  attn_sum_kernel<T><<<dim3((unsigned)grid), dim3(256), 0, st>>>(s);
+  attn_sum_kernel<T><<<dim3((unsigned)grid, n), dim3(256), 0, st>>>(s);
   EVE_CHECK_LAUNCH("eve_attn_bwd (sum of the splits)");
   return EVE_OK;
 }
@@ -1253,18 +1261,17 @@ int bwd_typed(AttnArgs& a, bool whole, const AttnPlan& pq, const AttnPlan& pk, h
   }
   if (a.rows > 0) {
     use_plan(a, pq);
-    int rc = launch_attn(pq.nw == 1 ? attn_dq_kernel<T, DP, 1> : attn_dq_kernel<T, DP, 4>, a, pq.nw, attn_lds<T, DP>(), st, "eve_attn_bwd (dq)");
+    int rc = launch_attn(pq.nw == 1 ? attn_dq_kernel<T, DP, 1> : attn_dq_kernel<T, DP, 4>, a, pq.nw, attn_lds<AttnCfg<T, DP>>(), st, "eve_attn_bwd (dq)");
     if (rc == EVE_OK && a.nsplit > 1)
-      rc = sum_parts<T>(a, a.part_a, a.dq, a.grad.q_b, a.grad.q_n, a.grad.q_h, a.G, a.rows, a.scale, st);
+      rc = sum_parts<T>({{sum_of(a, a.part_a, a.dq, a.grad.q_b, a.grad.q_n, a.grad.q_h, a.G, a.rows, a.scale)}}, 1, st);
     if (rc != EVE_OK) return rc;
   }
   if (a.Nk == 0) return EVE_OK;
   use_plan(a, pk);
   int rc = launch_attn(attn_dkv_kernel<T, DP, 4>, a, pk.nw, dkv_lds<T, DP>(), st, "eve_attn_bwd (dk, dv)");
   if (rc == EVE_OK && a.nsplit > 1)
-    rc = sum_parts<T>(a, a.part_a, a.dk, a.grad.k_b, a.grad.k_n, a.grad.k_h, 1, a.Nk, a.scale, st);
-  if (rc == EVE_OK && a.nsplit > 1)
-    rc = sum_parts<T>(a, a.part_b, a.dv, a.grad.v_b, a.grad.v_n, a.grad.v_h, 1, a.Nk, 1.f, st);
+    rc = sum_parts<T>({{sum_of(a, a.part_a, a.dk, a.grad.k_b, a.grad.k_n, a.grad.k_h, 1, a.Nk, a.scale),
+                        sum_of(a, a.part_b, a.dv, a.grad.v_b, a.grad.v_n, a.grad.v_h, 1, a.Nk, 1.f)}}, 2, st);
   return rc;
 }
 
