@@ -21,7 +21,8 @@
 // ahead of the one that is worked on.  A masked row is an offset outside the descriptor, for which the hardware delivers zeros.
 // The 16-byte chunks of a row are permuted (AttnCfg::swizzle) -- on the source side, since the transfer writes LDS in lane order --
 // so that both ways of reading, row fragments and transposed ones, spread over all banks.
-// No atomics: dq and dk/dv have a kernel each (7 products instead of 5), so results do not depend on the order of execution.
+// No atomics: dq and dk/dv have a kernel each (7 products instead of 5), or one workgroup has a head's whole backward, so results do
+// not depend on the order of execution.
 #include <math.h>
 
 #include <type_traits>
@@ -323,6 +324,10 @@ __device__ __forceinline__ void tiles_landed() { asm volatile("s_waitcnt vmcnt(0
 
 // ---------------------------------------------------------------------------------------------------------- forward
 // Block: NW waves of 32 rows each; the key tiles are staged for all of them.
+// Bound: the matrix unit and the vector unit, which hardly overlap in a CU: of a 64-key tile's 1400 cycles a wave the matrix unit
+// has 512, the vector unit 870 (the exponentials alone 530).  64 x 12 heads of 617 x 617: 121 us (620 TFLOP/s); 2 x 16 heads of
+// 4096 x 4096: 171 us (800), of width 128: 283 us (970).  One query of 4 x 16 heads on 4 over 16384 keys (NW = 1, 47 splits): 25 us,
+// 5.3 TB/s, the memory's rate.
 // The bounds on waves keep the register budget at 256, where the compiler holds accumulators in plain registers: in the larger
 // budget it moves them to and from accumulation registers, a third of the instructions of the loop.
 // (bf16 of width 65 to 128: tiles of 64 keys, half as many waits: 36 us instead of 41 for 3 x 16 heads on 4, 1001 x 1001.  The
@@ -574,6 +579,7 @@ __device__ __forceinline__ uint4 row_stats(float L, float delta, float inv_c) {
 
 // The forward's shape: columns are query rows, the key tiles pass by (or a split of them).  Also forms delta_i for the dk/dv
 // kernel.  -delta is the accumulator that the product do v^T starts from.
+// Bound as the forward (matrix unit 43 % busy, vector unit 47 %).  2 x 16 heads of 4096 x 4096: 240 us (860 TFLOP/s).
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ? 1 : sizeof(T) == 2 && DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -699,6 +705,9 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
 // p = 2^(c acc), ds = p acc'.  These terms are themselves a matrix product: a row's 16 bytes hold both values as three bf16 each
 // (exactly, 24 bits), which multiply ones; read as values, four at a time, they would be a third of the loop's LDS traffic.
 // A row past the end is all zeros: p = 1 there, and its q and do, which p and ds multiply, are zero.
+// Bound as the forward (matrix unit 51 % busy, vector unit 44 %).  2 x 16 heads of 4096 x 4096: 307 us (900 TFLOP/s); three
+// waves a SIMD instead of two change nothing.  Few live blocks (3 samples of 0 to 1001 keys, 16 heads on 4, width 128: 77 us) are
+// bound by a tile's way through the CU, 2.2 us.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -878,6 +887,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 // operand read once.  ds is exchanged between the waves through LDS as [key][64 rows]; a wave then multiplies one 32 x 32 block of
 // dq^T = k^T ds^T over half of the keys, and the two halves are added in a fixed order.  delta is formed from do and o by the
 // threads that a tile's rows are dealt to, one tile ahead.
+// Bound: latency.  64 x 12 heads of 237 x 237 take 82 us, the matrix unit is busy for 19 % of it: with 114 KiB and 226 registers a
+// CU holds one workgroup, and a head costs 11 k cycles before its first tile, then four times 7 k between two barriers each.
 __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef bf16_t T;
