@@ -437,12 +437,28 @@ def _on_device_of(which: int):
         @wraps(f)
         def on_device(*args, **kwargs):
             device = args[which].get_device()
+            if device < 0:
+                raise RuntimeError(f"eve_amd: {f.__name__} must be given GPU tensors; there is no CPU path")
             if device == torch.cuda.current_device():
                 return f(*args, **kwargs)
             with torch.cuda.device(device):
                 return f(*args, **kwargs)
         return on_device
     return wrap
+
+
+def _chk_all(like: torch.Tensor, **tensors):
+    """_chk of several at once, None among them: contiguous, of one type and on one device with `like`."""
+    dtype, device = like.dtype, like.device
+    for name, t in tensors.items():
+        if t is not None and not (t.dtype == dtype and t.device == device and t.is_contiguous()):
+            _chk(t, name, dtype)
+            raise RuntimeError(f"eve_amd: `{name}` is on {t.device}, not on {device}")
+
+
+def _chk_parts(q, k, v):
+    if k.device != q.device or v.device != q.device or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise RuntimeError("eve_amd: q, k and v must be on one device and of one type")
 
 
 def _attn_at(t: torch.Tensor):
@@ -485,6 +501,7 @@ def attn_dense(t: torch.Tensor) -> torch.Tensor:
 def attn_fwd(q, k, v, key_mask, scale: float, want_lse: bool = True):
     """q [B,Nq,H,D]; k, v [B,Nk,Hkv,D] (attn_readable); key_mask [B,Nk] bool | None -> (out [B,Nq,H,D], lse [B,H,Nq] | None).
     The order inside lse is the kernels' own."""
+    _chk_parts(q, k, v)
     return _attn_fwd((*q.shape[:3], *k.shape[1:]), (_attn_at(q), _attn_at(k), _attn_at(v)), q, key_mask, scale, want_lse)
 
 
@@ -496,6 +513,7 @@ def attn_qkv_fwd(qkv, key_mask, scale: float, want_lse: bool = True):
 
 def attn_bwd(dout, q, k, v, key_mask, out, lse, scale: float, dq, dk, dv) -> None:
     """Writes the gradients into dq, dk, dv, which have q's, k's, v's shapes and lie as attn_readable says."""
+    _chk_parts(q, k, v), _chk_parts(out, q, k), _chk_parts(q, dq, dk), _chk_parts(q, dq, dv)
     _attn_bwd((*q.shape[:3], *k.shape[1:]), (_attn_at(q), _attn_at(k), _attn_at(v)), dout, key_mask, out, lse, scale,
               (_attn_at(dq), _attn_at(dk), _attn_at(dv)))
 
@@ -549,8 +567,8 @@ def _attn_bwd(dims, at, dout, key_mask, out, lse, scale, grads_at):
 @_on_device_of(0)
 def linear_fwd(x, w, bias, gamma, row_scale, residual, rows_per_scale: int, act: int, save_z: bool = False):
     """x [S,K]; w [N,K]; bias, gamma [N] | None; row_scale [S / rows_per_scale] | None; residual [S,N] | None
-    -> (residual + row_scale * gamma * act(x w^T + bias) [S,N], z = x w^T + bias [S,N] | None).  All contiguous and of one type, as
-    fused_linear has seen to."""
+    -> (residual + row_scale * gamma * act(x w^T + bias) [S,N], z = x w^T + bias [S,N] | None)."""
+    _chk_all(x, x=x, weight=w, bias=bias, gamma=gamma, row_scale=row_scale, residual=residual)
     S, K = x.shape
     N = w.shape[0]
     y = x.new_empty((S, N))
@@ -562,7 +580,8 @@ def linear_fwd(x, w, bias, gamma, row_scale, residual, rows_per_scale: int, act:
 
 @_on_device_of(0)
 def linear_bwd(dy, x, w, z, gamma, row_scale, rows_per_scale: int, act: int, want):
-    """-> (dx, dw, dbias, dgamma), None where `want` (four truth values) does not ask for one; arguments as linear_fwd's."""
+    """-> (dx, dw, dbias, dgamma), None where `want` (four truth values) does not ask for one."""
+    _chk_all(x, dy=dy, x=x, weight=w, z=z, gamma=gamma, row_scale=row_scale)
     S, K = x.shape
     N = w.shape[0]
     outs = [x.new_empty(s) if yes else None for s, yes in zip(((S, K), (N, K), (N,), (N,)), want)]

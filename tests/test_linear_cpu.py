@@ -44,3 +44,15 @@ def test_c_entry_points_answer_bad_calls_with_codes():
     assert lib.eve_linear_bwd_workspace_bytes(4, 8, 8, 0) > 0
     assert bwd() == -2 and bwd(ws=16, n=8) == -2 and bwd(dy=None) == -1
     assert bwd(act=0, ws=16, n=1 << 20) == -1 and bwd(dg=16, ws=16, n=1 << 20) == -1  # both need z
+
+
+def test_the_wrappers_refuse_cpu_tensors():
+    from eve_amd import ops
+    x, w = torch.zeros(2, 8), torch.zeros(4, 8)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.linear_fwd(x, w, None, None, None, None, 1, ops.ACTS["identity"])
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.linear_bwd(torch.zeros(2, 4), x, w, None, None, None, 1, ops.ACTS["identity"], (True, True, False, False))
+    q = torch.zeros(1, 2, 1, 8)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.attn_fwd(q, q, q, None, 1.0)
