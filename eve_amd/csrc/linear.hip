@@ -16,7 +16,7 @@
 // quick_gelu, gamma and residual; the matrix unit is busy for 40 % of the cycles (a step takes 1070 for 768, a tile's epilogue 11 k
 // of 50 k), the clock falls to 1.6 GHz.  Reading fragments half a step ahead and 256-row tiles gained nothing.
 // linear_tile_kernel: any size and alignment, and small problems; tiles of 128 or 64, staged through registers with every element
-// outside an operand replaced by zero.  Bound: latency and the matrix unit, a half each (float32, 1899 x 750 -> 1001: 48 us, 59 of
+// outside an operand replaced by zero.  Bound: latency and the matrix unit, a half each (float32, 1899 x 750 -> 1001: 46 us, 62 of
 // 138 TFLOP/s; the vendor library's product 35).
 // linear_few_kernel (up to 4 rows) and linear_shared_kernel (few tiles, a long contraction): bound by a launch and the weight's way.
 // dW has few tiles and a long contraction (the rows of the batch): it is split, with fp32 parts added in order.
@@ -29,6 +29,7 @@ typedef __attribute__((ext_vector_type(8))) __bf16 li_bf16x8;
 typedef __attribute__((ext_vector_type(4))) short li_s16x4;
 typedef __attribute__((ext_vector_type(8))) short li_s16x8;
 typedef __attribute__((ext_vector_type(16))) float li_f32x16;
+typedef __attribute__((ext_vector_type(4))) float li_f32x4;
 
 enum { LIN_FWD = 0, LIN_PLAIN = 1, LIN_PART = 2 };
 constexpr int kActRuntime = -1;  // the activation is LinArgs::act
@@ -123,16 +124,16 @@ template <typename T> __device__ __forceinline__ void store_some(T* p, const uin
 }
 
 // a tile on its way to LDS through registers
-template <typename T, bool COL, int W> struct LinTile {
+template <typename T, bool COL, int W, int TH> struct LinTile {
   static constexpr int E = LT<T>::E, BK = LT<T>::BK;
   static constexpr int BYTES = W * 128;
-  static constexpr int N = BYTES / 16 / 256;
+  static constexpr int N = BYTES / 16 / TH;
   uint4 w[N];
   // ext: rows (columns) of the operand from the tile's first on; kext: contraction indices from the step's first on
   __device__ __forceinline__ void load(const T* p, int64_t ld, int ext, int kext, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * 256;
+      const int idx = tid + i * TH;
       if constexpr (!COL) {
         const int r = idx >> 3, c = (idx & 7) * E;
         w[i] = r < ext ? load_some<T>(p + r * ld + c, kext - c) : make_uint4(0, 0, 0, 0);
@@ -146,7 +147,7 @@ template <typename T, bool COL, int W> struct LinTile {
   __device__ __forceinline__ void store(char* tile, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * 256;
+      const int idx = tid + i * TH;
       if constexpr (!COL) {
         *reinterpret_cast<uint4*>(tile + row_off(idx >> 3, idx & 7)) = w[i];
       } else {
@@ -351,14 +352,17 @@ __device__ __forceinline__ void lin_epilogue(const li_f32x16 (&acc)[NTM][NTN], c
 }
 #endif
 
-// BT x BT tile, 4 waves of (BT/2) x (BT/2); two LDS stages, the next two steps' tiles in registers meanwhile.
+// BT x BT tile, 4 waves of (BT/2) x (BT/2); two LDS stages, the next two steps' tiles in registers meanwhile.  BT = 64: twice the
+// waves, half of a step's contraction each, added at the end (float32, 1899 x 750 -> 1001: 46 us instead of 48; bf16, 617 x
+// 4096 -> 1024: 31 instead of 35).
+template <int BT> constexpr int tile_threads() { return BT == 64 ? 512 : 256; }
 template <typename T, int BT, bool ACOL, bool BCOL, int MODE>
-__global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
+__global__ __launch_bounds__(tile_threads<BT>()) void linear_tile_kernel(LinArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int BK = LT<T>::BK, E = LT<T>::E, NT = BT / 64, NKS = BK / (2 * E);
+  constexpr int BK = LT<T>::BK, E = LT<T>::E, NT = BT / 64, TH = tile_threads<BT>(), SHARE = TH / 256, NKS = BK / (2 * E) / SHARE;
   constexpr int STAGE = 2 * BT * 128;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
+  const int tid = threadIdx.x, lane = tid & 63, wave = (tid >> 6) & 3, share = tid >> 8, wm = wave >> 1, wn = wave & 1;
   // Workgroups go round-robin over the 8 XCDs: each of them gets a run of tiles, columns fastest, so that the tiles it works on
   // at a time share a few row panels of A through its L2.
   const int tm = (a.M + BT - 1) / BT, tn = (a.N + BT - 1) / BT, total = tm * tn * a.nsplit;
@@ -382,8 +386,8 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  LinTile<T, ACOL, BT> ta[2];
-  LinTile<T, BCOL, BT> tb[2];
+  LinTile<T, ACOL, BT, TH> ta[2];
+  LinTile<T, BCOL, BT, TH> tb[2];
   const int steps = (k1 - k0 + BK - 1) / BK;
   auto fetch = [&](int t, int i) {  // past the last step: zeros
     ta[i].load(Ap + t * sa, a.lda, a.M - m0, k1 - k0 - t * BK, tid);
@@ -404,9 +408,9 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
       for (int ks = 0; ks < NKS; ++ks) {
         uint4 fa[NT], fb[NT];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) fa[i] = lfrag<T, ACOL, BT>(as, wm * (BT / 2) + 32 * i, ks, lane);
+        for (int i = 0; i < NT; ++i) fa[i] = lfrag<T, ACOL, BT>(as, wm * (BT / 2) + 32 * i, share * NKS + ks, lane);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) fb[j] = lfrag<T, BCOL, BT>(bs, wn * (BT / 2) + 32 * j, ks, lane);
+        for (int j = 0; j < NT; ++j) fb[j] = lfrag<T, BCOL, BT>(bs, wn * (BT / 2) + 32 * j, share * NKS + ks, lane);
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -415,7 +419,23 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinArgs a) {
     }
   }
   __syncthreads();  // the stages become the waves' epilogue images
-
+  if constexpr (SHARE == 2) {
+    static_assert(NT == 1, "one accumulator");
+    li_f32x4* part = reinterpret_cast<li_f32x4*>(smem) + (wave * 4) * 64 + lane;
+    if (share == 1) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) part[g * 64] = li_f32x4{acc[0][0][4 * g], acc[0][0][4 * g + 1], acc[0][0][4 * g + 2], acc[0][0][4 * g + 3]};
+    }
+    __syncthreads();
+    if (share == 0) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[0][0][4 * g + r] += part[g * 64][r];
+    }
+    __syncthreads();
+    if (share == 1) return;
+  }
   lin_epilogue<T, BT / 2, NT, NT, MODE, kActRuntime, false>(acc, smem, a, split, m0 + wm * (BT / 2), n0 + wn * (BT / 2), wave, lane);
 #endif
 }
@@ -714,7 +734,6 @@ __global__ __launch_bounds__(256) void linear_few_kernel(LinArgs a) {
 // Tile: R x R with R = 16 NTL.  Fragments come from memory as they are (16 rows by 64 bytes, neighbouring lines in the next steps of
 // a wave), one unit of U steps ahead; a row past the end is the last one again, whose results are not kept.
 #if defined(__HIP_DEVICE_COMPILE__)
-typedef __attribute__((ext_vector_type(4))) float li_f32x4;
 __device__ __forceinline__ li_f32x4 lmma16(const uint4& a, const uint4& b, li_f32x4 acc, bf16_t) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(li_bf16x8, a), __builtin_bit_cast(li_bf16x8, b), acc, 0, 0, 0);
 }
@@ -951,11 +970,16 @@ int check_dims(int rows, int T, int K, int N, int act, int dtype) {
 // Which kernel a product runs on: the rows of the streaming kernel's tile, or (negative) the edge of the general one's.
 // The streaming kernel wants 16-byte rows.  Its tile -- 192 rows (256 of a k-major A) or 128, which has 15 % more LDS traffic a row --
 // is the one whose fullest CU has less to do: 15168 x 768 is 474 tiles of 192 rows (64 us for a contraction of 2304), 714 of 128
-// (70 us), 360 of 256 (74 us: two on some CUs, one on others).  Problems of fewer tiles go to the general kernel's 64 x 64 tiles.
+// (70 us), 360 of 256 (74 us: two on some CUs, one on others).  Problems of fewer tiles go to the general kernel's 64 x 64 tiles;
+// in float32, which the matrix unit bounds, wherever the CUs have less to do so (400 rows of 1024 -> 4096: 44 us instead of 71).
 bool rows16(const void* p, int ld, int size) { return ((uintptr_t)p & 15) == 0 && (int64_t)ld * size % 16 == 0 && ld < (1 << 20); }
-int choose_tile(bool aligned, bool acol, int64_t M, int64_t N, int64_t splits, int cus) {
+int choose_tile(bool aligned, bool acol, int64_t M, int64_t N, int64_t splits, int size, int cus) {
   const int64_t tn = (N + 127) / 128 * splits;
   if ((M + 127) / 128 * tn < cus / 2) return -64;
+  if (size == 4 && !acol) {
+    const int64_t n64 = (M + 63) / 64 * ((N + 63) / 64), n128 = (M + 127) / 128 * tn;
+    if ((n64 > cus ? n64 : cus) * 29 < (n128 > cus ? n128 : cus) * 67) return -64;
+  }
   if (!aligned) return -128;
   const int large = acol ? 256 : 192;
   const int64_t n_large = (M + large - 1) / large * tn, n_small = (M + 127) / 128 * tn;
@@ -972,7 +996,7 @@ int launch_tile(const LinArgs& a, hipStream_t st) {
   const int64_t total = (int64_t)((a.M + BT - 1) / BT) * ((a.N + BT - 1) / BT) * a.nsplit;
   EVE_REQUIRE(total <= 0x7ffffff0LL, EVE_ERR_UNSUPPORTED, "eve_linear: too many tiles");
   constexpr int lds = 2 * 2 * BT * 128 > 4 * 32 * (BT / 2 + 4) * 4 ? 2 * 2 * BT * 128 : 4 * 32 * (BT / 2 + 4) * 4;
-  linear_tile_kernel<T, BT, ACOL, BCOL, MODE><<<dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), lds, st>>>(a);
+  linear_tile_kernel<T, BT, ACOL, BCOL, MODE><<<dim3((unsigned)((total + 7) / 8 * 8)), dim3(tile_threads<BT>()), lds, st>>>(a);
   EVE_CHECK_LAUNCH("eve_linear (product)");
   return EVE_OK;
 }
@@ -1020,11 +1044,16 @@ int product(const LinArgs& a, int tile, hipStream_t st) {
 }
 
 // Problems of few 64 x 64 tiles leave CUs idle while a long contraction goes by; then tiles of 16 or 32, whose contraction a
-// workgroup's waves share, are quicker.  A round of tiles over the CUs costs 10 (16 x 16), 21 (32 x 32) and 41 or, in float32, 72
-// (64 x 64): 40 rows of 4096 -> 1024 in bf16 take 9.6, 17 and 29 us, in float32 17, 33 and 101; 400 rows 52, 31 and 35 us.
+// workgroup's waves share, are quicker.  A tile takes a CU 10 (16 x 16), 21 (32 x 32) and 41 or, in float32, 72 (64 x 64); a launch
+// takes its tiles over the CUs, one tile at least (32 x 32: whole rounds, as two at a time on a CU gain it nothing): 40 rows of 4096 -> 1024 in bf16 take 9.6, 17 and 29 us, in float32 17, 33 and 101;
+// 400 rows 52, 31 and 31 us; 617 rows of 768 -> 2304 in float32 65, 47 and 35.
 // -> 1 or 2 (tiles of 16 of a side), 0: the general kernel.  A larger tile is kept unless a tenth is gained.
 int shared_tiles(int64_t M, int64_t N, int cost64, int cus) {
-  auto cost = [&](int r, int round) { return ((M + r - 1) / r * ((N + r - 1) / r) + cus - 1) / cus * round; };
+  auto cost = [&](int r, int tile) {
+    const int64_t n = ((M + r - 1) / r) * ((N + r - 1) / r);
+    if (r == 32) return (n + cus - 1) / cus * cus * tile;
+    return (n > cus ? n : cus) * tile;
+  };
   const int64_t c64 = cost(64, cost64), c32 = cost(32, 21), c16 = cost(16, 10);
   const int ntl = c32 * 11 < c64 * 10 ? 2 : 0;
   return c16 * 11 < (ntl ? c32 : c64) * 10 ? 1 : ntl;
@@ -1048,7 +1077,7 @@ int fwd_typed(const LinArgs& a, hipStream_t st) {
     EVE_CHECK_LAUNCH("eve_linear_fwd (few rows)");
     return EVE_OK;
   }
-  const int tile = choose_tile(product_aligned(a, false, false, sizeof(T)), false, a.M, a.N, 1, lin_cus());
+  const int tile = choose_tile(product_aligned(a, false, false, sizeof(T)), false, a.M, a.N, 1, sizeof(T), lin_cus());
   if (tile == -64) {
     const int ntl = shared_tiles(a.M, a.N, sizeof(T) == 2 ? 41 : 72, lin_cus());
     if (ntl == 1) return launch_shared<T, 1>(a, st);
@@ -1069,12 +1098,13 @@ BwdPlan bwd_plan(int rows, int K, int N, int dtype, int cus) {
   if (rows <= 64) p.dz_rows = 64;
   while (ceil_div(rows, p.dz_rows) > 32768) p.dz_rows *= 2;
   p.parts = ceil_div(rows, p.dz_rows);
-  // dW [N, K]: the contraction over the rows is split until there is a tile of 256 x 128 a CU, if that leaves few idle, else about
-  // two a CU; 256 rows each at least.  15168 rows, 768 x 768 (18 tiles): 14 splits 30 us and 9 for the sums, 28 splits 30 and 11;
-  // 2304 x 768 (54 tiles): 9 splits 69 and 11 us, 4 splits 105 and 6.
+  // dW [N, K]: the contraction over the rows is split until there are about two tiles of 256 x 128 a CU, 256 rows each at least; one
+  // a CU if that leaves few idle and no more than 1280 rows a split, where the parts cost more than the company on a CU gives.  15168
+  // rows, 768 x 768 (18 tiles): 14 splits 30 us and 9 for the sums, 28 splits 30 and 11; 2304 x 768 (54): 4 splits 105 and 6 us,
+  // 9 splits 69 and 11; 8000 rows, 2047 x 1023 (64): 4 splits 215 us in all, 8 splits 180.
   const int64_t tiles = (int64_t)ceil_div(N, 256) * ceil_div(K, 128);
   int64_t want = tiles > 0 ? cus / tiles : 1;
-  if (want * tiles * 20 < (int64_t)cus * 19) want = tiles > 0 ? 2 * (int64_t)cus / tiles : 1;
+  if (want * tiles * 20 < (int64_t)cus * 19 || rows > 1280 * want) want = tiles > 0 ? 2 * (int64_t)cus / tiles : 1;
   if (want > rows / 256) want = rows / 256;
   if (want < 1) want = 1;
   p.kspan = (int)align_up((size_t)((rows + want - 1) / want), 64);
@@ -1099,7 +1129,7 @@ int bwd_typed(const DzArgs& dzin, const void* x, const void* w, void* dx, void* 
   LinArgs w_ = {};
   w_.A = plain ? d.dy : ws + p.dz; w_.B = x; w_.C = dw; w_.M = N; w_.N = K; w_.K = rows; w_.lda = N; w_.ldb = K;
   w_.nsplit = p.nsplit; w_.kspan = p.kspan; w_.part = reinterpret_cast<float*>(ws + p.part_w);
-  const int tile_w = choose_tile(product_aligned(w_, true, true, sizeof(T)), true, N, K, p.nsplit, lin_cus());
+  const int tile_w = choose_tile(product_aligned(w_, true, true, sizeof(T)), true, N, K, p.nsplit, sizeof(T), lin_cus());
   // dz = dy: dbias is summed by the dW product while it has dy in registers, where the streaming kernel runs it
   const bool with_dw = plain && dbias && dw && !dgamma && tile_w > 0 && rows > 0 && N > 0 && K > 0;
   if (with_dw) w_.part_bias = reinterpret_cast<float*>(ws + p.part_s);
@@ -1117,7 +1147,7 @@ int bwd_typed(const DzArgs& dzin, const void* x, const void* w, void* dx, void* 
   if (dx && rows > 0 && K > 0) {
     LinArgs a = {};
     a.A = dz; a.B = w; a.C = dx; a.M = rows; a.N = K; a.K = N; a.lda = N; a.ldb = K; a.nsplit = 1;
-    const int rc = product<T, false, true, LIN_PLAIN>(a, choose_tile(product_aligned(a, false, true, sizeof(T)), false, rows, K, 1, lin_cus()), st);
+    const int rc = product<T, false, true, LIN_PLAIN>(a, choose_tile(product_aligned(a, false, true, sizeof(T)), false, rows, K, 1, sizeof(T), lin_cus()), st);
     if (rc != EVE_OK) return rc;
   }
   if (dw && N > 0 && K > 0) {
