@@ -1102,9 +1102,12 @@ BwdPlan bwd_plan(int rows, int K, int N, int dtype, int cus) {
   // a CU if that leaves few idle and no more than 1280 rows a split, where the parts cost more than the company on a CU gives.  15168
   // rows, 768 x 768 (18 tiles): 14 splits 30 us and 9 for the sums, 28 splits 30 and 11; 2304 x 768 (54): 4 splits 105 and 6 us,
   // 9 splits 69 and 11; 8000 rows, 2047 x 1023 (64): 4 splits 215 us in all, 8 splits 180.
-  const int64_t tiles = (int64_t)ceil_div(N, 256) * ceil_div(K, 128);
+  // (Float32 off 16-byte boundaries goes by its tiles of 128 x 128, as the matrix unit bounds it: 1899 rows, 1001 x 750: 5 splits 45 us
+  // and 8, 6 splits 55 and 9; 8000 rows, 2047 x 1023: 4 splits 337 us in all, 8 splits 368.)
+  const bool large = size == 2 || ((size_t)N * size % 16 == 0 && (size_t)K * size % 16 == 0);
+  const int64_t tiles = (int64_t)ceil_div(N, large ? 256 : 128) * ceil_div(K, 128);
   int64_t want = tiles > 0 ? cus / tiles : 1;
-  if (want * tiles * 20 < (int64_t)cus * 19 || rows > 1280 * want) want = tiles > 0 ? 2 * (int64_t)cus / tiles : 1;
+  if (want * tiles * 16 < (int64_t)cus * 15 || rows > 1280 * want) want = tiles > 0 ? 2 * (int64_t)cus / tiles : 1;
   if (want > rows / 256) want = rows / 256;
   if (want < 1) want = 1;
   p.kspan = (int)align_up((size_t)((rows + want - 1) / want), 64);
