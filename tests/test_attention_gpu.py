@@ -295,3 +295,36 @@ def test_gradient_that_starts_off_a_16_byte_boundary(packed):
     joined = torch.cat((torch.zeros(1, dtype=torch.bfloat16, device=DEV), out().flatten()))
     got, = torch.autograd.grad(joined, qkv, dout)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", ["tail", "head", "one"])
+@pytest.mark.parametrize("Nk", [200, 256])
+def test_whole_waves_of_masked_keys_hold_anything(kind, Nk):
+    """Enough heads for the one-kernel backward, 32 keys and more masked in a row: NaN there gives the bits that zeros give."""
+    B, Nq, H, D = 66, 70, 2, 64
+    q, k, v, do = _make(B, Nq, Nk, H, H, D, BF16, 21)
+    mask = _mask(kind, B, Nk, 21)
+    results = []
+    for bad in (0.0, float("nan")):
+        parts = [q.clone(), k.masked_fill(~mask[:, :, None, None], bad), v.masked_fill(~mask[:, :, None, None], bad)]
+        parts = [t.requires_grad_(True) for t in parts]
+        out = eve_amd.attention(*parts, mask)
+        results.append((out, *torch.autograd.grad(out, parts, do)))
+    for name, a, b in zip(("out", "dq", "dk", "dv"), *results):
+        assert torch.isfinite(b).all() and torch.equal(a, b), name
+    assert_within(dict(zip(("out", "dq", "dk", "dv"), results[1])), attention64(q, k, v, mask, dout=do), kind)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rise", [0.02, 0.11, 0.3])
+def test_scores_that_rise_from_key_to_key(dtype, rise):
+    """The maximum moves on in every tile, by less, about and more than what makes a row rescale."""
+    B, Nq, Nk, H, D = 1, 70, 700, 2, 64
+    q, k, v, do = _make(B, Nq, Nk, H, H, D, dtype, 31, std=0.3)
+    along = torch.ones(D, dtype=dtype, device=DEV)
+    q = q + along
+    k = k + (torch.arange(Nk, device=DEV)[:, None, None] * (rise / 8)).to(dtype) * along  # scale q . k grows by about `rise` a key
+    res = attention64(q, k, v, dout=do)
+    parts = [t.requires_grad_(True) for t in (q, k, v)]
+    out = eve_amd.attention(*parts)
+    assert_within(dict(zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, parts, do)))), res, f"rise {rise}")
