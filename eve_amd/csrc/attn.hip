@@ -614,17 +614,8 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
       }
     }
     delta = halves_sum(delta);
-    if (row_ok) {
-      L = a.lse[lrow];
-      if (half == 0 && split == 0) a.stats[lrow] = row_stats(L, delta, a.inv_c);
-    }
+    if (row_ok) L = a.lse[lrow];
   }
-  at_f32x16 minus_delta;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) minus_delta[r] = -delta;
-  at_f32x16 dq[C::ND];
-#pragma unroll
-  for (int i = 0; i < C::ND; ++i) dq[i] = acc_zero();
 
   const int ntiles = (a.Nk + C::KT - 1) / C::KT;
   const int t0 = split * a.tiles_per_split, t1 = min(ntiles, t0 + a.tiles_per_split);
@@ -639,6 +630,36 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
   };
   uint64_t bits = keys.of(t0);
   fetch(t0, bits);
+  if constexpr (sizeof(T) == 2) {
+    // All of a row's keys in one tile: delta is formed as sum p dp.  The result's rounding, which do . o sees, would be large next to
+    // what is left of ds where keys are few (5 keys, width 112: dq 1.8 % off).
+    if (ntiles == 1) {
+      tile_ready<0>();
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j) {
+        at_f32x16 s = acc_zero(), dp = acc_zero();
+#pragma unroll
+        for (int ks = 0; ks < C::NKS; ++ks) {
+          s = mma(rows.get(smem, 0, j, ks), qf[ks], s, T());
+          dp = mma(rows.get(smem, C::TILE, j, ks), gf[ks], dp, T());
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -L)) * dp[r];
+          sum += (bits >> (32 * j + (r & 3) + 8 * (r >> 2) + 4 * half)) & 1 ? x : 0.f;
+        }
+      }
+      delta = halves_sum(sum);
+    }
+  }
+  if (row_ok && half == 0 && split == 0) a.stats[lrow] = row_stats(L, delta, a.inv_c);
+  at_f32x16 minus_delta;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) minus_delta[r] = -delta;
+  at_f32x16 dq[C::ND];
+#pragma unroll
+  for (int i = 0; i < C::ND; ++i) dq[i] = acc_zero();
   for (int t = t0; t < t1; ++t) {
     const uint32_t ks_ = (t - t0) % C::NST * C::STAGE, vs_ = ks_ + C::TILE;
     tile_ready<0>();

@@ -328,3 +328,42 @@ def test_scores_that_rise_from_key_to_key(dtype, rise):
     parts = [t.requires_grad_(True) for t in (q, k, v)]
     out = eve_amd.attention(*parts)
     assert_within(dict(zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, parts, do)))), res, f"rise {rise}")
+
+
+def _few_key_gradients(q, k, v, do, mask, scale):
+    """dq and dk in 64 bits and what bf16 may be off: ds rounded once by u = 2^-8, the result once more, and of ds itself, with
+    w = 2^-24, 64 w (1 + max |score|) of its terms p |dp| and p |delta| (fp32 products of up to 128 terms, exponential, row sums)."""
+    u, w = 2.0 ** -8, 2.0 ** -24
+    q, k, v, do = (t.detach().cpu().double().transpose(1, 2) for t in (q, k, v, do))
+    keep = mask.cpu()[:, None, None, :]
+    s = (scale * q @ k.transpose(2, 3)).masked_fill(~keep, float("-inf"))
+    p = torch.softmax(s, 3)
+    dp = do @ v.transpose(2, 3)
+    delta = (p * dp).sum(3, keepdim=True)
+    ds = p * (dp - delta)
+    size = 64 * w * (1 + (scale * (q.abs() @ k.abs().transpose(2, 3)))) * p * (do.abs() @ v.abs().transpose(2, 3) + (p * dp.abs()).sum(3, keepdim=True))
+    t_ds = u * ds.abs() + size
+    dq, dk = scale * ds @ k, scale * ds.transpose(2, 3) @ q
+    t_dq, t_dk = scale * t_ds @ k.abs() + u * dq.abs(), scale * t_ds.transpose(2, 3) @ q.abs() + u * dk.abs()
+    return {n: t.transpose(1, 2) for n, t in (("dq", dq), ("dk", dk))}, {n: t.transpose(1, 2) for n, t in (("dq", t_dq), ("dk", t_dk))}
+
+
+@pytest.mark.parametrize("D", [16, 64, 112])
+@pytest.mark.parametrize("Nk", [1, 2, 3, 5, 17, 32])
+@pytest.mark.parametrize("low", [False, True])
+def test_gradients_of_a_few_keys_keep_their_digits(Nk, D, low):
+    """Where keys are few, ds is what is left of nearly equal numbers: the rounding of the stored result must not enter it.  `low`:
+    scores far below zero, next to masked keys (whose score would be zero)."""
+    B, Nq, H = 3, 40, 2
+    q, k, v, do = _make(B, Nq, Nk, H, H, D, BF16, 41 + Nk)
+    if low:
+        q, k = q - 4.0, k + 4.0
+    mask = torch.ones(B, Nk, dtype=torch.bool, device=DEV)
+    mask[0, Nk // 2 + 1:] = False
+    parts = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = eve_amd.attention(*parts, mask)
+    dq, dk, _ = torch.autograd.grad(out, parts, do)
+    want, tol = _few_key_gradients(q, k, v, do, mask, D ** -0.5)
+    for name, got in (("dq", dq), ("dk", dk)):
+        err = (got.detach().cpu().double() - want[name]).abs()
+        assert torch.isfinite(got).all() and bool((err <= 1.02 * tol[name] + 1e-30).all()), (name, float((err / (tol[name] + 1e-30)).max()))
