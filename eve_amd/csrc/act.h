@@ -20,7 +20,7 @@ template <int ACT, bool FAST> __device__ __forceinline__ float act_fwd(float z) 
   } else if constexpr (ACT == EVE_ACT_GELU) {
     return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
   } else if constexpr (ACT == EVE_ACT_RELU) {
-    return z > 0.f ? z : 0.f;
+    return z <= 0.f ? 0.f : z;  // NaN stays NaN
   } else {
     return z;
   }
@@ -33,7 +33,7 @@ template <int ACT, bool FAST> __device__ __forceinline__ float act_bwd(float z) 
   } else if constexpr (ACT == EVE_ACT_GELU) {
     return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.3989422804014327f * exp_<FAST>(-0.5f * z * z);
   } else if constexpr (ACT == EVE_ACT_RELU) {
-    return z > 0.f ? 1.f : 0.f;
+    return z <= 0.f ? 0.f : 1.f;  // (at NaN: the gradient passes, as in torch)
   } else {
     return 1.f;
   }
