@@ -116,6 +116,16 @@ def layer_norm(mod: nn.LayerNorm, x: Tensor) -> Tensor:
     return mod(x)
 
 
+_ALL_MODULES = torch.nn.modules.module  # where torch keeps the hooks of every module
+
+
+def _is_plain(mod: nn.Module, cls: type) -> bool:
+    """Whether a call of `mod` is `cls.forward` and nothing else: no other class, no forward of its own, no hooks."""
+    return (type(mod) is cls and "forward" not in mod.__dict__
+            and not (mod._forward_hooks or mod._forward_pre_hooks or mod._backward_hooks or mod._backward_pre_hooks
+                     or _ALL_MODULES._has_any_global_hook()))
+
+
 class Attention(nn.Module):
     """Reference :57-132.  `qkv` has no bias of its own; `q_bias` / `v_bias` are separate parameters (the key
     bias is fixed at zero), as in BEiT."""
@@ -146,13 +156,17 @@ class Attention(nn.Module):
         self.impl = impl
 
     def takes_fused(self, x: Tensor, mask: Optional[Tensor], relative_position_bias: Optional[Tensor]) -> bool:
-        """Whether the library's kernels compute this call: one type on the GPU, no bias on the scores, no dropout inside."""
+        """Whether the library's kernels compute this call: one type on the GPU, no bias on the scores, no dropout inside, and
+        parts that a call of them would have run just so (the kernels read the parameters past their modules)."""
         if self.impl != "fused" or relative_position_bias is not None or not x.is_cuda or x.dim() != 3 or torch.is_autocast_enabled():
             return False
-        dropout = self.training and (self.attn_drop.p > 0.0 or self.proj_drop.p > 0.0)
+        if not (all(_is_plain(m, nn.Linear) for m in (self.qkv, self.proj))
+                and all(_is_plain(m, nn.Dropout) and not (m.training and m.p > 0.0) for m in (self.attn_drop, self.proj_drop))):
+            return False
         params = (self.qkv.weight, self.q_bias, self.v_bias, self.proj.weight, self.proj.bias)
         width = x.shape[2] // self.num_heads
-        return (not dropout and x.dtype in (torch.float32, torch.bfloat16) and width % 8 == 0 and 8 <= width <= 128 and self.scale > 0
+        return (not (self.training and self.attn_drop.p > 0.0) and x.dtype in (torch.float32, torch.bfloat16)
+                and width % 8 == 0 and 8 <= width <= 128 and self.scale > 0
                 and self.qkv.weight.shape[0] == 3 * self.num_heads * width  # heads that do not divide the width: the stock path's error
                 and all(p is None or p.dtype == x.dtype for p in params) and (mask is None or tuple(mask.shape) == tuple(x.shape[:2])))
 
@@ -291,13 +305,16 @@ class MultiwayTransformerEnocderLayer(nn.Module):
         return row_scale
 
     def set_attention(self, impl: str = "stock") -> None:
-        self.attn.set_attention(impl)
+        if hasattr(self.attn, "set_attention"):
+            self.attn.set_attention(impl)
+        elif impl != "stock":
+            raise TypeError(f"eve_amd: the layer's attention is a {type(self.attn).__name__}, which has no {impl!r} form")
 
     def _attention_branch(self, residual: Tensor, attention_mask, relative_position_bias) -> Tensor:
         """residual + drop_path(gamma_1 * attn(norm1(residual))) (reference :338-341)."""
         x = layer_norm(self.norm1, residual)
         gamma = self.gamma_1 if isinstance(self.gamma_1, Tensor) else None
-        if (self.attn.takes_fused(x, attention_mask, relative_position_bias) and x.dtype == residual.dtype
+        if (_is_plain(self.attn, Attention) and self.attn.takes_fused(x, attention_mask, relative_position_bias) and x.dtype == residual.dtype
                 and (gamma is None or (gamma.dtype == x.dtype and tuple(gamma.shape) == (x.shape[-1],)))):
             return self.attn.fused(x, attention_mask, gamma, self._drop_path_scale(x), residual)
         x = self.attn(x, mask=attention_mask, relative_position_bias=relative_position_bias)

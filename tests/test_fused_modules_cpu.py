@@ -1,0 +1,135 @@
+"""`set_attention("fused")` takes a call only where the modules it reads past would have done nothing else: hooks, replaced modules
+and overridden forwards run the stock path.  Without a GPU: `takes_fused` sees a stand-in for a tensor on one."""
+import pytest
+import torch
+from torch import nn
+
+from eve_amd.encoder import Attention, MultiwayTransformerEnocderLayer
+
+
+class _OnGpu:
+    is_cuda, dtype, shape, device = True, torch.float32, torch.Size((2, 9, 64)), torch.device("cuda", 0)
+
+    def dim(self):
+        return 3
+
+
+def _attn(**kw):
+    attn = Attention(64, 4, qkv_bias=True, **kw)
+    attn.set_attention("fused")
+    assert attn.takes_fused(_OnGpu(), None, None)
+    return attn
+
+
+class _Scaled(nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+class _Adapter(nn.Module):
+    def __init__(self, base):
+        super().__init__()
+        self.base, self.extra = base, nn.Linear(base.in_features, base.out_features)
+        self.weight, self.bias = base.weight, base.bias
+
+    def forward(self, x):
+        return self.base(x) + self.extra(x)
+
+
+def _hook(*args):
+    return None
+
+
+@pytest.mark.parametrize("which", ["proj", "qkv", "attn_drop", "proj_drop"])
+@pytest.mark.parametrize("register", ["register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook",
+                                      "register_full_backward_pre_hook"])
+def test_hooks_keep_the_stock_path(which, register):
+    attn = _attn()
+    handle = getattr(getattr(attn, which), register)(_hook)
+    assert not attn.takes_fused(_OnGpu(), None, None)
+    handle.remove()
+    assert attn.takes_fused(_OnGpu(), None, None)
+
+
+@pytest.mark.parametrize("change", ["subclass", "adapter", "instance forward", "own bias", "parametrized", "identity drop", "other drop"])
+def test_replaced_parts_keep_the_stock_path(change):
+    attn = _attn()
+    if change == "subclass":
+        attn.proj = _Scaled(64, 64)
+    elif change == "adapter":
+        attn.proj = _Adapter(attn.proj)
+    elif change == "instance forward":
+        old = attn.proj.forward
+        attn.proj.forward = lambda x: old(x) + 1
+    elif change == "own bias":
+        attn.qkv = _Scaled(64, 192, bias=False)
+    elif change == "parametrized":
+        nn.utils.parametrizations.orthogonal(attn.proj)
+    elif change == "identity drop":
+        attn.proj_drop = nn.Sequential()
+    else:
+        attn.proj_drop = nn.Hardtanh()
+    assert not attn.takes_fused(_OnGpu(), None, None)
+
+
+@pytest.mark.parametrize("register", ["register_module_forward_hook", "register_module_forward_pre_hook", "register_module_full_backward_hook"])
+def test_hooks_on_all_modules_keep_the_stock_path(register):
+    attn = _attn()
+    handle = getattr(nn.modules.module, register)(_hook)
+    try:
+        assert not attn.takes_fused(_OnGpu(), None, None)
+    finally:
+        handle.remove()
+    assert attn.takes_fused(_OnGpu(), None, None)
+
+
+def _layer():
+    torch.manual_seed(0)
+    return MultiwayTransformerEnocderLayer(64, "quick_gelu", 4, 128, (5, 4), 0.0)
+
+
+class _Wrapped(nn.Module):
+    """An attention of the user's own, which knows nothing of `set_attention`."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner = inner
+
+    def forward(self, x, mask=None, relative_position_bias=None):
+        return 3 * self.inner(x, mask=mask, relative_position_bias=relative_position_bias)
+
+
+def test_an_attention_of_the_users_own_is_called():
+    lay, x = _layer(), torch.randn(2, 9, 64)
+    plain = lay._attention_branch(x, None, None) - x
+    lay.attn = _Wrapped(lay.attn)
+    torch.testing.assert_close(lay._attention_branch(x, None, None) - x, 3 * plain, rtol=1e-4, atol=1e-6)
+    lay.set_attention("stock")
+    with pytest.raises(TypeError, match="_Wrapped"):
+        lay.set_attention("fused")
+
+
+class _Doubled(Attention):
+    def forward(self, x, mask=None, relative_position_bias=None):
+        return 2 * super().forward(x, mask, relative_position_bias)
+
+
+@pytest.mark.parametrize("how", ["hook", "subclass", "instance"])
+def test_the_layer_calls_an_attention_that_does_more(how, monkeypatch):
+    """The branch may go past `attn` only where calling it would have done nothing else."""
+    lay, x = _layer(), torch.randn(2, 9, 64)
+    if how == "subclass":
+        lay.attn = _Doubled(64, 4, qkv_bias=True)
+    lay.set_attention("fused")
+    monkeypatch.setattr(Attention, "takes_fused", lambda self, x, mask, bias: not bias)  # the branch's call; forward's as well
+    monkeypatch.setattr(Attention, "fused", lambda self, x, mask, gamma=None, row_scale=None, residual=None:
+                        torch.ones_like(x) if residual is None else pytest.fail("past the module"))
+    factor = 2.0
+    if how == "hook":
+        lay.attn.register_forward_hook(lambda m, a, out: 2 * out)
+    elif how == "instance":
+        old = lay.attn.forward
+        lay.attn.forward = lambda *a, **k: 2 * old(*a, **k)
+    with torch.no_grad():
+        got = lay._attention_branch(x, None, None) - x
+    torch.testing.assert_close(got, (factor * lay.gamma_1).detach().expand_as(got), rtol=1e-4, atol=1e-5)
