@@ -15,6 +15,8 @@ from . import ops
 def _check(q: Tensor, Nk: int, Hkv: int, key_mask: Optional[Tensor], scale: Optional[float], on: bool):
     """-> (key_mask, scale) as the kernels take them; q [.., H, D] with the batch in front.  Shapes first, then the device."""
     B, H, D = q.shape[0], q.shape[-2], q.shape[-1]
+    if max(*q.shape, Nk, Hkv) >= 1 << 31:  # the C calls' sizes are 32-bit
+        raise ValueError(f"eve_amd.attention: sizes {tuple(q.shape)}, {Nk} keys of {Hkv} heads (2^31 and more are not supported)")
     if H < 1 or Hkv < 1 or H % Hkv:
         raise ValueError(f"eve_amd.attention: {H} query heads cannot share {Hkv} key/value heads")
     if D % 8 or not 8 <= D <= 128:

@@ -65,6 +65,8 @@ def fused_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activ
     ops._dt(x)
     dtype, device, lead = x.dtype, x.device, x.shape[:-1]
     N = weight.shape[0]
+    if max(math.prod(lead), *weight.shape) >= 1 << 31:  # the C calls' sizes are 32-bit
+        raise ValueError(f"eve_amd.fused_linear: x {tuple(x.shape)}, weight {tuple(weight.shape)} (2^31 rows or columns and more are not supported)")
     parts = (("weight", weight, weight.shape), ("bias", bias, (N,)), ("gamma", gamma, (N,)), ("row_scale", row_scale, x.shape[:1]),
              ("residual", residual, lead + (N,)))
     elsewhere = "" if not x.is_cuda else None

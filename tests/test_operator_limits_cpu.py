@@ -1,0 +1,32 @@
+"""What lies at the ends of what eve_amd.attention and eve_amd.fused_linear take, without a GPU."""
+import pytest
+import torch
+
+import eve_amd
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+BIG = (1 << 32) + 2  # what is left of it in 32 bits is 2
+
+
+@pytest.mark.parametrize("q,k", [((BIG, 1, 1, 8), (BIG, 1, 1, 8)), ((1, BIG, 1, 8), (1, 3, 1, 8)), ((1, 3, 1, 8), (1, BIG, 1, 8)),
+                                 ((1, 3, BIG, 8), (1, 3, 1, 8)), ((1, 1 << 31, 1, 8), (1, 3, 1, 8))])
+def test_attention_refuses_sizes_beyond_32_bits(q, k):
+    with pytest.raises(ValueError, match="2\\^31"):
+        eve_amd.attention(_meta(*q), _meta(*k), _meta(*k))
+
+
+def test_self_attention_refuses_sizes_beyond_32_bits():
+    for shape in ((BIG, 1, 3, 1, 8), (1, BIG, 3, 1, 8), (1, 1, 3, BIG, 8)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            eve_amd.self_attention(_meta(*shape))
+
+
+@pytest.mark.parametrize("x,w", [((BIG, 1), (2, 1)), ((1 << 16, 1 << 16, 1), (2, 1)), ((2, BIG), (1, BIG)), ((2, 1), (BIG, 1)),
+                                 ((1 << 31, 1), (1, 1))])
+def test_fused_linear_refuses_sizes_beyond_32_bits(x, w):
+    with pytest.raises(ValueError, match="2\\^31"):
+        eve_amd.fused_linear(_meta(*x), _meta(*w))
