@@ -487,7 +487,7 @@ def attn_readable(t: torch.Tensor) -> torch.Tensor:
     boundaries and at most 2^22 elements apart; else a copy."""
     unit = 16 // t.element_size()
     parts = (_attn_at(t),) if t.dim() == 4 else _attn_parts_at(t)
-    if t.stride(-1) == 1 and all(_attn_reads(at, unit) for at in parts) or not t.numel():
+    if t.stride(-1) == 1 and all(_attn_reads(at, unit) for at in parts):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

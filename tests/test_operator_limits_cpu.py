@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import eve_amd
+from eve_amd import ops
 
 
 def _meta(*shape, dtype=torch.bfloat16):
@@ -30,3 +31,12 @@ def test_self_attention_refuses_sizes_beyond_32_bits():
 def test_fused_linear_refuses_sizes_beyond_32_bits(x, w):
     with pytest.raises(ValueError, match="2\\^31"):
         eve_amd.fused_linear(_meta(*x), _meta(*w))
+
+
+@pytest.mark.parametrize("make", [lambda: torch.zeros(2, 5, 3, 9)[:, :0, :, :8], lambda: torch.zeros(2, 5, 3, 9)[:0, :, :, 1:],
+                                  lambda: torch.zeros(2, 5, 3, 16)[:, :0, :, ::2], lambda: torch.zeros(2, 5, 3, 3, 9)[:, :0, :, :, :8]])
+def test_what_is_empty_lies_as_the_kernels_want_it(make):
+    """An empty part of a tensor has that tensor's strides, which the entry points check all the same."""
+    t = ops.attn_readable(make())
+    assert t.shape == make().shape and t.stride(-1) == 1
+    assert all(s % 4 == 0 for s in t.stride()[:-1]), t.stride()
