@@ -1243,7 +1243,7 @@ int launch_attn(void (*kern)(AttnArgs), AttnArgs& a, int nw, int lds, hipStream_
   const int64_t per = (int64_t)a.nblk * a.nsplit;
   a.by_xcd = a.heads % 8 == 0 || a.heads >= 64;
   const int64_t grid = (a.by_xcd ? ((int64_t)a.heads + 7) / 8 * 8 : a.heads) * per;
-  EVE_REQUIRE(grid <= 0x7fffffffLL && per <= 0x7fffffffLL, EVE_ERR_UNSUPPORTED, "%s: too many workgroups", name);
+  EVE_REQUIRE(grid <= kMaxThreads / (nw * 64) && per <= 0x7fffffffLL, EVE_ERR_UNSUPPORTED, "%s: too many workgroups", name);
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     EVE_REQUIRE(e == hipSuccess, EVE_ERR_LAUNCH, "%s: %d bytes of LDS: %s", name, lds, hipGetErrorString(e));
@@ -1265,7 +1265,7 @@ int fwd_typed(AttnArgs& a, const AttnPlan& p, hipStream_t st) {
   const int rc = launch_attn(p.nw == 1 ? attn_fwd_kernel<T, DP, 1> : attn_fwd_kernel<T, DP, 4>, a, p.nw,
                              p.nw == 1 ? attn_lds<FwdCfg<T, DP, 1>>() : attn_lds<FwdCfg<T, DP, 4>>(), st, "eve_attn_fwd");
   if (rc != EVE_OK || a.nsplit == 1) return rc;
-  EVE_REQUIRE((int64_t)a.heads * a.rows <= 0x7fffffffLL, EVE_ERR_UNSUPPORTED, "eve_attn_fwd: too many rows");
+  EVE_REQUIRE((int64_t)a.heads * a.rows <= kMaxThreads / 256, EVE_ERR_UNSUPPORTED, "eve_attn_fwd: too many rows");
   attn_join_kernel<T><<<dim3((unsigned)(a.heads * a.rows)), dim3(256), 0, st>>>(a);
   EVE_CHECK_LAUNCH("eve_attn_fwd (join)");
   return EVE_OK;
@@ -1277,7 +1277,7 @@ AttnSum sum_of(const AttnArgs& a, const float* part, void* g, int64_t g_b, int64
 template <typename T>
 int sum_parts(const AttnSums& s, int n, hipStream_t st) {  // n of one size
   const int64_t grid = (s.s[0].total + 255) / 256;
-  EVE_REQUIRE(grid <= 0x7fffffffLL, EVE_ERR_UNSUPPORTED, "eve_attn_bwd: too many rows");
+  EVE_REQUIRE(grid <= kMaxThreads / 256, EVE_ERR_UNSUPPORTED, "eve_attn_bwd: too many rows");
   attn_sum_kernel<T><<<dim3((unsigned)grid, n), dim3(256), 0, st>>>(s);
   EVE_CHECK_LAUNCH("eve_attn_bwd (sum of the splits)");
   return EVE_OK;

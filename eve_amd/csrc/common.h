@@ -11,6 +11,7 @@ namespace eve {
 typedef __bf16 bf16_t;
 
 constexpr int kWave = 64;
+constexpr int64_t kMaxThreads = 0xffffffffLL;  // of a launch's dimension
 
 // ---- error plumbing -------------------------------------------------------------
 void set_error(const char* fmt, ...);

@@ -994,7 +994,7 @@ bool product_aligned(const LinArgs& a, bool acol, bool bcol, int size) {
 template <typename T, int BT, bool ACOL, bool BCOL, int MODE>
 int launch_tile(const LinArgs& a, hipStream_t st) {
   const int64_t total = (int64_t)((a.M + BT - 1) / BT) * ((a.N + BT - 1) / BT) * a.nsplit;
-  EVE_REQUIRE(total <= 0x7ffffff0LL, EVE_ERR_UNSUPPORTED, "eve_linear: too many tiles");
+  EVE_REQUIRE(total <= kMaxThreads / tile_threads<BT>() - 8, EVE_ERR_UNSUPPORTED, "eve_linear: too many tiles");
   constexpr int lds = 2 * 2 * BT * 128 > 4 * 32 * (BT / 2 + 4) * 4 ? 2 * 2 * BT * 128 : 4 * 32 * (BT / 2 + 4) * 4;
   linear_tile_kernel<T, BT, ACOL, BCOL, MODE><<<dim3((unsigned)((total + 7) / 8 * 8)), dim3(tile_threads<BT>()), lds, st>>>(a);
   EVE_CHECK_LAUNCH("eve_linear (product)");
@@ -1004,7 +1004,7 @@ template <typename T, int BM, bool ACOL, bool BCOL, int MODE, int ACT = EVE_ACT_
 int launch_stream(LinArgs a, hipStream_t st) {
   const int tn = ceil_div(a.N, kStreamN);
   const int64_t total = (int64_t)ceil_div(a.M, BM) * tn * a.nsplit;
-  EVE_REQUIRE(total <= 0x7ffffff0LL, EVE_ERR_UNSUPPORTED, "eve_linear: too many tiles");
+  EVE_REQUIRE(total <= kMaxThreads / 256 - 8, EVE_ERR_UNSUPPORTED, "eve_linear: too many tiles");
   // half an L2 (2 MiB) of B a group, and groups of equal width
   const int64_t panel = (int64_t)kStreamN * (MODE == LIN_PART ? a.kspan : a.K) * (int)sizeof(T);
   int width = (int)((2 << 20) / (panel > 0 ? panel : 1));
@@ -1061,8 +1061,9 @@ int shared_tiles(int64_t M, int64_t N, int cost64, int cus) {
 template <typename T, int NTL>
 int launch_shared(const LinArgs& a, hipStream_t st) {
   constexpr int R = 16 * NTL;
-  const int total = (a.M + R - 1) / R * ((a.N + R - 1) / R);  // below 4096: 128 x 128 tiles fill less than half of the CUs
-  linear_shared_kernel<T, NTL><<<dim3((total + 7) / 8 * 8), dim3(512), 0, st>>>(a);
+  const int64_t total = (int64_t)((a.M + R - 1) / R) * ((a.N + R - 1) / R);
+  EVE_REQUIRE(total <= kMaxThreads / 512 - 8, EVE_ERR_UNSUPPORTED, "eve_linear: too many tiles");
+  linear_shared_kernel<T, NTL><<<dim3((unsigned)((total + 7) / 8 * 8)), dim3(512), 0, st>>>(a);
   EVE_CHECK_LAUNCH("eve_linear_fwd (shared contraction)");
   return EVE_OK;
 }
@@ -1168,6 +1169,7 @@ int bwd_typed(const DzArgs& dzin, const void* x, const void* w, void* dx, void* 
     s.n_c = N; s.parts_c = with_dw ? p.nsplit : p.parts; s.blocks_c = ceil_div(N, 32);
   }
   const int64_t blocks = s.blocks_w + (s.n_c ? 2 * (int64_t)s.blocks_c : 0);
+  EVE_REQUIRE(blocks <= kMaxThreads / 256, EVE_ERR_UNSUPPORTED, "eve_linear: too many weights");
   if (blocks > 0) {
     linear_sum_kernel<T><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(s);
     EVE_CHECK_LAUNCH("eve_linear_bwd (sums)");

@@ -1,9 +1,11 @@
 """What lies at the ends of what eve_amd.attention and eve_amd.fused_linear take, without a GPU."""
+import ctypes
+
 import pytest
 import torch
 
 import eve_amd
-from eve_amd import ops
+from eve_amd import _lib, ops
 
 
 def _meta(*shape, dtype=torch.bfloat16):
@@ -40,3 +42,16 @@ def test_what_is_empty_lies_as_the_kernels_want_it(make):
     t = ops.attn_readable(make())
     assert t.shape == make().shape and t.stride(-1) == 1
     assert all(s % 4 == 0 for s in t.stride()[:-1]), t.stride()
+
+
+def test_more_workgroups_than_a_launch_holds_are_refused():
+    """2^32 threads in a dimension: one-wave workgroups for a head of up to 64 rows, four waves else."""
+    lib, p = _lib.load(), ctypes.addressof
+    lay = _lib.AttnLayout(*[8] * 9)
+
+    def fwd(**kw):
+        s = _lib.AttnShape(**{**dict(B=1, Nq=1, Nk=1, H=1, Hkv=1, D=8, dtype=_lib.BF16, scale=1.0), **kw})
+        return lib.eve_attn_fwd(p(s), p(lay), 16, 16, 16, None, 16, None, None, 0, None)
+
+    assert fwd(B=1 << 26) == -4 and b"workgroups" in lib.eve_moe_last_error()
+    assert fwd(B=1 << 24, Nq=65) == -4 and b"workgroups" in lib.eve_moe_last_error()
