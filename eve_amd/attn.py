@@ -22,8 +22,8 @@ def _check(q: Tensor, Nk: int, Hkv: int, key_mask: Optional[Tensor], scale: Opti
     if D % 8 or not 8 <= D <= 128:
         raise ValueError(f"eve_amd.attention: head width {D} (a multiple of 8 up to 128 is supported)")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"eve_amd.attention: scale {scale} (must be positive and finite)")
+    if not ops.ATTN_SCALES[0] <= scale <= ops.ATTN_SCALES[1]:
+        raise ValueError(f"eve_amd.attention: scale {scale} (must lie between 2^-100 and 2^100)")
     if key_mask is not None:
         if key_mask.shape != (B, Nk):
             raise ValueError(f"eve_amd.attention: `key_mask` has shape {tuple(key_mask.shape)}, the keys need {(B, Nk)}")
@@ -82,7 +82,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor] = None
 
     q [B, Nq, H, D]; k, v [B, Nk, Hkv, D], float32 or bfloat16, at any strides (read in place where the last dimension is
     contiguous and rows start on 16-byte boundaries, else copied); H a multiple of Hkv: head h reads key head h // (H // Hkv).
-    D is a multiple of 8 up to 128.  key_mask [B, Nk]: nonzero = visible.  scale: D ** -0.5 unless given, positive.
+    D is a multiple of 8 up to 128.  key_mask [B, Nk]: nonzero = visible.  scale: D ** -0.5 unless given, from 2^-100 to 2^100.
     -> [B, Nq, H, D].  A sample without a visible key gives zeros and passes no gradient; masked keys and values may hold
     anything, NaN included.  Scores and sums are float32; results do not depend on the order of execution."""
     for t, n in ((q, "q"), (k, "k"), (v, "v")):

@@ -1197,6 +1197,8 @@ BwdWs bwd_ws(const eve_attn_shape& s, const AttnPlan& pq, const AttnPlan& pk) {
   return w;
 }
 
+constexpr float kLeastScale = 0x1p-100f;
+
 int check_shape(const eve_attn_shape* s) {
   EVE_REQUIRE(s, EVE_ERR_ARG, "eve_attn: null shape");
   EVE_REQUIRE(s->dtype == EVE_F32 || s->dtype == EVE_BF16, EVE_ERR_ARG, "eve_attn: dtype %d", s->dtype);
@@ -1204,7 +1206,8 @@ int check_shape(const eve_attn_shape* s) {
   EVE_REQUIRE(s->H >= 1 && s->Hkv >= 1 && s->H % s->Hkv == 0, EVE_ERR_ARG, "eve_attn: %d query heads do not share %d key heads", s->H, s->Hkv);
   EVE_REQUIRE((int64_t)s->H * s->D <= (1 << 22), EVE_ERR_UNSUPPORTED, "eve_attn: %d heads of %d", s->H, s->D);
   EVE_REQUIRE(s->D >= 8 && s->D <= 128 && s->D % 8 == 0, EVE_ERR_UNSUPPORTED, "eve_attn: head width %d (a multiple of 8 up to 128)", s->D);
-  EVE_REQUIRE(s->scale > 0.f && s->scale <= 3.4e38f, EVE_ERR_ARG, "eve_attn: scale must be positive and finite");
+  // the backward works with L / c, c = scale log2 e: both it and 1 / c have to be normal numbers of 32 bits
+  EVE_REQUIRE(s->scale >= kLeastScale && s->scale <= 1.f / kLeastScale, EVE_ERR_ARG, "eve_attn: scale must lie between 2^-100 and 2^100");
   EVE_REQUIRE((int64_t)s->Nq * (s->H / s->Hkv) <= 0x7fff0000LL && s->Nk <= 0x7fff0000, EVE_ERR_UNSUPPORTED, "eve_attn: too many rows");
   EVE_REQUIRE((int64_t)s->B * s->Hkv <= 0x7fff0000LL && (int64_t)s->B * s->Nq <= 0x7fff0000LL, EVE_ERR_UNSUPPORTED, "eve_attn: batch too large");
   return EVE_OK;

@@ -33,6 +33,7 @@ from .experts import MultiwayTransformerMLP
 from .layer import MoE
 from .linear import fused_linear
 from .multiway import ModalitySplitFFN
+from .ops import ATTN_SCALES
 
 
 class DropPath(nn.Module):
@@ -166,7 +167,7 @@ class Attention(nn.Module):
         params = (self.qkv.weight, self.q_bias, self.v_bias, self.proj.weight, self.proj.bias)
         width = x.shape[2] // self.num_heads
         return (not (self.training and self.attn_drop.p > 0.0) and x.dtype in (torch.float32, torch.bfloat16)
-                and width % 8 == 0 and 8 <= width <= 128 and self.scale > 0
+                and width % 8 == 0 and 8 <= width <= 128 and ATTN_SCALES[0] <= self.scale <= ATTN_SCALES[1]
                 and self.qkv.weight.shape[0] == 3 * self.num_heads * width  # heads that do not divide the width: the stock path's error
                 and all(p is None or p.dtype == x.dtype for p in params) and (mask is None or tuple(mask.shape) == tuple(x.shape[:2])))
 

@@ -430,6 +430,9 @@ def scale_residual_bwd(dout, x, gamma, row_scale, T: int):
 
 
 # ----------------------------------------------------------------------------------- attention of the encoder layer
+ATTN_SCALES = (2.0 ** -100, 2.0 ** 100)  # what eve_attn_* take
+
+
 def _on_device_of(which: int):
     """Decorates a wrapper: its calls are enqueued on the current stream of the device of argument `which`, whichever device is
     current."""

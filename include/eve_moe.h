@@ -401,7 +401,7 @@ int eve_scale_residual_bwd(const void* dout, const void* x, const void* gamma, c
  * (NULL: all); h' = h / (H / Hkv): query heads may share a key/value head.  A sample without a visible key gives zeros, and what
  * a masked key or value row holds (NaN included) takes no part.  q [B,Nq,H,D], k and v [B,Nk,Hkv,D] lie anywhere with the last
  * dimension contiguous (strides below, in elements, multiples of 16 bytes; every pointer 16-byte aligned), so the three parts of
- * one qkv product are read where they are.  D is a multiple of 8 up to 128; scale > 0.  out, dout: contiguous [B,Nq,H,D].
+ * one qkv product are read where they are.  D is a multiple of 8 up to 128; 2^-100 <= scale <= 2^100.  out, dout: contiguous [B,Nq,H,D].
  * lse [B, H, Nq] fp32 (opaque order; may be NULL without a backward) is what the backward recomputes the probabilities from.
  * Scores, maxima, sums and accumulators are fp32; with EVE_BF16 the probabilities and ds enter the second products as bf16.
  * No atomics: results do not depend on the order of execution. */

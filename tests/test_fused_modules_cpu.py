@@ -133,3 +133,9 @@ def test_the_layer_calls_an_attention_that_does_more(how, monkeypatch):
     with torch.no_grad():
         got = lay._attention_branch(x, None, None) - x
     torch.testing.assert_close(got, (factor * lay.gamma_1).detach().expand_as(got), rtol=1e-4, atol=1e-5)
+
+
+def test_a_scale_that_the_kernels_refuse_runs_stock():
+    attn = _attn()
+    attn.scale = 2.0 ** -110
+    assert not attn.takes_fused(_OnGpu(), None, None)

@@ -55,3 +55,16 @@ def test_more_workgroups_than_a_launch_holds_are_refused():
 
     assert fwd(B=1 << 26) == -4 and b"workgroups" in lib.eve_moe_last_error()
     assert fwd(B=1 << 24, Nq=65) == -4 and b"workgroups" in lib.eve_moe_last_error()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -101, 1e-38, 2.0 ** 101, 3e38])
+def test_scales_whose_reciprocal_leaves_float32_are_refused(scale):
+    t = torch.zeros(1, 4, 2, 64)
+    with pytest.raises(ValueError, match="scale"):
+        eve_amd.attention(t, t, t, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        eve_amd.self_attention(torch.zeros(1, 4, 3, 2, 64), scale=scale)
+    s = _lib.AttnShape(1, 4, 4, 2, 2, 64, _lib.F32, scale)
+    lay = _lib.AttnLayout(*[512, 128, 64] * 3)
+    p = ctypes.addressof
+    assert _lib.load().eve_attn_fwd(p(s), p(lay), 16, 16, 16, None, 16, None, None, 0, None) == -1
