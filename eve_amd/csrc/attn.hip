@@ -568,11 +568,12 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
   mid = __float_as_uint(r) & 0xffff0000u;
   lo = __float_as_uint(r - __uint_as_float(mid)) & 0xffff0000u;
 }
-// -L / c and -delta as three bf16 each (a row that sees nothing: p = 2^(-1e30) = 0)
+// -L / c and -delta as three bf16 each (a row that sees nothing: p = 2^(-1e30) = 0; NaN stays).  The matrix unit multiplies what it does
+// not add by zero, so that a delta that is no number would spoil p too: it is left out, as do . v is no number either in such a row.
 __device__ __forceinline__ uint4 row_stats(float L, float delta, float inv_c) {
   uint32_t l0, l1, l2, d0, d1, d2;
-  split3(fminf(L, 1e30f) * -inv_c, l0, l1, l2);
-  split3(-delta, d0, d1, d2);
+  split3((L > 1e30f ? 1e30f : L) * -inv_c, l0, l1, l2);
+  split3(__builtin_fabsf(delta) < INFINITY ? -delta : 0.f, d0, d1, d2);
   return make_uint4((l0 >> 16) | l1, (l2 >> 16) | d0, (d1 >> 16) | d2, 0);
 }
 #endif
