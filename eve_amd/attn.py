@@ -83,7 +83,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, key_mask: Optional[Tensor] = None
     q [B, Nq, H, D]; k, v [B, Nk, Hkv, D], float32 or bfloat16, at any strides (read in place where the last dimension is
     contiguous and rows start on 16-byte boundaries, else copied); H a multiple of Hkv: head h reads key head h // (H // Hkv).
     D is a multiple of 8 up to 128.  key_mask [B, Nk]: nonzero = visible.  scale: D ** -0.5 unless given, from 2^-100 to 2^100.
-    -> [B, Nq, H, D].  A sample without a visible key gives zeros and passes no gradient; masked keys and values may hold
+    -> [B, Nq, H, D].  A sample without a visible key gives zeros and passes no gradient (a row whose
+    visible scores are all -inf is NaN, as the formula has it); masked keys and values may hold
     anything, NaN included.  Scores and sums are float32; results do not depend on the order of execution."""
     for t, n in ((q, "q"), (k, "k"), (v, "v")):
         if t.dim() != 4:

@@ -83,6 +83,7 @@ template <typename T, int DP, bool LONG = false> struct AttnCfg {
   }
 };
 
+constexpr float kLowest = -3.4028234663852886e38f;  // the lowest finite number
 constexpr int kBitTiles = 64;  // tiles whose mask words a workgroup holds
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -363,6 +364,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
 #pragma unroll
   for (int i = 0; i < C::ND; ++i) o[i] = acc_zero();
   float m = -INFINITY, l = 0.f;
+  bool any = false;  // key seen so far
 
   const int ntiles = (a.Nk + C::KT - 1) / C::KT;
   const int t0 = split * a.tiles_per_split, t1 = min(ntiles, t0 + a.tiles_per_split);
@@ -383,6 +385,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
     const uint64_t bits_next = keys.of(t + 1);
     fetch(t + 1, bits_next);
     if (bits) {
+      any = true;
       at_f32x16 s[C::NJ];
 #pragma unroll
       for (int j = 0; j < C::NJ; ++j) {
@@ -416,7 +419,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
       }
-      const float ms = m == -INFINITY ? 0.f : m;  // nothing visible so far: 2^(-inf - 0) = 0
+      const float ms = m == -INFINITY ? 0.f : m;  // only scores of -inf so far: 2^(-inf - 0) = 0, should others follow
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < C::NJ; ++j)
@@ -443,7 +446,8 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
   l = halves_sum(l);
   if (!row_ok) return;
   if (a.nsplit == 1) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // no visible key: zeros
+    const float none = any ? NAN : 0.f;  // no visible key: zeros; visible keys whose scores are all -inf: NaN, as -inf - (-inf) is
+    const float inv = l == 0.f ? none : 1.f / l;
     T* op = static_cast<T*>(a.out) + (((int64_t)b * a.Nq + qi) * (a.Hkv * a.G) + qh) * a.D;
 #pragma unroll
     for (int i = 0; i < C::ND; ++i)
@@ -452,7 +456,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
         const int d = 32 * i + 8 * g + 4 * half;
         if (d < a.D) store4<T>(op + d, o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv);
       }
-    if (a.lse && half == 0) a.lse[(int64_t)head * a.rows + row] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (a.lse && half == 0) a.lse[(int64_t)head * a.rows + row] = l == 0.f ? (any ? NAN : INFINITY) : m + __builtin_amdgcn_logf(l);
   } else {
     const int64_t at = ((int64_t)head * a.nsplit + split) * a.rows + row;
     float* op = a.part_o + at * a.D;
@@ -464,7 +468,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 1 : DP == 128 ? 2 : sizeof(T) ==
         if (d < a.D) store4<float>(op + d, o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
       }
     if (half == 0) {
-      a.part_ml[2 * at] = m;
+      a.part_ml[2 * at] = any ? fmaxf(m, kLowest) : m;  // -inf tells the join that nothing was visible
       a.part_ml[2 * at + 1] = l;
     }
   }
@@ -523,11 +527,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     x.z += y.z;
     x.w += y.w;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const bool any = top != -INFINITY;
+  const float inv = l == 0.f ? (any ? NAN : 0.f) : 1.f / l;
   const int b = head / a.Hkv, hk = head % a.Hkv;
   T* op = static_cast<T*>(a.out) + (((int64_t)b * a.Nq + row / a.G) * (a.Hkv * a.G) + hk * a.G + row % a.G) * a.D;
   store4<T>(op + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-  if (a.lse && tid == 0) a.lse[(int64_t)head * a.rows + row] = l == 0.f ? INFINITY : top + __builtin_amdgcn_logf(l);
+  if (a.lse && tid == 0) a.lse[(int64_t)head * a.rows + row] = l == 0.f ? (any ? NAN : INFINITY) : top + __builtin_amdgcn_logf(l);
 #endif
 }
 

@@ -398,7 +398,7 @@ int eve_scale_residual_bwd(const void* dout, const void* x, const void* gamma, c
 
 /* ------------------------------------------------ attention of the encoder layer, models/multiway_transformer.py:99-132
  * out[b,i,h] = sum_j p_ij v[b,j,h'], p = softmax_j(scale q[b,i,h] . k[b,j,h']) over the keys whose key_mask[b,j] is nonzero
- * (NULL: all); h' = h / (H / Hkv): query heads may share a key/value head.  A sample without a visible key gives zeros, and what
+ * (NULL: all); h' = h / (H / Hkv): query heads may share a key/value head.  A sample without a visible key gives zeros (visible scores that are all -inf: NaN), and what
  * a masked key or value row holds (NaN included) takes no part.  q [B,Nq,H,D], k and v [B,Nk,Hkv,D] lie anywhere with the last
  * dimension contiguous (strides below, in elements, multiples of 16 bytes; every pointer 16-byte aligned), so the three parts of
  * one qkv product are read where they are.  D is a multiple of 8 up to 128; 2^-100 <= scale <= 2^100.  out, dout: contiguous [B,Nq,H,D].

@@ -66,3 +66,32 @@ def test_a_gradient_that_is_no_number_stays_in_its_column_of_dv(way, bad):
     assert not bool(torch.isfinite(dv[1, :Nk - 2, 1][:, gone]).any())
     assert torch.equal(dv[1, :, 1][:, ~gone], clean[3][1, :, 1][:, ~gone])
     assert torch.equal(dv[:, :, 0], clean[3][:, :, 0]) and torch.equal(dk[:, :, 0], clean[2][:, :, 0])
+
+
+@pytest.mark.parametrize("way", WAYS, ids=lambda w: "x".join(map(str, w[:6])) + str(w[6])[6:])
+def test_rows_whose_visible_scores_are_all_minus_infinity(way):
+    """exp(-inf - max) with max = -inf is NaN; keys of score -inf beside others take no part; no visible key at all gives zeros."""
+    B, Nq, Nk, H, Hkv, D, dtype = way
+    q, k, v, do = _make(*way)
+    q = q.abs() + 0.1
+    mask = torch.ones(B, Nk, dtype=torch.bool, device=DEV)
+    mask[:, Nk - 2:] = False
+    half = Nk // 2
+    some = k.clone()
+    some[:, :half] = float("-inf")
+    got = eve_amd.attention(q, some, v, mask)
+    later = mask.clone()
+    later[:, :half] = False
+    want = eve_amd.attention(q, k, v, later)
+    eps = 4 * 2.0 ** -8 if dtype == BF16 else Nk * 2.0 ** -22  # tiles fall otherwise: each result is rounded p's and its own rounding off
+    assert bool(((got - want).float().abs() <= eps * (1 + v.float().abs().amax())).all())
+    k[1, :, 1] = float("-inf")
+    mask[0] = False
+    out, dq, dk, dv = _grads(q, k, v, do, mask)
+    mine = slice(H // Hkv, 2 * H // Hkv)
+    assert bool(torch.isnan(out[1][:, mine]).all()), "out"
+    assert bool(torch.isnan(dq[1][:, mine]).all()), "dq"
+    assert bool(torch.isnan(dk[1, :Nk - 2, 1]).all()) and bool(torch.isnan(dv[1, :Nk - 2, 1]).all()), "dk, dv"
+    assert bool(torch.isfinite(out[1][:, :H // Hkv]).all())
+    for t in (out[0], dq[0], dk[0], dv[0], dk[1, Nk - 2:], dv[1, Nk - 2:]):
+        assert float(t.abs().sum()) == 0.0
