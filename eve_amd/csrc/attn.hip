@@ -285,6 +285,43 @@ template <int KT, int NW> struct KeyBits {
   }
 };
 
+// Whether a sample sees so few keys that the backward forms delta as sum p dp: do . o sees the rounding of the stored result, which
+// is large next to what is left of the ds of a few keys (bf16, 5 keys, width 112: dq 1.8 % off; 2 keys of width 64: 0.4 % instead of
+// 0.2).  It goes by the keys that are seen, so that a sample's gradients do not depend on its padding.
+constexpr int kFewKeys = 64;
+// The same answer in all threads of NW waves; `scratch`: NW ints of LDS.  1024 keys and more a round, until enough are seen.
+template <int NW> struct FewKeys {
+  static constexpr int PER = 4;  // keys a thread and round
+  const uint8_t* mask;
+  int Nk, tid;
+  uint8_t first[PER];  // of the first round, requested early
+  __device__ __forceinline__ bool in(int key) const { return key < Nk && mask[key] != 0; }
+  __device__ __forceinline__ FewKeys(const uint8_t* mask, int Nk, int tid) : mask(mask), Nk(Nk), tid(tid) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) first[i] = mask && Nk > kFewKeys ? in(i * NW * 64 + tid) : 0;
+  }
+  __device__ __forceinline__ bool operator()(int* scratch) const {
+    if (Nk <= kFewKeys) return true;
+    if (!mask) return false;
+    int seen = 0;
+    for (int k0 = 0; k0 < Nk && seen <= kFewKeys; k0 += PER * NW * 64) {
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) mine += __popcll(__ballot(k0 == 0 ? first[i] : in(k0 + i * NW * 64 + tid)));
+      if (NW > 1) {
+        if ((tid & 63) == 0) scratch[tid >> 6] = mine;
+        __syncthreads();
+        mine = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) mine += scratch[w];
+        __syncthreads();
+      }
+      seen += mine;
+    }
+    return __builtin_amdgcn_readfirstlane(seen) <= kFewKeys;
+  }
+};
+
 // Pieces of 1 KiB of a tile, dealt to the NW waves; lane l of piece p holds chunk l % CPR of row p (64 / CPR) + l / CPR.
 template <typename C, int NW> struct TileLoader {
   static constexpr int N = C::TILE / 1024 / NW;  // a wave's transfers for a tile
@@ -575,11 +612,15 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
 }
 // -L / c and -delta as three bf16 each (a row that sees nothing: p = 2^(-1e30) = 0; NaN stays).  The matrix unit multiplies what it does
 // not add by zero, so that a delta that is no number would spoil p too: it is left out, as do . v is no number either in such a row.
-__device__ __forceinline__ uint4 row_stats(float L, float delta, float inv_c) {
-  uint32_t l0, l1, l2, d0, d1, d2;
-  split3((L > 1e30f ? 1e30f : L) * -inv_c, l0, l1, l2);
+__device__ __forceinline__ uint4 with_delta(const uint4& stats, float delta) {
+  uint32_t d0, d1, d2;
   split3(__builtin_fabsf(delta) < INFINITY ? -delta : 0.f, d0, d1, d2);
-  return make_uint4((l0 >> 16) | l1, (l2 >> 16) | d0, (d1 >> 16) | d2, 0);
+  return make_uint4(stats.x, (stats.y & 0xffffu) | d0, (d1 >> 16) | d2, 0);
+}
+__device__ __forceinline__ uint4 row_stats(float L, float delta, float inv_c) {
+  uint32_t l0, l1, l2;
+  split3((L > 1e30f ? 1e30f : L) * -inv_c, l0, l1, l2);
+  return with_delta(make_uint4((l0 >> 16) | l1, l2 >> 16, 0, 0), delta);
 }
 #endif
 
@@ -603,6 +644,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
   const int qi = row / a.G, qh = hk * a.G + row % a.G;
   const int64_t lrow = (int64_t)head * a.rows + row;
 
+  const FewKeys<NW> few_keys(sizeof(T) == 2 ? mask : nullptr, a.Nk, tid);
   uint4 qf[C::NKS], gf[C::NKS];  // q and do
   float L = INFINITY, delta = 0.f;
   {
@@ -622,6 +664,7 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
     delta = halves_sum(delta);
     if (row_ok) L = a.lse[lrow];
   }
+  const bool few = sizeof(T) == 2 && few_keys(reinterpret_cast<int*>(smem));
 
   const int ntiles = (a.Nk + C::KT - 1) / C::KT;
   const int t0 = split * a.tiles_per_split, t1 = min(ntiles, t0 + a.tiles_per_split);
@@ -637,23 +680,32 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
   uint64_t bits = keys.of(t0);
   fetch(t0, bits);
   if constexpr (sizeof(T) == 2) {
-    // All of a row's keys in one tile: delta is formed as sum p dp.  The result's rounding, which do . o sees, would be large next to
-    // what is left of ds where keys are few (5 keys, width 112: dq 1.8 % off).
-    if (ntiles == 1) {
-      tile_ready<0>();
+    if (few) {  // FewKeys: all of the sample's tiles, whatever the split; this split's first is on its way already
+      const KeyBits<C::KT, NW> all{mask, keys.words + kBitTiles, a.Nk, 0, ntiles, wave, lane};
       float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < C::NJ; ++j) {
-        at_f32x16 s = acc_zero(), dp = acc_zero();
-#pragma unroll
-        for (int ks = 0; ks < C::NKS; ++ks) {
-          s = mma(rows.get(smem, 0, j, ks), qf[ks], s, T());
-          dp = mma(rows.get(smem, C::TILE, j, ks), gf[ks], dp, T());
+      for (int t = 0; t < ntiles; ++t) {
+        const uint64_t b = all.of(t);
+        if (!b) continue;
+        const uint32_t at = t == t0 ? 0 : C::STAGE;
+        if (t != t0) {
+          __syncthreads();  // the stage's last tile has been read
+          kl.load(kb + (int64_t)t * C::KT * a.in.k_n, smem + at, wave_u, b);
+          vl.load(vb + (int64_t)t * C::KT * a.in.v_n, smem + at + C::TILE, wave_u, b);
         }
+        tile_ready<0>();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -L)) * dp[r];
-          sum += (bits >> (32 * j + (r & 3) + 8 * (r >> 2) + 4 * half)) & 1 ? x : 0.f;
+        for (int j = 0; j < C::NJ; ++j) {
+          at_f32x16 s = acc_zero(), dp = acc_zero();
+#pragma unroll
+          for (int ks = 0; ks < C::NKS; ++ks) {
+            s = mma(rows.get(smem, at, j, ks), qf[ks], s, T());
+            dp = mma(rows.get(smem, at + C::TILE, j, ks), gf[ks], dp, T());
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -L)) * dp[r];
+            sum += (b >> (32 * j + (r & 3) + 8 * (r >> 2) + 4 * half)) & 1 ? x : 0.f;
+          }
         }
       }
       delta = halves_sum(sum);
@@ -922,7 +974,7 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
   using C = AttnCfg<T, 64>;
   constexpr int NW = 8, KEYS = NW * 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr uint32_t kKeys = 0, kRing = KEYS * 128, kDs = kRing + 2 * C::STAGE, kHalf = kDs + KEYS * 128, kStats = kHalf + 4 * 4096;
+  constexpr uint32_t kKeys = 0, kRing = KEYS * 128, kDs = kRing + 2 * C::STAGE, kHalf = kDs + KEYS * 128, kStats = kHalf + 4 * 4096, kDelta = kStats + 2 * 1024;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, wave_u = __builtin_amdgcn_readfirstlane(wave);
   int head, blk, split;
   if (!block_coord(a, head, blk, split)) return;
@@ -999,6 +1051,10 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
   if (!wave_sees) {  // its part of ds stays zero
     for (int i = lane; i < 32 * 8; i += 64) *reinterpret_cast<uint4*>(smem + kDs + wave * 4096 + i * 16) = make_uint4(0, 0, 0, 0);
   }
+  float* part_delta = reinterpret_cast<float*>(smem + kDelta) + wave * 64;  // [wave][64 rows]; before the first tile: the wave's visible keys
+  const int wave_keys = __popcll(__ballot(see)) >> 1;  // (a key's column lies in both halves)
+  if (lane == 0) *part_delta = (float)wave_keys;
+  bool few = false;
   at_f32x16 dk[2], dv[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) dk[i] = dv[i] = acc_zero();
@@ -1038,6 +1094,46 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) *reinterpret_cast<at_u32x4*>(smem + kKeys + key * C::RB + half * 64 + c * 16) = at_u32x4{0, 0, 0, 0};
     }
+    if (t == 0) {
+      float seen = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) seen += reinterpret_cast<const float*>(smem + kDelta)[w * 64];
+      few = __builtin_amdgcn_readfirstlane(seen <= kFewKeys);
+    }
+    if (few) {  // FewKeys: delta of the tile's rows as sum p dp, over a wave's keys and then over the waves
+      __syncthreads();  // (tile 0: the counts have been read)
+      if (wave_sees) {
+#pragma unroll 1
+        for (int j = 0; j < 2; ++j) {
+          const uint4 both = lds16(st_ + (32 * j + (lane & 31)) * 16);
+          at_f32x16 s = acc_zero(), dp = acc_zero();
+#pragma unroll
+          for (int ks = 0; ks < C::NKS; ++ks) {
+            s = mma(rows.get(smem, qs_, j, ks), kf[ks], s, T());
+            dp = mma(rows.get(smem, gs_, j, ks), vf[ks], dp, T());
+          }
+          s = mma(both, one_L, s, T());
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float x = see ? __builtin_amdgcn_exp2f(s[r] * a.c) * dp[r] : 0.f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+            if ((lane & 31) == 0) part_delta[32 * j + (r & 3) + 8 * (r >> 2) + 4 * half] = x;
+          }
+        }
+      } else {
+        part_delta[lane] = 0.f;
+      }
+      __syncthreads();
+      if (tid < 64) {
+        float delta = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) delta += reinterpret_cast<const float*>(smem + kDelta)[w * 64 + tid];
+        uint4* st = reinterpret_cast<uint4*>(smem + kStats + (t & 1) * 1024) + tid;
+        *st = with_delta(*st, delta);
+      }
+      __syncthreads();
+    }
     stats_store(t + 1);
     stats_request(t + 2);
     if (t > 0 && !upper) dq_store(t - 1);
@@ -1045,12 +1141,14 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint4 both = lds16(st_ + (32 * j + (lane & 31)) * 16);
-        at_f32x16 s = mma(both, one_L, acc_zero(), T()), dp = mma(both, one_d, acc_zero(), T());
+        at_f32x16 s = acc_zero(), dp = acc_zero();
 #pragma unroll
         for (int ks = 0; ks < C::NKS; ++ks) {
           s = mma(rows.get(smem, qs_, j, ks), kf[ks], s, T());
           dp = mma(rows.get(smem, gs_, j, ks), vf[ks], dp, T());
         }
+        s = mma(both, one_L, s, T());  // last, as in attn_dkv_kernel
+        dp = mma(both, one_d, dp, T());
         ColFrags<T, C> f;  // of do, read while the matrix unit works
         f.read(smem, gs_, j, cols, lane);
 #pragma unroll
@@ -1121,7 +1219,7 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
     }
 #endif
 }
-constexpr int kWholeLds = 256 * 128 + 2 * AttnCfg<bf16_t, 64>::STAGE + 256 * 128 + 4 * 4096 + 2 * 1024;
+constexpr int kWholeLds = 256 * 128 + 2 * AttnCfg<bf16_t, 64>::STAGE + 256 * 128 + 4 * 4096 + 2 * 1024 + 8 * 256;
 
 // ---------------------------------------------------------------------------------------------------------- host
 namespace {
@@ -1246,6 +1344,7 @@ AttnArgs base_args(const eve_attn_shape& s) {
 
 // the ring, and behind it the mask's words or the rows' statistics
 template <typename C> constexpr int attn_lds() { return C::NST * C::STAGE + kBitTiles * 8; }
+template <typename C> constexpr int dq_lds() { return attn_lds<C>() + kBitTiles * 8; }  // and the words of the pass for delta
 template <typename T, int DP> constexpr int dkv_lds() { return AttnCfg<T, DP>::NST * (AttnCfg<T, DP>::STAGE + 1024); }
 
 int launch_attn(void (*kern)(AttnArgs), AttnArgs& a, int nw, int lds, hipStream_t st, const char* name) {
@@ -1302,7 +1401,7 @@ int bwd_typed(AttnArgs& a, bool whole, const AttnPlan& pq, const AttnPlan& pk, h
   }
   if (a.rows > 0) {
     use_plan(a, pq);
-    int rc = launch_attn(pq.nw == 1 ? attn_dq_kernel<T, DP, 1> : attn_dq_kernel<T, DP, 4>, a, pq.nw, attn_lds<AttnCfg<T, DP>>(), st, "eve_attn_bwd (dq)");
+    int rc = launch_attn(pq.nw == 1 ? attn_dq_kernel<T, DP, 1> : attn_dq_kernel<T, DP, 4>, a, pq.nw, dq_lds<AttnCfg<T, DP>>(), st, "eve_attn_bwd (dq)");
     if (rc == EVE_OK && a.nsplit > 1)
       rc = sum_parts<T>({{sum_of(a, a.part_a, a.dq, a.grad.q_b, a.grad.q_n, a.grad.q_h, a.G, a.rows, a.scale)}}, 1, st);
     if (rc != EVE_OK) return rc;
