@@ -39,9 +39,8 @@ template <int ACT, bool FAST> __device__ __forceinline__ float act_bwd(float z) 
   }
 }
 
-// Two elements at a time on v_pk_*_f32 (a wave's VALU issues one instruction per ~4 cycles whatever it is, so the
-// packed forms halve the issue time of the GEMM epilogues, which are bound by it): forward activation `a` and the
-// derivative `g` = act'(z) from ONE sigmoid.  The MFMA expert-FFN kernels save g (not z) for the backward pass,
+// Two elements at a time, as the GEMM epilogues hold them (the library is built without packed fp32 instructions: each
+// is computed by itself): forward activation `a` and the derivative `g` = act'(z) from ONE sigmoid.  The MFMA expert-FFN kernels save g (not z) for the backward pass,
 // whose epilogue is then a multiply: with t = z * (-1.702 log2 e), s = 1 / (1 + 2^t):
 //   a = z s,   g = s (1 + 1.702 z (1 - s)) = s + 1.702 (a - a s).
 typedef float f32x2_t __attribute__((ext_vector_type(2)));

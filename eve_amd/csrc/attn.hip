@@ -356,16 +356,21 @@ template <int NEWER> __device__ __forceinline__ void tile_ready() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// What the waves have written to LDS is seen by all of them (tiles on their way stay so).
+__device__ __forceinline__ void lds_exchange() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 // No transfer may be on its way into LDS when the workgroup ends.
 __device__ __forceinline__ void tiles_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 #endif  // __HIP_DEVICE_COMPILE__
 
 // ---------------------------------------------------------------------------------------------------------- forward
 // Block: NW waves of 32 rows each; the key tiles are staged for all of them.
-// Bound: the matrix unit and the vector unit, which hardly overlap in a CU: of a 64-key tile's 1400 cycles a wave the matrix unit
-// has 512, the vector unit 870 (the exponentials alone 530).  64 x 12 heads of 617 x 617: 121 us (620 TFLOP/s); 2 x 16 heads of
-// 4096 x 4096: 171 us (800), of width 128: 283 us (970).  One query of 4 x 16 heads on 4 over 16384 keys (NW = 1, 47 splits): 25 us,
-// 5.3 TB/s, the memory's rate.
+// Bound: the vector unit, busy for 74 % of a CU's cycles (250 instructions a wave and 64-key tile, the exponentials foremost; the
+// matrix unit 33 %).  64 x 12 heads of 617 x 617: 123 us (610 TFLOP/s); 2 x 16 heads of 4096 x 4096: 171 to 187 us (740 to 800; 72 % and
+// 42 %).  One query of 4 x 16 heads on 4 over 16384 keys (NW = 1, 47 splits): 25 us, 5.3 TB/s, the memory's rate.
 // The bounds on waves keep the register budget at 256, where the compiler holds accumulators in plain registers: in the larger
 // budget it moves them to and from accumulation registers, a third of the instructions of the loop.
 // (bf16 of width 65 to 128: tiles of 64 keys, half as many waits: 36 us instead of 41 for 3 x 16 heads on 4, 1001 x 1001.  The
@@ -626,7 +631,8 @@ __device__ __forceinline__ uint4 row_stats(float L, float delta, float inv_c) {
 
 // The forward's shape: columns are query rows, the key tiles pass by (or a split of them).  Also forms delta_i for the dk/dv
 // kernel.  -delta is the accumulator that the product do v^T starts from.
-// Bound as the forward (matrix unit 43 % busy, vector unit 47 %).  2 x 16 heads of 4096 x 4096: 240 us (860 TFLOP/s).
+// Bound: matrix and vector unit, 43 and 47 % busy, and a barrier a tile between them.  2 x 16 heads of 4096 x 4096: 245 to 265 us
+// (780 to 840 TFLOP/s).
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ? 1 : sizeof(T) == 2 && DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -784,9 +790,9 @@ __global__ __launch_bounds__(NW * 64, NW == 1 || (sizeof(T) == 4 && DP == 128) ?
 // p = 2^(c acc), ds = p acc'.  These terms are themselves a matrix product: a row's 16 bytes hold both values as three bf16 each
 // (exactly, 24 bits), which multiply ones; read as values, four at a time, they would be a third of the loop's LDS traffic.
 // A row past the end is all zeros: p = 1 there, and its q and do, which p and ds multiply, are zero.
-// Bound as the forward (matrix unit 51 % busy, vector unit 44 %).  2 x 16 heads of 4096 x 4096: 307 us (900 TFLOP/s); three
-// waves a SIMD instead of two change nothing.  Few live blocks (3 samples of 0 to 1001 keys, 16 heads on 4, width 128: 77 us) are
-// bound by a tile's way through the CU, 2.2 us.
+// Bound: matrix and vector unit, 51 and 44 % busy.  2 x 16 heads of 4096 x 4096: 312 to 339 us (810 to 880 TFLOP/s); three
+// waves a SIMD instead of two change nothing.  Few live blocks (3 samples of 0 to 1001 keys, 16 heads on 4, width 128: 78 us; the units
+// 23 and 19 % busy) are bound by a tile's way through the CU, 2.2 us.
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -966,8 +972,9 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 128 ? 1 : 2) void 
 // operand read once.  ds is exchanged between the waves through LDS as [key][64 rows]; a wave then multiplies one 32 x 32 block of
 // dq^T = k^T ds^T over half of the keys, and the two halves are added in a fixed order.  delta is formed from do and o by the
 // threads that a tile's rows are dealt to, one tile ahead.
-// Bound: latency.  64 x 12 heads of 237 x 237 take 82 us, the matrix unit is busy for 19 % of it: with 114 KiB and 226 registers a
-// CU holds one workgroup, and a head costs 11 k cycles before its first tile, then four times 7 k between two barriers each.
+// Bound: latency.  64 x 12 heads of 237 x 237 take 82 us, the matrix unit is busy for 19 % of it, the vector unit for 27: with 116 KiB
+// and 243 registers a CU holds one workgroup, and a head costs 11 k cycles before its first tile, then four times 7 k between two
+// barriers each.  A sample of few visible keys (FewKeys) takes three more barriers a tile: 87 us instead of 70 if all see 40 keys.
 __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef bf16_t T;
@@ -1052,9 +1059,8 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
     for (int i = lane; i < 32 * 8; i += 64) *reinterpret_cast<uint4*>(smem + kDs + wave * 4096 + i * 16) = make_uint4(0, 0, 0, 0);
   }
   float* part_delta = reinterpret_cast<float*>(smem + kDelta) + wave * 64;  // [wave][64 rows]; before the first tile: the wave's visible keys
-  const int wave_keys = __popcll(__ballot(see)) >> 1;  // (a key's column lies in both halves)
-  if (lane == 0) *part_delta = (float)wave_keys;
-  bool few = false;
+  const uint32_t wave_bits = (uint32_t)__ballot(see);  // (the other half holds the same keys)
+  if (lane == 0) *part_delta = (float)__popc(wave_bits);
   at_f32x16 dk[2], dv[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) dk[i] = dv[i] = acc_zero();
@@ -1062,6 +1068,11 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
   const uint4 one_d = half ? make_uint4(0, 0, 0, 0) : make_uint4(0, 0x3f800000u, 0x3f803f80u, 0);
   stats_store(0);
   stats_request(1);
+  lds_exchange();
+  int seen = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) seen += (int)reinterpret_cast<const float*>(smem + kDelta)[w * 64];
+  seen = __builtin_amdgcn_readfirstlane(seen);
 
   const int qblk = wave & 1, dblk = (wave >> 1) & 1, upper = wave_u >> 2;  // my block of dq^T, my half of the keys
   char* ds_at = smem + kDs + key * 128 + half * 8;
@@ -1085,7 +1096,7 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
       }
     }
   };
-  for (int t = 0; t < nt; ++t) {
+  auto tile = [&](int t, auto few) __attribute__((always_inline)) {
     const uint32_t qs_ = kRing + (t & 1) * C::STAGE, gs_ = qs_ + C::TILE;
     const char* st_ = smem + kStats + (t & 1) * 1024;
     tile_ready<0>();
@@ -1094,37 +1105,32 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) *reinterpret_cast<at_u32x4*>(smem + kKeys + key * C::RB + half * 64 + c * 16) = at_u32x4{0, 0, 0, 0};
     }
-    if (t == 0) {
-      float seen = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) seen += reinterpret_cast<const float*>(smem + kDelta)[w * 64];
-      few = __builtin_amdgcn_readfirstlane(seen <= kFewKeys);
-    }
-    if (few) {  // FewKeys: delta of the tile's rows as sum p dp, over a wave's keys and then over the waves
-      __syncthreads();  // (tile 0: the counts have been read)
+    if constexpr (decltype(few)::value) {  // FewKeys: delta of the tile's rows as sum p dp; operands swapped, so that a row is a lane and its keys are registers
       if (wave_sees) {
+        const uint32_t bits = wave_bits >> (4 * half);
 #pragma unroll 1
         for (int j = 0; j < 2; ++j) {
           const uint4 both = lds16(st_ + (32 * j + (lane & 31)) * 16);
           at_f32x16 s = acc_zero(), dp = acc_zero();
 #pragma unroll
           for (int ks = 0; ks < C::NKS; ++ks) {
-            s = mma(rows.get(smem, qs_, j, ks), kf[ks], s, T());
-            dp = mma(rows.get(smem, gs_, j, ks), vf[ks], dp, T());
+            s = mma(kf[ks], rows.get(smem, qs_, j, ks), s, T());
+            dp = mma(vf[ks], rows.get(smem, gs_, j, ks), dp, T());
           }
-          s = mma(both, one_L, s, T());
+          s = mma(one_L, both, s, T());
+          float sum = 0.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            float x = see ? __builtin_amdgcn_exp2f(s[r] * a.c) * dp[r] : 0.f;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-            if ((lane & 31) == 0) part_delta[32 * j + (r & 3) + 8 * (r >> 2) + 4 * half] = x;
+            const float x = __builtin_amdgcn_exp2f(s[r] * a.c) * dp[r];
+            sum += (bits >> ((r & 3) + 8 * (r >> 2))) & 1 ? x : 0.f;
           }
+          sum = halves_sum(sum);
+          if (half == 0) part_delta[32 * j + lane] = sum;
         }
       } else {
         part_delta[lane] = 0.f;
       }
-      __syncthreads();
+      lds_exchange();
       if (tid < 64) {
         float delta = 0.f;
 #pragma unroll
@@ -1132,7 +1138,7 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
         uint4* st = reinterpret_cast<uint4*>(smem + kStats + (t & 1) * 1024) + tid;
         *st = with_delta(*st, delta);
       }
-      __syncthreads();
+      lds_exchange();
     }
     stats_store(t + 1);
     stats_request(t + 2);
@@ -1178,9 +1184,7 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
           for (int i = 0; i < 2; ++i) dk[i] = mma(f.f[cc * 2 + i], ds[cc], dk[i], T());
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // ds is whole (the tiles on their way stay so)
-    asm volatile("" ::: "memory");
+    lds_exchange();  // ds is whole
     dq = acc_zero();
     const uint32_t ka = kKeys + upper * (KEYS / 2 * 128) + (cols.base[0] ^ (dblk << 6));
     const uint32_t da = kDs + upper * (KEYS / 2 * 128) + (cols.base[0] ^ (qblk << 6));
@@ -1195,6 +1199,11 @@ __global__ __launch_bounds__(512) void attn_bwd_whole_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) *reinterpret_cast<at_f32x4*>(part + i * 1024) = at_f32x4{dq[4 * i], dq[4 * i + 1], dq[4 * i + 2], dq[4 * i + 3]};
     }
+  };
+  if (seen <= kFewKeys) {
+    for (int t = 0; t < nt; ++t) tile(t, std::true_type());
+  } else {
+    for (int t = 0; t < nt; ++t) tile(t, std::false_type());
   }
   tile_ready<0>();
   if (nt > 0 && !upper) dq_store(nt - 1);
@@ -1240,6 +1249,9 @@ int attn_cus() {
 // How a kernel's rows (or keys) are cut into blocks, and the tiles that pass by them into splits.
 struct AttnPlan { int nw, nblk, tiles_per_split, nsplit; };
 
+// A split has four tiles at least.  Fewer would win where the whole launch is small and long (12 heads, one query, 1000 keys: 11.0 us, 8.1
+// with one tile; float32 6 heads, 129 on 333: 25 us, 19 with two) and lose where the join costs as much as a tile (12 heads of 237 x 237:
+// 8.0 us, 11.8 with two; 2 x 12 heads of 617, backward: 44 us, 48 with two, 39 with eight).
 AttnPlan plan_of(int64_t rows, int nw, int64_t heads, int64_t tiles, int64_t want_blocks, int64_t least_tiles) {
   AttnPlan p;
   p.nw = nw;
@@ -1275,9 +1287,12 @@ AttnPlan dkv_plan(const eve_attn_shape& s, int cus) {
   return plan_of(s.Nk, 4, (int64_t)s.B * s.Hkv, tiles_of(s.Nq, tile_rows(s)) * (s.H / s.Hkv), (int64_t)cus * 2, 4);
 }
 
-// The backward of whole heads, a workgroup each: where there is one for every other CU at least and their waves have keys.
-// (64 samples x 12 heads, 237 x 237: 80 us against 100 by the two kernels, which win where heads are few: 2 x 12 heads leave it
-// 24 workgroups.)
+// The backward of whole heads, a workgroup each: where there is one for every other CU at least and their waves have keys.  Times in us
+// of both ways, unmasked, width 64, heads x keys (whole | two kernels):
+//   32 x 237   20.7 | 21.0    128 x 237  23.2 | 24.3    256 x 237  27.6 | 35.1    768 x 237  75.3 | 92.4
+//   32 x 129   15.8 | 18.2    128 x 129  17.0 | 19.4    256 x 129  18.6 | 27.8    768 x 129  53.8 | 72.0
+//   32 x 64    15.4 | 11.9    128 x 100  12.7 | 15.9    256 x 100  13.9 | 17.6    768 x 100  39.3 | 38.9
+// (On fewer heads than cus / 2 it gains little.)
 bool whole_heads(const eve_attn_shape& s, int cus) {
   return s.dtype == EVE_BF16 && s.D <= 64 && s.Nk > 128 && s.Nk <= 256 && (int64_t)s.B * s.Hkv >= cus / 2;
 }

@@ -364,7 +364,7 @@ template <int PER> __device__ __forceinline__ void wait_tiles_in_flight(int tile
 }
 
 // Eight consecutive columns of one output row, read back from the staging image as two float4 (accumulator + bias),
-// finished two elements at a time on packed fp32 instructions (the activation epilogues are bound by the VALU's
+// finished two elements at a time (the activation epilogues are bound by the VALU's
 // instruction issue: in-kernel stamps put the conversions / activation of a half slab at the sum of both SIMD
 // partners' instruction counts x 4 cycles).
 //   MEPI_BIAS_ACT: out2 = a = act(z);  out1 = g = act'(z), what the backward pass needs of z -- saved in its place

@@ -12,9 +12,9 @@
 // linear_stream_kernel: rows on 16-byte boundaries.  Tiles of 192 x 128 (256 x 128 of a k-major A, 128 x 128 of smaller problems),
 // 4 waves, each half the rows and half the columns, so that five fragments feed six matrix instructions; steps of 64 bytes of the
 // contraction go from memory to LDS directly, two or three steps ahead: two workgroups a CU, one of which computes while the other
-// waits.  Bound: instruction issue.  39488 x 1024 -> 4096 takes 396 us (840 TFLOP/s; the vendor library's product 270), 435 with
-// quick_gelu, gamma and residual; the matrix unit is busy for 40 % of the cycles (a step takes 1070 for 768, a tile's epilogue 11 k
-// of 50 k), the clock falls to 1.6 GHz.  Reading fragments half a step ahead and 256-row tiles gained nothing.
+// waits.  Bound: instruction issue.  39488 x 1024 -> 4096 with quick_gelu, gamma and residual takes 438 us at best, 505 in the mean of
+// ten launches from a cold start (660 to 760 TFLOP/s; the vendor library's product alone 270 us); the matrix unit is busy for 40 % of the cycles.
+// Reading fragments half a step ahead and 256-row tiles gained nothing.
 // linear_tile_kernel: any size and alignment, and small problems; tiles of 128 or 64, staged through registers with every element
 // outside an operand replaced by zero.  Bound: latency and the matrix unit, a half each (float32, 1899 x 750 -> 1001: 46 us, 62 of
 // 138 TFLOP/s; the vendor library's product 35).
@@ -685,6 +685,7 @@ __global__ __launch_bounds__(256, 2) void linear_stream_kernel(LinArgs a) {
 #endif
 }
 
+#if defined(__HIP_DEVICE_COMPILE__)
 // the epilogue of one element
 template <typename T> __device__ __forceinline__ void lin_finish(const LinArgs& a, int m, int n, float v) {
   const int64_t at = (int64_t)m * a.N + n;
@@ -696,6 +697,7 @@ template <typename T> __device__ __forceinline__ void lin_finish(const LinArgs& 
   if (a.residual) v += to_f32<T>(static_cast<const T*>(a.residual)[at]);
   static_cast<T*>(a.C)[at] = from_f32<T>(v);
 }
+#endif
 
 // A few rows: one wave a column, the weight's row read once for all of them.
 template <typename T, int R>
@@ -1101,8 +1103,9 @@ BwdPlan bwd_plan(int rows, int K, int N, int dtype, int cus) {
   p.parts = ceil_div(rows, p.dz_rows);
   // dW [N, K]: the contraction over the rows is split until there are about two tiles of 256 x 128 a CU, 256 rows each at least; one
   // a CU if that leaves few idle and no more than 1280 rows a split, where the parts cost more than the company on a CU gives.  15168
-  // rows, 768 x 768 (18 tiles): 14 splits 30 us and 9 for the sums, 28 splits 30 and 11; 2304 x 768 (54): 4 splits 105 and 6 us,
-  // 9 splits 69 and 11; 8000 rows, 2047 x 1023 (64): 4 splits 215 us in all, 8 splits 180.
+  // rows, 768 x 768 (18 tiles): 14 splits 35 us with the sums, 28 splits 41; 2304 x 768 (54): 4 splits 105 and 6 us,
+  // 9 splits 69 and 11; off 16-byte boundaries, 8000 rows, 2047 x 1023 (64): 4 splits 215 us in all, 8 splits 180.  (The bound of 1280
+  // rows is for those: on 16-byte boundaries it changes little, 15168 rows, 2048 x 1024: 4 splits 80 us, 8 splits 81; 10000 rows: 61 and 63.)
   // (Float32 off 16-byte boundaries goes by its tiles of 128 x 128, as the matrix unit bounds it: 1899 rows, 1001 x 750: 5 splits 45 us
   // and 8, 6 splits 55 and 9; 8000 rows, 2047 x 1023: 4 splits 337 us in all, 8 splits 368.)
   const bool large = size == 2 || ((size_t)N * size % 16 == 0 && (size_t)K * size % 16 == 0);

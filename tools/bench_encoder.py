@@ -2,6 +2,7 @@
 BASELINE configs[1] shape: batch 64 x (197 vision + 40 text) tokens, bf16, one MI355X.
 
     python tools/bench_encoder.py            # eve_amd FFN paths (HIP kernels)
+    python tools/bench_encoder.py --attention both   # the same with stock and with fused attention in turn, training and evaluation
     python tools/bench_encoder.py --stock    # the reference's formulation of the FFN branches, issued with stock
                                              # PyTorch-ROCm ops on the same GPU (slice / cat, per-expert nn.Linear loop,
                                              # dense one-hot [S,E,C] dispatch / combine einsums)
@@ -23,6 +24,7 @@ ap.add_argument("--batch", type=int, default=64)
 ap.add_argument("--steps", type=int, default=10)
 ap.add_argument("--warmup", type=int, default=3)
 ap.add_argument("--layers", type=int, default=12)
+ap.add_argument("--attention", choices=("stock", "fused", "both"), default="stock")
 a = ap.parse_args()
 dev = torch.device("cuda", 0)
 torch.manual_seed(0)
@@ -122,14 +124,35 @@ def step():
     torch.autograd.backward([out, gl], [dout, torch.ones_like(gl)])
 
 
-for _ in range(a.warmup):
-    step()
-torch.cuda.synchronize()
-t0 = time.perf_counter()
-for _ in range(a.steps):
-    step()
-torch.cuda.synchronize()
-ms = (time.perf_counter() - t0) / a.steps * 1e3
+def timed(fn, n):
+    """-> (ms a call, ms of host time a call)"""
+    for _ in range(a.warmup):
+        fn()
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    for _ in range(n):
+        fn()
+    host = time.perf_counter() - t0
+    torch.cuda.synchronize()
+    return (time.perf_counter() - t0) / n * 1e3, host / n * 1e3
+
+
+if a.attention == "both":
+    for rep in range(3):
+        for impl in ("stock", "fused"):
+            enc.set_attention(impl)
+            enc.train()
+            torch.cuda.reset_peak_memory_stats()
+            ms, host = timed(step, a.steps)
+            peak = torch.cuda.max_memory_allocated() / 2**30
+            enc.eval()
+            with torch.no_grad():
+                ev = [timed(lambda: enc(x0[:b], mask[:b], mode="vl"), 2 * a.steps)[0] for b in (B, 1)]
+            print(f"attention {impl}: {ms:.2f} ms/step fwd+bwd (host {host:.2f}), peak {peak:.1f} GiB; evaluation {ev[0]:.2f} ms, one sample "
+                  f"{ev[1]:.2f} ms", flush=True)
+    sys.exit(0)
+enc.set_attention(a.attention)
+ms, _ = timed(step, a.steps)
 print(f"{'stock-ops reference formulation' if a.stock else 'eve_amd'}: {len(enc.layers)} layers, B={B}, T={T}, bf16: "
       f"{ms:.2f} ms/step fwd+bwd = {B * T / ms * 1e3 / 1e6:.3f} M tokens/s; peak memory "
       f"{torch.cuda.max_memory_allocated() / 2**30:.1f} GiB", flush=True)
