@@ -1,6 +1,6 @@
 // Diagnostic: issue cost of the VALU instructions the GEMM epilogues are made of, at one and at two waves per
 // SIMD (the epilogues run at two).  Not part of the library.
-//   hipcc --offload-arch=gfx950 -O3 tools/valu_rate.hip -o tools/valu_rate.bin
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/valu_rate.hip -o tools/valu_rate.bin
 // Each test is 64 independent chains x 16 rounds of one instruction between two s_memtime stamps; reported:
 // cycles per wave-instruction seen by one wave (so with two waves per SIMD the SIMD's rate is half that figure).
 #include <hip/hip_runtime.h>
@@ -21,15 +21,6 @@ __global__ __launch_bounds__(512) void k(float* out, unsigned* cyc, int rounds) 
     if constexpr (KIND == 0) {  // v_mul_f32
 #pragma unroll
       for (int i = 0; i < 16; ++i) asm volatile("v_mul_f32 %0, 0x3f7ff000, %0" : "+v"(v[i]));
-    } else if constexpr (KIND == 1) {  // v_pk_mul_f32
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        f2 a = {v[i], v[i + 1]};
-        asm volatile("v_pk_mul_f32 %0, %0, %1" : "+v"(a) : "v"(a));
-        asm volatile("v_pk_mul_f32 %0, %0, %1" : "+v"(a) : "v"(a));
-        v[i] = a.x; v[i + 1] = a.y;
-      }
     } else if constexpr (KIND == 2) {  // v_exp_f32
 #pragma unroll
       for (int i = 0; i < 16; ++i) asm volatile("v_exp_f32 %0, %0" : "+v"(v[i]));
@@ -42,15 +33,6 @@ __global__ __launch_bounds__(512) void k(float* out, unsigned* cyc, int rounds) 
     } else if constexpr (KIND == 5) {  // v_add_f32
 #pragma unroll
       for (int i = 0; i < 16; ++i) asm volatile("v_add_f32 %0, 1.0, %0" : "+v"(v[i]));
-    } else if constexpr (KIND == 6) {  // v_pk_fma_f32
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        f2 a = {v[i], v[i + 1]};
-        asm volatile("v_pk_fma_f32 %0, %0, %1, %1" : "+v"(a) : "v"(a));
-        asm volatile("v_pk_fma_f32 %0, %0, %1, %1" : "+v"(a) : "v"(a));
-        v[i] = a.x; v[i + 1] = a.y;
-      }
     } else if constexpr (KIND == 7) {  // the quick-GELU chain per element: mul, exp, add, rcp, mul (scalar forms)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -95,8 +77,6 @@ int main() {
   run<0>("v_mul_f32", 16);
   run<5>("v_add_f32", 16);
   run<8>("v_lshlrev_b32", 16);
-  run<1>("v_pk_mul_f32", 16);
-  run<6>("v_pk_fma_f32", 16);
   run<4>("v_cvt_pk_bf16_f32", 16);
   run<2>("v_exp_f32", 16);
   run<3>("v_rcp_f32", 16);
