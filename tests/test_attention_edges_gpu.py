@@ -99,3 +99,26 @@ def test_masks_of_more_tiles_than_are_held_at_a_time(B, Nq, Nk, H, D, dtype, kin
         at = slice(b, b + 1), slice(None), slice(h, h + 1)
         res = attention64(q[at], k[at], v[at], mask[b:b + 1], dout=do[at])
         assert_within(dict(zip(("out", "dq", "dk", "dv"), [t[at] for t in (out, *grads)])), res, f"sample {b}, head {h}")
+
+
+def _calls():
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).to(DEV)
+    x, w = r(2, 5, 16), r(24, 16)
+    qkv = r(2, 9, 3, 2, 16)
+    return {"attention": (lambda t: eve_amd.attention(*t.unbind(2)), qkv), "self_attention": (eve_amd.self_attention, qkv),
+            "fused_linear": (lambda t: eve_amd.fused_linear(t, w, activation="gelu"), x)}
+
+
+@pytest.mark.parametrize("name", ["attention", "self_attention", "fused_linear"])
+def test_second_derivatives_and_forward_mode_are_refused(name):
+    fn, x = _calls()[name]
+    x = x.requires_grad_(True)
+    dx, = torch.autograd.grad(fn(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+    import torch.autograd.forward_ad as fwad
+    with fwad.dual_level(), torch.no_grad():
+        dual = fwad.make_dual(x.detach(), torch.ones_like(x))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            fn(dual)
