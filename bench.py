@@ -441,7 +441,7 @@ def gemm_traffic(world, args, B):
     from eve_amd import _lib
     if not (world == 1 and args.dtype == "bf16" and args.model == "base" and B == 64):
         return None, None
-    for name in ("r03_gemm_traffic.json", "r02_gemm_traffic.json", "r01_gemm_traffic.json"):
+    for name in ("gemm_traffic.json", "r03_gemm_traffic.json", "r02_gemm_traffic.json", "r01_gemm_traffic.json"):
         path = os.path.join(REPO, "profiles", name)
         if not os.path.exists(path):
             continue

@@ -1,6 +1,6 @@
 """HBM-side traffic of the grouped-GEMM launches from two separate rocprofv3 --pmc passes (FETCH_SIZE, WRITE_SIZE).
 
-    python tools/gemm_traffic.py <dir of the FETCH_SIZE pass> <dir of the WRITE_SIZE pass> > profiles/rNN_gemm_traffic.json
+    python tools/gemm_traffic.py <dir of the FETCH_SIZE pass> <dir of the WRITE_SIZE pass> > profiles/gemm_traffic.json
 
 Corrections as /opt/skills/guides/MI355X_MICROARCH.md (HBM section) prescribes for gfx950: both counters are in KiB;
 FETCH_SIZE tallies the 128-byte requests of 16-byte-per-lane streaming reads (all of these kernels' operand fetches are
